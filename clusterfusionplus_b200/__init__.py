@@ -21,4 +21,7 @@ from .checkpoint import convert_state_dict, describe_config, load_decoder  # noq
 from .decoder import PythiaDecoder, rope_table  # noqa: F401
 from .llama import LlamaLayerStack  # noqa: F401
 from .quality import DecodeQuality, evaluate_decode_quality, step_metrics  # noqa: F401
+from .serving import (  # noqa: F401
+    PagedKvPlan, TokenLogprobs, kv4_append, kv4_attention, kv4_cache, kv4_read, paged_kv_plan, paged_kv_release, token_logprobs,
+)
 from .tp import TPDecoder, shard_cache, shard_dims, shard_head_weights, shard_layer_weights  # noqa: F401

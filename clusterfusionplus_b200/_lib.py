@@ -46,6 +46,8 @@ class CfDecoderConfig(C.Structure):
 
 
 CF_DECODER_GELU_ERF = 1
+CF_DTYPE_FP16, CF_DTYPE_BF16, CF_DTYPE_FP32 = 0, 1, 2
+CF_PLAN_NO_PAGES, CF_PLAN_TABLE_WIDTH, CF_PLAN_MAX_TOKENS, CF_PLAN_MAX_ROWS, CF_PLAN_BAD_LENGTH, CF_PLAN_BAD_PAGE = 1, 2, 4, 8, 16, 32
 CF_ACT_NONE, CF_ACT_GELU_TANH, CF_ACT_GELU_ERF = 0, 1, 2
 
 
@@ -105,6 +107,17 @@ SIGNATURES = {
                                     C.c_int64, C.c_int, C.c_void_p]),
     "cf_prefill_layernorm2": (C.c_int, [C.c_void_p] * 7 + [C.c_int64, C.c_int64, C.c_float, C.c_void_p]),
     "cf_prefill_rope_split": (C.c_int, [C.c_void_p] * 6 + [C.c_int64] * 5 + [C.c_void_p]),
+    "cf_paged_kv_plan": (C.c_int, [C.c_void_p] * 2 + [C.c_int64, C.c_void_p] + [C.c_int64] * 2 + [C.c_void_p, C.c_int64]
+                         + [C.c_void_p] * 2 + [C.c_int64] + [C.c_void_p] * 4 + [C.c_int64] + [C.c_void_p] * 2
+                         + [C.c_int64] + [C.c_void_p] * 2),
+    "cf_paged_kv_release": (C.c_int, [C.c_void_p] * 2 + [C.c_int64, C.c_void_p] + [C.c_int64] * 2 + [C.c_void_p, C.c_int64]
+                            + [C.c_void_p] * 2 + [C.c_int64] + [C.c_void_p] * 2),
+    "cf_kv4_append": (C.c_int, [C.c_void_p] * 2 + [C.c_int] + [C.c_int64] * 7 + [C.c_void_p] * 2 + [C.c_int64] * 2 + [C.c_void_p]),
+    "cf_kv4_read": (C.c_int, [C.c_void_p] + [C.c_int64] * 4 + [C.c_void_p, C.c_int64] + [C.c_void_p] * 2 + [C.c_int, C.c_void_p]),
+    "cf_kv4_attention": (C.c_int, [C.c_void_p, C.c_int] + [C.c_int64] * 5 + [C.c_void_p] + [C.c_int64] * 3 + [C.c_void_p]
+                         + [C.c_int64] * 2 + [C.c_void_p] * 2 + [C.c_int64] * 2 + [C.c_float] + [C.c_void_p] * 2),
+    "cf_token_logprobs": (C.c_int, [C.c_void_p, C.c_int] + [C.c_int64] * 3 + [C.c_void_p, C.c_int, C.c_int64]
+                          + [C.c_void_p] * 5),
 }
 
 

@@ -2,10 +2,10 @@
 
     python clusterfusionplus_b200/build.py [--force] [--verbose]
 
-Four translation units, compiled separately (objects cached under lib/obj/) and linked into one
+Seven translation units, compiled separately (objects cached under lib/obj/) and linked into one
 shared library: the decode kernel with the C ABI, the batched Llama decode blocks (hand-written
-tcgen05 skinny GEMMs + paged attention), the elementwise kernels of the prompt pass, and the tensor-core prefill
-GEMM, which is built from the CUTLASS / CuTe headers found in the Python environment (the `flashinfer` wheel
+tcgen05 skinny GEMMs + paged attention), the elementwise kernels of the prompt pass, the plan of a step over a
+paged cache, the cache held in 4 bits, the log probabilities of tokens, and the tensor-core prefill GEMM, which is built from the CUTLASS / CuTe headers found in the Python environment (the `flashinfer` wheel
 vendors them; set CUTLASS_INCLUDE to use another copy).  The library has no torch dependency;
 it links the CUDA runtime statically and finds the driver's tensor-map encoder at run time.
 """
@@ -30,6 +30,9 @@ UNITS = {
     "llama_batch.cu": (["llama_batch_kernel.cuh", "pipeline.cuh", "host_common.h", HEADER], False),
     "prefill_gemm.cu": (["prefill_gemm.h"], True),
     "prefill_ops.cu": (["host_common.h", HEADER], False),
+    "serve_plan.cu": (["host_common.h", HEADER], False),
+    "kv4_cache.cu": (["kv4_layout.cuh", "host_common.h", HEADER], False),
+    "logprobs.cu": (["host_common.h", HEADER], False),
 }
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

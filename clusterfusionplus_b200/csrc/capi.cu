@@ -869,12 +869,14 @@ int cf_get_status(int* status) {
         int s = 0;
         if ((rc = cf_host_lb_probe_status(ds->dev, &s))) return rc;
         if (s != 0) worst = s;
+        if ((rc = cf_host_kv4_probe_status(&s))) return rc;
+        if (s != 0) worst = s;
     }
     *status = worst;
     if (worst != 0)
         return fail(CF_ERR_DEVICE,
                     "device status %d (1-2 TMA ring, 3 grid barrier / flag wait, 4 cluster exchange, 5 bad seq_len, "
-                    "6 drain, 7 tensor-parallel peer never answered)",
+                    "6 drain, 7 tensor-parallel peer never answered, 8 page or slot outside the 4-bit cache)",
                     worst);
     return CF_OK;
 }

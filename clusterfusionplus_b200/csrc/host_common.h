@@ -15,3 +15,5 @@ int cf_host_fail(int code, const char* fmt, ...);
 int cf_host_refuse_in_capture(cudaStream_t st, const char* what);
 // status word of the batched Llama path on device `dev` (0 when unused); cleared when it was set
 int cf_host_lb_probe_status(int dev, int* status);
+// status word of the 4-bit cache's kernels on the current device (0 when unused); cleared when it was set
+int cf_host_kv4_probe_status(int* status);

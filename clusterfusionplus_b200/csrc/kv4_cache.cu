@@ -1,0 +1,313 @@
+// The paged cache held in 4 bits (layout: kv4_layout.cuh): rows written at their slots, rows read back, and attention over
+// it.  Asymmetric 4-bit codes over groups of 32 values of one token and head:
+//   m = fp16(min x), s = fp16((max x - m) / 15), code = clamp(rint((x - m) / s), 0, 15), value = code * s + m
+// x in fp32 (clamped to fp16's range, which bf16 exceeds); the codes are computed against the rounded s and m, so the rounding of
+// the parameters costs no accuracy but the last step's.  A group that is constant has s = 0 and code 0; one that holds a
+// NaN or whose extremes are not finite in the input stores NaN as its scale: it comes back as NaN instead of as numbers.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/clusterfusion_b200.h"
+#include "host_common.h"
+#include "kv4_layout.cuh"
+
+namespace {
+
+using namespace cfb;
+
+__device__ int g_kv4_status = 0;
+
+__device__ __forceinline__ void report_bad_slot() { atomicCAS(&g_kv4_status, 0, ST_BAD_SLOT); }
+
+template <class T> __device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <class T> __device__ __forceinline__ void load4(const T* p, float (&x)[4]) {
+    const uint2 raw = *reinterpret_cast<const uint2*>(p);
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = to_float<T>(e[i]);
+}
+template <class T> __device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
+    uint2 raw;
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = from_float<T>(x[i]);
+    *reinterpret_cast<uint2*>(p) = raw;
+}
+
+// codes of this lane's four values (16 bits), scale and minimum of its group; the eight lanes of a group work together
+__device__ __forceinline__ unsigned quantise4(const float (&x)[4], bool real, __half* scale, __half* low) {
+    float lo = 65504.f, hi = -65504.f, v[4];
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        finite &= !real || fabsf(x[i]) <= 3.4028234663852886e38f;  // false for NaN and the infinities
+        v[i] = fminf(fmaxf(x[i], -65504.f), 65504.f);
+        if (real) {
+            lo = fminf(lo, v[i]);
+            hi = fmaxf(hi, v[i]);
+        }
+    }
+    unsigned bad = !finite;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+    }
+    const __half m = __float2half_rn(lo);
+    const float mf = __half2float(m);
+    const __half s = __float2half_rn((hi - mf) / 15.f);
+    const float sf = __half2float(s);
+    unsigned codes = 0;
+    if (real && sf > 0.f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float c = rintf((v[i] - mf) / sf);
+            codes |= static_cast<unsigned>(fminf(fmaxf(c, 0.f), 15.f)) << (4 * i);
+        }
+    }
+    *scale = bad ? __ushort_as_half(0x7fff) : s;
+    *low = m;
+    return bad ? 0u : codes;
+}
+
+// One warp for a (token, head); lane l holds dims 4 l .. 4 l + 3 of the key and the value.
+template <class T>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ key, const T* __restrict__ value, const int* __restrict__ slot_map,
+                                                         uint8_t* __restrict__ cache, long long tokens, int heads, int D, int page, long long slots,
+                                                         long long k_ts, long long k_hs, long long v_ts, long long v_hs) {
+    const int G = kv4_groups(D), lane = threadIdx.x & 31;
+    const long long item = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+    if (item >= tokens * heads) return;
+    const long long tok = item / heads;
+    const int head = static_cast<int>(item - tok * heads);
+    const int slot = slot_map[tok];
+    if (slot < 0) return;  // a padded row
+    if (slot >= slots) {
+        if (lane == 0) report_bad_slot();
+        return;
+    }
+    const int dim = 4 * lane;
+    const bool real = dim < D, stored = dim < 32 * G;
+    float xk[4] = {0.f, 0.f, 0.f, 0.f}, xv[4] = {0.f, 0.f, 0.f, 0.f};
+    if (real) {
+        load4(key + tok * k_ts + head * k_hs + dim, xk);
+        load4(value + tok * v_ts + head * v_hs + dim, xv);
+    }
+    __half ks, km, vs, vm;
+    const unsigned kc = quantise4(xk, real, &ks, &km), vc = quantise4(xv, real, &vs, &vm);
+    if (!stored) return;
+    const int at = slot % page, row = at % KV4_TILE;
+    uint8_t* tile = cache + ((static_cast<long long>(slot / page) * heads + head) * (page / KV4_TILE) + at / KV4_TILE) * kv4_tile_bytes(G);
+    *reinterpret_cast<uint16_t*>(tile + kv4_key_half(G, row, dim)) = static_cast<uint16_t>(kc);
+    *reinterpret_cast<uint16_t*>(tile + kv4_value_half(G, row, dim)) = static_cast<uint16_t>(vc);
+    if ((lane & 7) < 4) {
+        const int which = lane & 3;
+        *reinterpret_cast<__half*>(tile + kv4_param(G, row, which, lane >> 3)) = which == 0 ? ks : which == 1 ? km : which == 2 ? vs : vm;
+    }
+}
+
+__device__ __forceinline__ void unpack4(unsigned codes, float s, float m, float (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = fmaf(static_cast<float>((codes >> (4 * i)) & 15u), s, m);
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ slot_map, T* __restrict__ key,
+                                                       T* __restrict__ value, long long tokens, int heads, int D, int page, long long slots) {
+    const int G = kv4_groups(D), lane = threadIdx.x & 31;
+    const long long item = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+    if (item >= tokens * heads) return;
+    const long long tok = item / heads;
+    const int head = static_cast<int>(item - tok * heads);
+    const int slot = slot_map[tok], dim = 4 * lane;
+    if (dim >= D) return;
+    float xk[4] = {0.f, 0.f, 0.f, 0.f}, xv[4] = {0.f, 0.f, 0.f, 0.f};
+    if (slot >= 0 && slot < slots) {
+        const int at = slot % page, row = at % KV4_TILE, g = lane >> 3;
+        const uint8_t* tile = cache + ((static_cast<long long>(slot / page) * heads + head) * (page / KV4_TILE) + at / KV4_TILE) * kv4_tile_bytes(G);
+        auto par = [&](int which) { return __half2float(*reinterpret_cast<const __half*>(tile + kv4_param(G, row, which, g))); };
+        unpack4(*reinterpret_cast<const uint16_t*>(tile + kv4_key_half(G, row, dim)), par(0), par(1), xk);
+        unpack4(*reinterpret_cast<const uint16_t*>(tile + kv4_value_half(G, row, dim)), par(2), par(3), xv);
+    } else if (slot >= slots && lane == 0) {
+        report_bad_slot();
+    }
+    store4(key + (tok * heads + head) * D + dim, xk);
+    store4(value + (tok * heads + head) * D + dim, xv);
+}
+
+struct AttnArgs {
+    const void* query;
+    const uint8_t* cache;
+    const int* table;
+    const int* kv_lens;
+    const int* qo_indptr;  // null: one query a request
+    void* out;
+    long long q_ts, q_hs, table_stride, table_width, rows;
+    int batch, heads, kv_heads, D, page, pages;
+    float scale_log2;
+};
+
+// The plainest form: one warp for a (query row, head), keys one after another, the running maximum and sum of the softmax.
+template <class T>
+__global__ void __launch_bounds__(128) kv4_attention_kernel(const AttnArgs a) {
+    const int lane = threadIdx.x & 31, G = kv4_groups(a.D), dim = 4 * lane;
+    const long long item = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+    if (item >= a.rows * a.heads) return;
+    const long long row = item / a.heads;
+    const int head = static_cast<int>(item - row * a.heads), kvh = head / (a.heads / a.kv_heads);
+    int b = static_cast<int>(row), first = b, count = 1;
+    if (a.qo_indptr) {
+        if (row < a.qo_indptr[0] || row >= a.qo_indptr[a.batch]) return;  // rows of no request stay as they were
+        int lo = 0, hi = a.batch;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.qo_indptr[mid] <= row) lo = mid;
+            else hi = mid;
+        }
+        b = lo;
+        first = a.qo_indptr[b];
+        count = a.qo_indptr[b + 1] - first;
+    } else if (row >= a.batch) return;
+    const bool real = dim < a.D;
+    float q[4] = {0.f, 0.f, 0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+    if (real) load4(static_cast<const T*>(a.query) + row * a.q_ts + head * a.q_hs + dim, q);
+    const long long cap = a.table_width * a.page;
+    const long long seen = min(static_cast<long long>(a.kv_lens[b]) - count + (row - first) + 1, cap);
+    for (long long p = 0; p < seen; ++p) {
+        const int held = a.table[b * a.table_stride + p / a.page];
+        if (held < 0 || held >= a.pages) {
+            if (lane == 0) report_bad_slot();
+            continue;
+        }
+        const int at = static_cast<int>(p % a.page), r = at % KV4_TILE, g = lane >> 3;
+        const uint8_t* tile = a.cache + ((static_cast<long long>(held) * a.kv_heads + kvh) * (a.page / KV4_TILE) + at / KV4_TILE) * kv4_tile_bytes(G);
+        float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (real) {
+            auto par = [&](int which) { return __half2float(*reinterpret_cast<const __half*>(tile + kv4_param(G, r, which, g))); };
+            unpack4(*reinterpret_cast<const uint16_t*>(tile + kv4_key_half(G, r, dim)), par(0), par(1), k);
+            unpack4(*reinterpret_cast<const uint16_t*>(tile + kv4_value_half(G, r, dim)), par(2), par(3), v);
+        }
+        float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+        s *= a.scale_log2;
+        const float top = fmaxf(m, s), ref = top == -INFINITY ? 0.f : top;
+        const float keep = exp2f(m - ref), e = exp2f(s - ref);
+        l = l * keep + e;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = o[i] * keep + e * v[i];
+        m = top;
+    }
+    if (!real) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = l > 0.f ? o[i] / l : (l == 0.f ? 0.f : l);  // no key seen: zeros; NaN stays NaN
+    store4(static_cast<T*>(a.out) + (row * a.heads + head) * a.D + dim, o);
+}
+
+int check_cache(int64_t pages, int64_t kv_heads, int64_t page, int64_t D) {
+    if (D < 16 || D > KV4_MAX_DIM || D % 8 != 0) return cf_host_fail(CF_ERR_INVALID, "head_dim %lld must be a multiple of 8 in 16..%d", (long long)D, KV4_MAX_DIM);
+    if (page < KV4_TILE || page % KV4_TILE != 0 || page > 65536) return cf_host_fail(CF_ERR_INVALID, "page size %lld must be a multiple of %d, at most 65536", (long long)page, KV4_TILE);
+    if (pages < 1 || kv_heads < 1 || kv_heads > 1024 || pages > 0x7fffffff / page)
+        return cf_host_fail(CF_ERR_INVALID, "cache of %lld pages of %lld rows, %lld heads (at most 2^31 - 1 rows)", (long long)pages, (long long)page, (long long)kv_heads);
+    return CF_OK;
+}
+
+int check_launch(const char* what) {
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cf_host_fail(CF_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
+    return CF_OK;
+}
+
+bool aligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+}  // namespace
+
+int cf_host_kv4_probe_status(int* status) {
+    *status = 0;
+    const int zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(status, g_kv4_status, sizeof(int));
+    if (e == cudaSuccess && *status != 0) e = cudaMemcpyToSymbol(g_kv4_status, &zero, sizeof(int));
+    if (e != cudaSuccess) return cf_host_fail(CF_ERR_CUDA, "4-bit cache status: %s", cudaGetErrorString(e));
+    return CF_OK;
+}
+
+extern "C" {
+
+int cf_kv4_append(const void* key, const void* value, int dtype, int64_t tokens, int64_t kv_heads, int64_t head_dim, int64_t key_token_stride,
+                  int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride, const int* slot_map, void* cache, int64_t pages,
+                  int64_t page_size, void* stream) {
+    if (int rc = check_cache(pages, kv_heads, page_size, head_dim)) return rc;
+    if (dtype != CF_DTYPE_FP16 && dtype != CF_DTYPE_BF16) return cf_host_fail(CF_ERR_INVALID, "dtype %d is neither fp16 nor bf16", dtype);
+    if (tokens < 0 || tokens > 0x7fffffff) return cf_host_fail(CF_ERR_INVALID, "tokens %lld", (long long)tokens);
+    if (tokens == 0) return CF_OK;
+    if (!key || !value || !slot_map || !cache) return cf_host_fail(CF_ERR_INVALID, "null pointer");
+    if (!aligned(key, 8) || !aligned(value, 8) || !aligned(cache, 16) || (key_token_stride | key_head_stride | value_token_stride | value_head_stride) % 4 != 0)
+        return cf_host_fail(CF_ERR_INVALID, "keys and values need 8-byte aligned rows (strides in multiples of 4 elements), the cache 16 bytes");
+    const int64_t warps = tokens * kv_heads, grid = (warps + 7) / 8;
+    if (grid > 0x7fffffff) return cf_host_fail(CF_ERR_INVALID, "%lld tokens of %lld heads in one call", (long long)tokens, (long long)kv_heads);
+    auto go = [&](auto* k, auto kernel) {
+        kernel<<<static_cast<unsigned>(grid), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+            k, static_cast<decltype(k)>(value), slot_map, static_cast<uint8_t*>(cache), tokens, static_cast<int>(kv_heads), static_cast<int>(head_dim),
+            static_cast<int>(page_size), pages * page_size, key_token_stride, key_head_stride, value_token_stride, value_head_stride);
+    };
+    if (dtype == CF_DTYPE_FP16) go(static_cast<const __half*>(key), kv4_append_kernel<__half>);
+    else go(static_cast<const __nv_bfloat16*>(key), kv4_append_kernel<__nv_bfloat16>);
+    return check_launch("4-bit append");
+}
+
+int cf_kv4_read(const void* cache, int64_t pages, int64_t page_size, int64_t kv_heads, int64_t head_dim, const int* slot_map, int64_t tokens, void* key,
+                void* value, int dtype, void* stream) {
+    if (int rc = check_cache(pages, kv_heads, page_size, head_dim)) return rc;
+    if (dtype != CF_DTYPE_FP16 && dtype != CF_DTYPE_BF16) return cf_host_fail(CF_ERR_INVALID, "dtype %d is neither fp16 nor bf16", dtype);
+    if (tokens < 0 || tokens > 0x7fffffff) return cf_host_fail(CF_ERR_INVALID, "tokens %lld", (long long)tokens);
+    if (tokens == 0) return CF_OK;
+    if (!key || !value || !slot_map || !cache) return cf_host_fail(CF_ERR_INVALID, "null pointer");
+    if (!aligned(key, 16) || !aligned(value, 16) || !aligned(cache, 16)) return cf_host_fail(CF_ERR_INVALID, "storage must be 16-byte aligned");
+    const int64_t warps = tokens * kv_heads, grid = (warps + 7) / 8;
+    if (grid > 0x7fffffff) return cf_host_fail(CF_ERR_INVALID, "%lld tokens of %lld heads in one call", (long long)tokens, (long long)kv_heads);
+    auto go = [&](auto* k, auto kernel) {
+        kernel<<<static_cast<unsigned>(grid), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+            static_cast<const uint8_t*>(cache), slot_map, k, static_cast<decltype(k)>(value), tokens, static_cast<int>(kv_heads), static_cast<int>(head_dim),
+            static_cast<int>(page_size), pages * page_size);
+    };
+    if (dtype == CF_DTYPE_FP16) go(static_cast<__half*>(key), kv4_read_kernel<__half>);
+    else go(static_cast<__nv_bfloat16*>(key), kv4_read_kernel<__nv_bfloat16>);
+    return check_launch("4-bit read");
+}
+
+int cf_kv4_attention(const void* query, int dtype, int64_t rows, int64_t heads, int64_t head_dim, int64_t query_token_stride, int64_t query_head_stride,
+                     const void* cache, int64_t pages, int64_t page_size, int64_t kv_heads, const int* block_table, int64_t table_width,
+                     int64_t table_stride, const int* kv_lens, const int* qo_indptr, int64_t batch, int64_t max_q_len, float scale, void* out,
+                     void* stream) {
+    if (int rc = check_cache(pages, kv_heads, page_size, head_dim)) return rc;
+    if (dtype != CF_DTYPE_FP16 && dtype != CF_DTYPE_BF16) return cf_host_fail(CF_ERR_INVALID, "dtype %d is neither fp16 nor bf16", dtype);
+    if (heads < kv_heads || heads % kv_heads != 0) return cf_host_fail(CF_ERR_INVALID, "%lld query heads over %lld cached heads", (long long)heads, (long long)kv_heads);
+    if (rows < 0 || rows > 0x7fffffff || batch < 1 || batch > 0x7fffffff || max_q_len < 1)
+        return cf_host_fail(CF_ERR_INVALID, "rows %lld, batch %lld, max_q_len %lld", (long long)rows, (long long)batch, (long long)max_q_len);
+    if (!qo_indptr && rows < batch) return cf_host_fail(CF_ERR_INVALID, "%lld query rows for %lld requests", (long long)rows, (long long)batch);
+    if (table_width < 1 || table_stride < table_width || table_width > 0x7fffffff) return cf_host_fail(CF_ERR_INVALID, "block table of %lld columns, %lld entries apart", (long long)table_width, (long long)table_stride);
+    if (rows == 0) return CF_OK;
+    if (!query || !cache || !block_table || !kv_lens || !out) return cf_host_fail(CF_ERR_INVALID, "null pointer");
+    if (!aligned(query, 16) || !aligned(out, 16) || !aligned(cache, 16) || (query_token_stride | query_head_stride) % 8 != 0)
+        return cf_host_fail(CF_ERR_INVALID, "queries need 16-byte aligned rows (strides in multiples of 8 elements), cache and output 16 bytes");
+    const AttnArgs a{query, static_cast<const uint8_t*>(cache), block_table, kv_lens, qo_indptr, out, query_token_stride, query_head_stride, table_stride, table_width, rows,
+                     static_cast<int>(batch), static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(head_dim), static_cast<int>(page_size),
+                     static_cast<int>(pages), scale * 1.4426950408889634f};
+    const int64_t grid = (rows * heads + 3) / 4;
+    if (grid > 0x7fffffff) return cf_host_fail(CF_ERR_INVALID, "%lld query rows of %lld heads in one call", (long long)rows, (long long)heads);
+    if (dtype == CF_DTYPE_FP16) kv4_attention_kernel<__half><<<static_cast<unsigned>(grid), 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    else kv4_attention_kernel<__nv_bfloat16><<<static_cast<unsigned>(grid), 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    return check_launch("4-bit attention");
+}
+
+}  // extern "C"

@@ -15,6 +15,7 @@ import torch.nn.functional as F
 from . import _lib
 from ._lib import CF_ACT_GELU_ERF, CF_ACT_GELU_TANH, CF_ACT_NONE, CF_DECODER_GELU_ERF, CfDecoderConfig, CfDims, CfHeadWeights, CfLayerWeights, check, lib
 from .api import _req, _wrap
+from .serving import TokenLogprobs, token_logprobs
 
 _LAYER_KEYS = {
     "qkv_weight": "qkv_weight", "qkv_bias": "qkv_bias", "o_weight": "o_weight", "o_bias": "o_bias",
@@ -165,11 +166,16 @@ class PythiaDecoder:
         leaves it to the HuggingFace model (tests/benchmark_full.py:195-199).  The decoder is
         then positioned on the last prompt token, so the next step() consumes it through the
         fused decode kernel and yields the first generated token."""
+        self._ingest(tokens)
+
+    def _ingest(self, tokens: Sequence[int]):
+        """The work of prefill(): (token ids on the device, hidden states of all but the last before the final norm)."""
         ids = torch.as_tensor(list(tokens), dtype=torch.long, device=self.device)
         n = int(ids.numel())
         if n < 1 or n > self.max_seq - 1:
             raise RuntimeError(f"prompt of {n} tokens does not fit {self.max_seq} cache rows")
         m = n - 1
+        x = None
         if m > 0:
             d = self.dims
             H, NH, D, R = d.hidden, d.heads, d.head_dim, d.rotary
@@ -199,6 +205,28 @@ class PythiaDecoder:
                 h = prefill_linear(attn, w["o_weight"], w["o_bias"], residual=x)
                 x = prefill_linear(mid, w["mlp_down_weight"], w["mlp_down_bias"], residual=h)
         self.reset(m, int(ids[-1].item()))
+        return ids, x
+
+    @torch.no_grad()
+    def score(self, tokens: Sequence[int], top_k: int = 0) -> TokenLogprobs:
+        """prefill(tokens), and the log probabilities of tokens[1:] given what precedes each, the entropy of every prediction
+        and its top_k alternatives (token_logprobs; len(tokens) - 1 rows).  The logits of the prompt are fp16, as the LM head's
+        tensor-core product leaves them: a log probability is off by up to half an fp16 step of the logits (4e-3 at
+        logits of 8 to 16); those of step() are fp32.  The vocabulary has to be a multiple of 8."""
+        ids, x = self._ingest(tokens)
+        d = self.dims
+        if x is None:
+            none = torch.empty(0, dtype=torch.float32, device=self.device)
+            return TokenLogprobs(none, none, none.new_empty(0, int(top_k)), torch.empty(0, int(top_k), dtype=torch.int64, device=self.device))
+        y = torch.empty_like(x)
+        h = self.head
+        check(lib.cf_prefill_layernorm2(x.data_ptr(), _req(h["final_ln_weight"], "final_ln_weight", d.hidden),
+                                        _req(h["final_ln_bias"], "final_ln_bias", d.hidden), None, None, y.data_ptr(), None, x.shape[0],
+                                        d.hidden, 1e-5, torch.cuda.current_stream().cuda_stream))
+        # 2048 rows of logits at a time (206 MB for a vocabulary of 50304)
+        parts = [token_logprobs(prefill_linear(y[i:i + 2048], h["embed_out"]), ids[1 + i:1 + i + 2048], top_k)
+                 for i in range(0, y.shape[0], 2048)]
+        return TokenLogprobs(*(torch.cat(p) for p in zip(*parts)))
 
     def generate_from_prompt(self, tokens: Sequence[int], n_tokens: int) -> List[int]:
         """prefill(tokens), then n_tokens greedy steps; returns the generated ids."""

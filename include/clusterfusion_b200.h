@@ -86,7 +86,8 @@ int cf_launch_info(int model, int* sm_count, int* grid, int* cluster, int* stage
  * (synchronises the device) -- clears what was set and re-arms the barrier words.
  * *status = 0 when every launch so far finished normally; otherwise the call returns
  * CF_ERR_DEVICE and *status is 1-2 TMA ring, 3 grid barrier / flag wait, 4 cluster exchange,
- * 5 bad seq_len, 6 drain, 7 tensor-parallel peer never answered. */
+ * 5 bad seq_len, 6 drain, 7 tensor-parallel peer never answered, 8 a page or slot outside the
+ * 4-bit cache (its rows were skipped). */
 int cf_get_status(int* status);
 
 /* Fused decoder layer, one token at batch 1.  The first call with a given set of tensors
@@ -393,6 +394,94 @@ int cf_prefill_layernorm2(const void* x, const void* gamma1, const void* beta1, 
                           void* y1, void* y2, int64_t m, int64_t hidden, float eps, void* stream);
 int cf_prefill_rope_split(const void* qkv, const float* cos, const float* sin, void* q_out, void* k_rows, void* v_rows,
                           int64_t m, int64_t heads, int64_t head_dim, int64_t rotary, int64_t kv_row_stride, void* stream);
+
+/* -------------------------------------------------------------------------
+ * Serving a batch over a paged cache.  The reference's batched entry point takes page lists that its caller (a serving
+ * framework) builds, keeps its cache in fp16 and leaves sampling to the caller
+ * (include/5090/llama/llama_kernel_batch_sglang_dispatch.cu:6-111); these calls are additions.  None of them allocates,
+ * synchronises or keeps state between calls, so all can be captured and calls on different streams may overlap as
+ * long as their tensors do not.  They launch at once; cf_batch_begin does not record them.
+ * ------------------------------------------------------------------------- */
+#define CF_DTYPE_FP16 0
+#define CF_DTYPE_BF16 1
+#define CF_DTYPE_FP32 2
+
+/* Bits of the status word of a plan or a release. */
+#define CF_PLAN_NO_PAGES 1     /* plan: the free list holds too few pages; release: it has no room */
+#define CF_PLAN_TABLE_WIDTH 2  /* a request needs more pages than the block table has columns */
+#define CF_PLAN_MAX_TOKENS 4   /* more new tokens than max_tokens */
+#define CF_PLAN_MAX_ROWS 8     /* more cached rows than max_rows (max_rows = 0: than 2^31 - 1) */
+#define CF_PLAN_BAD_LENGTH 16  /* a negative length, or a request of more than 2^31 - 1 tokens */
+#define CF_PLAN_BAD_PAGE 32    /* release: a table entry below 0 among the pages to be released */
+
+/* Plans one step: request b holds cached_lens[b] tokens and gets new_lens[b] more (both int32 [batch], batch 1..4096; 0 is
+ * fine).  Pages of page_size tokens (1..65536) that this takes come from the top of the free list: free_pages[0 .. *free_count)
+ * are free page numbers, request by request and column by column the topmost is taken next.  Writes
+ *   block_table  int32 [batch][table_stride], table_width columns: the entries of the fresh pages (nothing else)
+ *   *free_count_out  what is left of the list (must not alias free_count; pass it as free_count of the next step)
+ *   kv_lens      int32 [batch]: cached + new (must not alias the lengths read)
+ *   qo_indptr    int32 [batch + 1]: first new token of each request among all new tokens
+ *   positions    int64 [max_tokens], slot_map int32 [max_tokens]: position in its request and row in the cache of every
+ *                new token (row = page * page_size + position % page_size); behind the last token 0 and -1
+ *   kv_indptr    int32 [batch + 1], kv_indices int32 [max_rows]: the cache rows of every request, all cached + new of them,
+ *                as cf_llama_decoder_layer_batch_sglang reads them; behind the last row -1.  max_rows = 0: only kv_indptr.
+ *                kv_indices must be 16-byte aligned.
+ *   *status      0, or CF_PLAN_* bits.  All or nothing: with a bit set the table and the count stay as they are, kv_lens =
+ *                cached_lens, the indptr arrays are 0 and the lists empty (0 / -1).
+ * A table entry below 0, or a row beyond 2^31 - 1, gives -1 in the lists.  Page numbers are not checked against a pool. */
+int cf_paged_kv_plan(const int* cached_lens, const int* new_lens, int64_t batch, int* block_table, int64_t table_width,
+                     int64_t table_stride, const int* free_pages, int64_t n_free_pages, const int* free_count,
+                     int* free_count_out, int64_t page_size, int* kv_lens, int* qo_indptr, int64_t* positions, int* slot_map,
+                     int64_t max_tokens, int* kv_indptr, int* kv_indices, int64_t max_rows, int* status, void* stream);
+
+/* Gives the pages of the requests with finished[b] != 0 (int32 [batch]) back: the first ceil(kv_lens[b] / page_size) entries
+ * of their table rows go on top of the free list (capacity n_free_pages) in request and column order and become -1.
+ * *free_count_out as above.  All or nothing, *status as above. */
+int cf_paged_kv_release(const int* finished, const int* kv_lens, int64_t batch, int* block_table, int64_t table_width,
+                        int64_t table_stride, int* free_pages, int64_t n_free_pages, const int* free_count, int* free_count_out,
+                        int64_t page_size, int* status, void* stream);
+
+/* The paged cache held in 4 bits: uint8 [pages][kv_heads][page_size][40 * G], G = ceil(head_dim / 32), page_size a multiple
+ * of 16, head_dim a multiple of 8 in 16..128, at most 2^31 - 1 rows, 16-byte aligned.  Every 32 values of one token and head
+ * (the last group of a head may be shorter) share an fp16 minimum m and an fp16 scale s = (max - m) / 15; a value is
+ * code * s + m with code = rint((x - m) / s) in 0..15 (x clamped to fp16's range; a group holding a NaN or an infinity reads
+ * back as NaN).  The order of the codes inside a page is described in csrc/kv4_layout.cuh.  Row r of the cache is token
+ * r % page_size of page r / page_size.
+ *
+ * cf_kv4_append writes token i's keys and values, [tokens][kv_heads][head_dim] with the given strides (elements; multiples
+ * of 4, the last axis contiguous), to row slot_map[i].  A row below 0 is skipped; one beyond the cache is skipped and
+ * recorded (cf_get_status 8).  Two tokens of a call must not name the same row (its content would be a mixture).
+ * cf_kv4_read writes the values of rows slot_map[0 .. tokens) to key and value [tokens][kv_heads][head_dim] contiguous;
+ * zeros for a row below 0 or beyond the cache (the latter recorded).  dtype: CF_DTYPE_FP16 or CF_DTYPE_BF16. */
+int cf_kv4_append(const void* key, const void* value, int dtype, int64_t tokens, int64_t kv_heads, int64_t head_dim,
+                  int64_t key_token_stride, int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride,
+                  const int* slot_map, void* cache, int64_t pages, int64_t page_size, void* stream);
+int cf_kv4_read(const void* cache, int64_t pages, int64_t page_size, int64_t kv_heads, int64_t head_dim, const int* slot_map,
+                int64_t tokens, void* key, void* value, int dtype, void* stream);
+
+/* Causal attention over that cache.  query [rows][heads][head_dim] (fp16 or bf16; strides in elements, multiples of 8, last
+ * axis contiguous), out [rows][heads][head_dim] contiguous, heads a multiple of kv_heads (query head h reads cached head
+ * h / (heads / kv_heads)).  Request b owns query rows qo_indptr[b] .. qo_indptr[b + 1) (int32 [batch + 1], ascending; NULL: row
+ * b); they are its last tokens: of n queries and kv_lens[b] cached tokens, query i sees the first kv_lens[b] - n + i + 1
+ * tokens, which lie in the pages block_table[b][0 ..].  A query that sees no token gives zeros.  Rows of out that no
+ * request owns stay as they are.  A page number outside the cache is skipped as if its tokens were not there, and recorded
+ * (cf_get_status 8); tokens beyond table_width pages are not there either.  max_q_len: the most query rows a request
+ * has, for the choice and the size of the launch; the result does not depend on it.  scale: of q . k (1 / sqrt(head_dim)
+ * as a rule). */
+int cf_kv4_attention(const void* query, int dtype, int64_t rows, int64_t heads, int64_t head_dim, int64_t query_token_stride,
+                     int64_t query_head_stride, const void* cache, int64_t pages, int64_t page_size, int64_t kv_heads,
+                     const int* block_table, int64_t table_width, int64_t table_stride, const int* kv_lens,
+                     const int* qo_indptr, int64_t batch, int64_t max_q_len, float scale, void* out, void* stream);
+
+/* Log probabilities from logits [rows][vocab] (fp16, bf16 or fp32, row_stride elements apart, natural alignment):
+ *   logprobs[r] = log softmax(logits[r])[tokens[r]] (tokens int32 or int64, token_bytes 4 or 8; -inf for a token outside the
+ *   vocabulary), entropy[r] = -sum p log p, and the top_k (0..32, at most vocab) most probable tokens with their log
+ *   probabilities, top_logprobs / top_tokens [rows][top_k], greatest first, equal ones by the lower token.
+ * A logit of -inf has probability 0; a row that holds +inf or NaN, or nothing but -inf, gives NaN (in the order of the top k NaN
+ * comes first).  All statistics in fp32. */
+int cf_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride, const void* tokens,
+                      int token_bytes, int64_t top_k, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_tokens,
+                      void* stream);
 
 #ifdef __cplusplus
 }
