@@ -1,5 +1,5 @@
-// The paged cache held in 4 bits (layout: kv4_layout.cuh): rows written at their slots, rows read back, and attention over
-// it.  Asymmetric 4-bit codes over groups of 32 values of one token and head:
+// The paged cache held in 4 bits (layout: kv4_layout.cuh): rows written at their slots and read back, and the C entry
+// points.  Asymmetric 4-bit codes over groups of 32 values of one token and head:
 //   m = fp16(min x), s = fp16((max x - m) / 15), code = clamp(rint((x - m) / s), 0, 15), value = code * s + m
 // x in fp32 (clamped to fp16's range, which bf16 exceeds); the codes are computed against the rounded s and m, so the rounding of
 // the parameters costs no accuracy but the last step's.  A group that is constant has s = 0 and code 0; one that holds a
@@ -12,6 +12,7 @@
 
 #include "../../include/clusterfusion_b200.h"
 #include "host_common.h"
+#include "kv4_attention.h"
 #include "kv4_layout.cuh"
 
 namespace {
@@ -145,75 +146,6 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* __restrict
     store4(value + (tok * heads + head) * D + dim, xv);
 }
 
-struct AttnArgs {
-    const void* query;
-    const uint8_t* cache;
-    const int* table;
-    const int* kv_lens;
-    const int* qo_indptr;  // null: one query a request
-    void* out;
-    long long q_ts, q_hs, table_stride, table_width, rows;
-    int batch, heads, kv_heads, D, page, pages;
-    float scale_log2;
-};
-
-// The plainest form: one warp for a (query row, head), keys one after another, the running maximum and sum of the softmax.
-template <class T>
-__global__ void __launch_bounds__(128) kv4_attention_kernel(const AttnArgs a) {
-    const int lane = threadIdx.x & 31, G = kv4_groups(a.D), dim = 4 * lane;
-    const long long item = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    if (item >= a.rows * a.heads) return;
-    const long long row = item / a.heads;
-    const int head = static_cast<int>(item - row * a.heads), kvh = head / (a.heads / a.kv_heads);
-    int b = static_cast<int>(row), first = b, count = 1;
-    if (a.qo_indptr) {
-        if (row < a.qo_indptr[0] || row >= a.qo_indptr[a.batch]) return;  // rows of no request stay as they were
-        int lo = 0, hi = a.batch;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.qo_indptr[mid] <= row) lo = mid;
-            else hi = mid;
-        }
-        b = lo;
-        first = a.qo_indptr[b];
-        count = a.qo_indptr[b + 1] - first;
-    } else if (row >= a.batch) return;
-    const bool real = dim < a.D;
-    float q[4] = {0.f, 0.f, 0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-    if (real) load4(static_cast<const T*>(a.query) + row * a.q_ts + head * a.q_hs + dim, q);
-    const long long cap = a.table_width * a.page;
-    const long long seen = min(static_cast<long long>(a.kv_lens[b]) - count + (row - first) + 1, cap);
-    for (long long p = 0; p < seen; ++p) {
-        const int held = a.table[b * a.table_stride + p / a.page];
-        if (held < 0 || held >= a.pages) {
-            if (lane == 0) report_bad_slot();
-            continue;
-        }
-        const int at = static_cast<int>(p % a.page), r = at % KV4_TILE, g = lane >> 3;
-        const uint8_t* tile = a.cache + ((static_cast<long long>(held) * a.kv_heads + kvh) * (a.page / KV4_TILE) + at / KV4_TILE) * kv4_tile_bytes(G);
-        float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (real) {
-            auto par = [&](int which) { return __half2float(*reinterpret_cast<const __half*>(tile + kv4_param(G, r, which, g))); };
-            unpack4(*reinterpret_cast<const uint16_t*>(tile + kv4_key_half(G, r, dim)), par(0), par(1), k);
-            unpack4(*reinterpret_cast<const uint16_t*>(tile + kv4_value_half(G, r, dim)), par(2), par(3), v);
-        }
-        float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-#pragma unroll
-        for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-        s *= a.scale_log2;
-        const float top = fmaxf(m, s), ref = top == -INFINITY ? 0.f : top;
-        const float keep = exp2f(m - ref), e = exp2f(s - ref);
-        l = l * keep + e;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = o[i] * keep + e * v[i];
-        m = top;
-    }
-    if (!real) return;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = l > 0.f ? o[i] / l : (l == 0.f ? 0.f : l);  // no key seen: zeros; NaN stays NaN
-    store4(static_cast<T*>(a.out) + (row * a.heads + head) * a.D + dim, o);
-}
-
 int check_cache(int64_t pages, int64_t kv_heads, int64_t page, int64_t D) {
     if (D < 16 || D > KV4_MAX_DIM || D % 8 != 0) return cf_host_fail(CF_ERR_INVALID, "head_dim %lld must be a multiple of 8 in 16..%d", (long long)D, KV4_MAX_DIM);
     if (page < KV4_TILE || page % KV4_TILE != 0 || page > 65536) return cf_host_fail(CF_ERR_INVALID, "page size %lld must be a multiple of %d, at most 65536", (long long)page, KV4_TILE);
@@ -300,14 +232,24 @@ int cf_kv4_attention(const void* query, int dtype, int64_t rows, int64_t heads, 
     if (!query || !cache || !block_table || !kv_lens || !out) return cf_host_fail(CF_ERR_INVALID, "null pointer");
     if (!aligned(query, 16) || !aligned(out, 16) || !aligned(cache, 16) || (query_token_stride | query_head_stride) % 8 != 0)
         return cf_host_fail(CF_ERR_INVALID, "queries need 16-byte aligned rows (strides in multiples of 8 elements), cache and output 16 bytes");
-    const AttnArgs a{query, static_cast<const uint8_t*>(cache), block_table, kv_lens, qo_indptr, out, query_token_stride, query_head_stride, table_stride, table_width, rows,
-                     static_cast<int>(batch), static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(head_dim), static_cast<int>(page_size),
-                     static_cast<int>(pages), scale * 1.4426950408889634f};
-    const int64_t grid = (rows * heads + 3) / 4;
-    if (grid > 0x7fffffff) return cf_host_fail(CF_ERR_INVALID, "%lld query rows of %lld heads in one call", (long long)rows, (long long)heads);
-    if (dtype == CF_DTYPE_FP16) kv4_attention_kernel<__half><<<static_cast<unsigned>(grid), 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    else kv4_attention_kernel<__nv_bfloat16><<<static_cast<unsigned>(grid), 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    return check_launch("4-bit attention");
+    if (rows > 0x3fffffff / heads) return cf_host_fail(CF_ERR_INVALID, "%lld query rows of %lld heads in one call", (long long)rows, (long long)heads);
+    if (batch * kv_heads > 0x7fffffff / 8) return cf_host_fail(CF_ERR_INVALID, "%lld requests of %lld cached heads in one call", (long long)batch, (long long)kv_heads);
+    static int* status_word[64] = {};  // address of the device status word, by device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= 64)) return cf_host_fail(CF_ERR_UNSUPPORTED, "device index %d", dev);
+    if (e == cudaSuccess && !status_word[dev]) {
+        void* p = nullptr;
+        e = cudaGetSymbolAddress(&p, g_kv4_status);
+        if (e == cudaSuccess) status_word[dev] = static_cast<int*>(p);
+    }
+    if (e != cudaSuccess) return cf_host_fail(CF_ERR_CUDA, "4-bit attention: %s", cudaGetErrorString(e));
+    const Kv4AttnArgs a{query, static_cast<const uint8_t*>(cache), block_table, kv_lens, qo_indptr, out, query_token_stride, query_head_stride, table_stride, table_width, rows,
+                        static_cast<int>(batch), static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(head_dim), static_cast<int>(page_size),
+                        static_cast<int>(pages), scale * 1.4426950408889634f, status_word[dev]};
+    e = kv4_attention_few(a, dtype == CF_DTYPE_BF16, max_q_len, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cf_host_fail(CF_ERR_CUDA, "4-bit attention launch failed: %s", cudaGetErrorString(e));
+    return CF_OK;
 }
 
 }  // extern "C"
