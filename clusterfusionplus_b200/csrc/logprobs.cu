@@ -4,13 +4,15 @@
 //   log p_i = (x_i - m) - log z,   H = log z - w / z
 //
 // Nothing is formed as a difference of large numbers (no log-sum-exp is subtracted from a logit), so logits of any size keep
-// fp32's relative precision.  The floor is reading the logits once.  One CTA takes a row (or a cluster of CTAs a row when
-// there are few rows: the partial results meet in distributed shared memory, so no workspace and no second launch).
+// fp32's relative precision.  The floor is reading the logits once; one exponential an element comes second (2047 rows of
+// 50304: 32 us of reading, 23 us of MUFU).  One CTA takes a row, or a cluster of CTAs a row when there are few rows: the partial
+// results meet in distributed shared memory, so there is no workspace and no second launch.
 //
-// The top k (at most 32) cost next to nothing: every thread knows the largest element it met.  The k-th largest of these
-// maxima is a lower bound of the k-th largest element, and only the (at most k) threads whose maximum reaches it can hold any of
-// the top k.  Their elements are looked through once more, what reaches the bound is kept (a little over k values), ranked
-// and written.  Order: greater first, equal values by the lower index, NaN before everything, -0 equal to +0.
+// The top k (at most 32) cost little more: every thread remembers its greatest element.  Of 64 groups of threads, the k-th
+// greatest group maximum bounds the k-th greatest element from below (k groups hold one each), and only a thread whose own greatest
+// reaches the bound can hold any of the top k.  There are a few more than k of them: their elements are looked through
+// once more, what reaches the bound is kept, ranked by counting and written.  Order: greater first, equal values by the lower
+// index, NaN before everything, -0 equal to +0.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -23,8 +25,9 @@
 
 namespace {
 
-constexpr int LT = 512;        // threads of a CTA
+constexpr int LT = 256;        // threads of a CTA
 constexpr int LW = LT / 32;
+constexpr int GROUPS = 64;     // of LT / GROUPS threads, for the bound of the top k
 constexpr int MAX_TOP = 32;
 constexpr int MAX_CLUSTER = 8;
 constexpr int KEEP = 1024;     // candidates that are kept; more (adversarial orders only) take the slow way
@@ -51,10 +54,33 @@ __device__ __forceinline__ unsigned long long ranked(float x, int idx) {  // gre
     return static_cast<unsigned long long>(order_key(x)) << 32 | (0x7fffffffu - static_cast<unsigned>(idx));
 }
 
+__device__ __forceinline__ float key_value(unsigned key) {  // the value back (NaN for NaN)
+    return __uint_as_float(key == 0xffffffffu ? 0x7fffffffu : key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
 template <class T> __device__ __forceinline__ float to_float(T v);
 template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// greatest and least of the 16 bytes' elements (NaN left out), the 16-bit types two at a time
+__device__ __forceinline__ void extremes(const uint4& v, float& hi, float& lo, float) {
+    const float a = __uint_as_float(v.x), b = __uint_as_float(v.y), c = __uint_as_float(v.z), d = __uint_as_float(v.w);
+    hi = fmaxf(fmaxf(a, b), fmaxf(c, d));
+    lo = fminf(fminf(a, b), fminf(c, d));
+}
+template <class P, class F> __device__ __forceinline__ void extremes_of_pairs(const uint4& v, float& hi, float& lo, F to_float2) {
+    const P* p = reinterpret_cast<const P*>(&v);
+    const float2 h = to_float2(__hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]))), l = to_float2(__hmin2(__hmin2(p[0], p[1]), __hmin2(p[2], p[3])));
+    hi = fmaxf(h.x, h.y);
+    lo = fminf(l.x, l.y);
+}
+__device__ __forceinline__ void extremes(const uint4& v, float& hi, float& lo, __half) {
+    extremes_of_pairs<__half2>(v, hi, lo, [](__half2 x) { return __half22float2(x); });
+}
+__device__ __forceinline__ void extremes(const uint4& v, float& hi, float& lo, __nv_bfloat16) {
+    extremes_of_pairs<__nv_bfloat162>(v, hi, lo, [](__nv_bfloat162 x) { return __bfloat1622float2(x); });
+}
 
 // running statistics; m starts at the lowest finite number so that no difference of infinities is ever formed
 struct Stat {
@@ -65,8 +91,8 @@ struct Stat {
         z *= r;
         m = top;
     }
-    __device__ __forceinline__ void add(float x) {  // x <= m; NaN goes through
-        const float d = max_nan(x - m, -150.f), e = ex2(d * LOG2E);
+    template <bool CLAMP> __device__ __forceinline__ void add(float x) {  // x <= m; NaN goes through; CLAMP where x may be -inf (0 times infinity in w)
+        const float d = CLAMP ? max_nan(x - m, -150.f) : x - m, e = ex2(d * LOG2E);
         z += e;
         w = fmaf(e, d, w);
     }
@@ -137,66 +163,82 @@ __device__ __forceinline__ unsigned long long peer_u64(uint32_t a) {
 }
 
 struct __align__(16) Shared {
-    float part[LW][3];
-    float stat[3];
-    unsigned long long bests[LT];
+    unsigned long long best[LT];
+    unsigned long long group[GROUPS];
     unsigned long long keep[KEEP];
     unsigned long long top[MAX_TOP];
     unsigned long long all[MAX_CLUSTER * MAX_TOP];
     unsigned long long bound;
+    float part[LW][3];
+    float stat[3];
     int kept;
 };
 
-// The k greatest of [w.begin, w.end) as ranked() words in sh.top, greatest first, 0 where there are fewer.  `best`: this
-// thread's greatest (0 for none).
+// For each of n <= LT / PARTS values: how many of the n are greater; PARTS neighbouring threads work on a value and all get the count
+template <int PARTS> __device__ __forceinline__ int count_greater(const unsigned long long* v, int n, unsigned long long x) {
+    int c = 0;
+    for (int j = threadIdx.x % PARTS; j < n; j += PARTS) c += v[j] > x;
+#pragma unroll
+    for (int o = 1; o < PARTS; o <<= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+    return c;
+}
+
+// The k greatest of [w.begin, w.end) as ranked() words in sh.top, greatest first, 0 where there are fewer.  `best`: this thread's greatest (0
+// for none), its index rounded down to the start of its vector.  In this coarser order k elements reach the bound, and one
+// that does not has k elements above it in the exact order too.
 template <class T> __device__ void block_top(const Walk<T>& w, unsigned long long best, int k, Shared& sh) {
-    const int tid = threadIdx.x, lane = tid & 31;
-    sh.bests[tid] = best;
-    if (tid == 0) sh.kept = 0;
+    constexpr int E = Walk<T>::E;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    sh.best[tid] = best;
+    unsigned long long mine = best;
+#pragma unroll
+    for (int o = 1; o < LT / GROUPS; o <<= 1) {
+        const unsigned long long x = __shfl_xor_sync(0xffffffffu, mine, o);
+        mine = x > mine ? x : mine;
+    }
+    if (tid % (LT / GROUPS) == 0) sh.group[tid / (LT / GROUPS)] = mine;
+    if (tid == 0) sh.kept = 0, sh.bound = 0;
     if (tid < MAX_TOP) sh.top[tid] = 0;
     __syncthreads();
-    if (tid < 32) {  // the k-th greatest of the threads' bests
-        unsigned long long mine[LW];
-#pragma unroll
-        for (int i = 0; i < LW; ++i) mine[i] = sh.bests[i * 32 + lane];
-        unsigned long long top = 0;
-        for (int r = 0; r < k; ++r) {
-            unsigned long long x = 0;
-#pragma unroll
-            for (int i = 0; i < LW; ++i) x = mine[i] > x ? mine[i] : x;
-            const unsigned hi = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(x >> 32));
-            const unsigned lo = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(x >> 32) == hi ? static_cast<unsigned>(x) : 0u);
-            top = static_cast<unsigned long long>(hi) << 32 | lo;
-#pragma unroll
-            for (int i = 0; i < LW; ++i) mine[i] = mine[i] == top ? 0 : mine[i];
-        }
-        if (lane == 0) sh.bound = top;
+    {   // groups without elements have 0 and share a count: with fewer than k others the bound stays 0 and everything is kept
+        const unsigned long long x = sh.group[tid / (LT / GROUPS)];
+        if (count_greater<LT / GROUPS>(sh.group, GROUPS, x) == k - 1 && tid % (LT / GROUPS) == 0) sh.bound = x;
     }
     __syncthreads();
     const unsigned long long bound = sh.bound;
-    auto keep = [&](float x, int idx) {
-        const unsigned long long r = ranked(x, idx);
-        if (r >= bound) {
+    auto keep = [&](float x, int idx, int start) {
+        if (ranked(x, start) >= bound) {
             const int at = atomicAdd(&sh.kept, 1);
-            if (at < KEEP) sh.keep[at] = r;
+            if (at < KEEP) sh.keep[at] = ranked(x, idx);
         }
     };
     // the threads that reach the bound: each one's elements are dealt out to a warp
     int nth = 0;
     for (int i = 0; i < LW; ++i) {
-        const unsigned long long theirs = sh.bests[i * 32 + lane];
+        const unsigned long long theirs = sh.best[i * 32 + lane];
         unsigned who = __ballot_sync(0xffffffffu, theirs >= bound && theirs != 0);
         for (; who; who &= who - 1) {
-            if (nth++ % LW != tid >> 5) continue;
+            if (nth++ % LW != warp) continue;
             const int o = i * 32 + __ffs(who) - 1, s = w.single(o);
-            if (s >= 0 && lane == 0) keep(to_float(w.row[s]), s);
-            for (int v = o + lane * LT; v < w.vecs; v += 32 * LT)
+            if (s >= 0 && lane == 0) keep(to_float(w.row[s]), s, s);
+            for (int v = o + lane * LT; v < w.vecs; v += 32 * LT) {
+                const int at = w.vec_at(v);
+                const uint4 raw = __ldg(reinterpret_cast<const uint4*>(w.row + at));
+                const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-                for (int j = 0; j < Walk<T>::E; ++j) keep(to_float(w.row[w.vec_at(v) + j]), w.vec_at(v) + j);
+                for (int j = 0; j < E; ++j) keep(to_float(e[j]), at + j, at);
+            }
         }
     }
     __syncthreads();
     const int kept = sh.kept;
+    if (kept <= LT / 4) {  // the usual case: four threads a value
+        const unsigned long long x = tid / 4 < kept ? sh.keep[tid / 4] : 0;
+        const int rank = count_greater<4>(sh.keep, kept, x);
+        if (tid / 4 < kept && tid % 4 == 0 && rank < k) sh.top[rank] = x;
+        __syncthreads();
+        return;
+    }
     if (kept <= KEEP) {
         for (int c = tid; c < kept; c += LT) {
             const unsigned long long x = sh.keep[c];
@@ -218,12 +260,12 @@ template <class T> __device__ void block_top(const Walk<T>& w, unsigned long lon
         const int s = w.single(tid);
         if (s >= 0) look(to_float(w.row[s]), s);
         for (int v = tid; v < w.vecs; v += LT)
-            for (int i = 0; i < Walk<T>::E; ++i) look(to_float(w.row[w.vec_at(v) + i]), w.vec_at(v) + i);
+            for (int i = 0; i < E; ++i) look(to_float(w.row[w.vec_at(v) + i]), w.vec_at(v) + i);
         __syncthreads();
-        sh.bests[tid] = x;
+        sh.best[tid] = x;
         __syncthreads();
         x = 0;
-        for (int j = 0; j < LT; ++j) x = sh.bests[j] > x ? sh.bests[j] : x;
+        for (int j = 0; j < LT; ++j) x = sh.best[j] > x ? sh.best[j] : x;
         if (tid == 0) sh.top[r] = x;
         if (x == 0) break;
         last = x;
@@ -232,7 +274,7 @@ template <class T> __device__ void block_top(const Walk<T>& w, unsigned long lon
 }
 
 template <class T>
-__global__ void __launch_bounds__(LT) token_logprobs_kernel(const LogprobArgs a, int cluster) {
+__global__ void __launch_bounds__(LT, 6) token_logprobs_kernel(const LogprobArgs a, int cluster) {
     __shared__ Shared sh;
     constexpr int E = Walk<T>::E;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -243,8 +285,13 @@ __global__ void __launch_bounds__(LT) token_logprobs_kernel(const LogprobArgs a,
     const int begin = min(rank * share, a.vocab), end = min(begin + share, a.vocab);
     const Walk<T> w(row, begin, end);
 
+    float asked = -INFINITY;  // the given token's logit
+    if (tid == 0 && rank == 0) {
+        const long long tok = a.tokens64 ? static_cast<const long long*>(a.tokens)[r] : static_cast<const int*>(a.tokens)[r];
+        if (tok >= 0 && tok < a.vocab) asked = to_float(row[tok]);
+    }
     Stat st;
-    int best_at = -1;  // first index of the vector (or single) that holds this thread's first maximum
+    int best_at = -1;  // start of the vector (or the single) that holds this thread's first maximum
     const int single = w.single(tid);
     auto take_single = [&] {
         const float x = to_float(row[single]);
@@ -252,23 +299,24 @@ __global__ void __launch_bounds__(LT) token_logprobs_kernel(const LogprobArgs a,
             st.refer_to(x);
             best_at = single;
         } else if (best_at < 0) best_at = single;
-        st.add(x);
+        st.template add<true>(x);
     };
     if (single >= 0 && tid < E) take_single();
     auto take = [&](const uint4& raw, int at) {
         const T* e = reinterpret_cast<const T*>(&raw);
-        float x[E], top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            x[i] = to_float(e[i]);
-            top = fmaxf(top, x[i]);
-        }
-        if (top > st.m) {
-            st.refer_to(top);
+        float hi, lo;
+        extremes(raw, hi, lo, T());
+        if (hi > st.m) {
+            st.refer_to(hi);
             best_at = at;
         } else if (best_at < 0) best_at = at;
+        if (lo == -INFINITY) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) st.add(x[i]);
+            for (int i = 0; i < E; ++i) st.template add<true>(to_float(e[i]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) st.template add<false>(to_float(e[i]));
+        }
     };
     const uint4* vec = reinterpret_cast<const uint4*>(row + w.vec_at(0));
     constexpr int UNROLL = 4;
@@ -286,19 +334,13 @@ __global__ void __launch_bounds__(LT) token_logprobs_kernel(const LogprobArgs a,
     if (a.top > 0) {
         unsigned long long best = 0;
         if (best_at >= 0) {
-            if (st.z == st.z) {
-                const int n = best_at == single ? 1 : E;
-                for (int i = 0; i < n; ++i) {
-                    const unsigned long long y = ranked(to_float(row[best_at + i]), best_at + i);
-                    best = y > best ? y : best;
-                }
-                if (st.m == -FLT_MAX) best = 0;
-            }
-            if (best == 0) {  // a NaN, an infinity or nothing above the lowest number among them: look at each
+            if (st.z == st.z && st.m > -FLT_MAX) {
+                best = ranked(st.m, best_at);
+            } else {  // a NaN, an infinity or nothing above the lowest number among them: look at each
                 if (single >= 0) best = ranked(to_float(row[single]), single);
                 for (int u = tid; u < w.vecs; u += LT)
                     for (int i = 0; i < E; ++i) {
-                        const unsigned long long y = ranked(to_float(row[w.vec_at(u) + i]), w.vec_at(u) + i);
+                        const unsigned long long y = ranked(to_float(row[w.vec_at(u) + i]), w.vec_at(u));
                         best = y > best ? y : best;
                     }
             }
@@ -306,54 +348,52 @@ __global__ void __launch_bounds__(LT) token_logprobs_kernel(const LogprobArgs a,
         block_top(w, best, a.top, sh);
     }
 
+    auto join_lanes = [&](int width) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float m = __shfl_xor_sync(0xffffffffu, st.m, o), z = __shfl_xor_sync(0xffffffffu, st.z, o), ww = __shfl_xor_sync(0xffffffffu, st.w, o);
-        st.join(m, z, ww);
-    }
+        for (int o = 16; o > 0; o >>= 1) {
+            if (o >= width) continue;
+            const float m = __shfl_xor_sync(0xffffffffu, st.m, o), z = __shfl_xor_sync(0xffffffffu, st.z, o), ww = __shfl_xor_sync(0xffffffffu, st.w, o);
+            st.join(m, z, ww);
+        }
+    };
+    join_lanes(32);
     if (lane == 0) sh.part[warp][0] = st.m, sh.part[warp][1] = st.z, sh.part[warp][2] = st.w;
     __syncthreads();
-    if (tid == 0) {
-        Stat all;
-        for (int i = 0; i < LW; ++i) all.join(sh.part[i][0], sh.part[i][1], sh.part[i][2]);
-        sh.stat[0] = all.m, sh.stat[1] = all.z, sh.stat[2] = all.w;
+    if (warp == 0) {
+        st.m = sh.part[lane % LW][0], st.z = sh.part[lane % LW][1], st.w = sh.part[lane % LW][2];
+        join_lanes(LW);
+        if (lane == 0) sh.stat[0] = st.m, sh.stat[1] = st.z, sh.stat[2] = st.w;
     }
     if (cluster > 1) cluster_sync();
-    else __syncthreads();
     if (rank == 0) {
-        Stat all;
-        if (cluster == 1) {
-            all.m = sh.stat[0], all.z = sh.stat[1], all.w = sh.stat[2];
-        } else {
-            for (int c = 0; c < cluster; ++c) all.join(peer_float(peer(&sh.stat[0], c)), peer_float(peer(&sh.stat[1], c)), peer_float(peer(&sh.stat[2], c)));
-            if (a.top > 0) {
-                const int n = cluster * a.top;
-                for (int i = tid; i < n; i += LT) sh.all[i] = peer_u64(peer(&sh.top[i % a.top], i / a.top));
-                __syncthreads();
-                unsigned long long x = 0;
-                int at = a.top;
-                if (tid < n) {
-                    x = sh.all[tid];
-                    at = 0;
-                    for (int j = 0; j < n; ++j) at += sh.all[j] > x;
-                }
-                if (x != 0 && at < a.top) sh.keep[at] = x;
-                __syncthreads();
-                if (tid < a.top) sh.top[tid] = sh.keep[tid];
+        if (cluster > 1 && a.top > 0) {  // the CTAs' lists, ranked by counting (at most 256 entries: one thread each)
+            const int n = cluster * a.top;
+            unsigned long long x = 0;
+            if (tid < n) sh.all[tid] = x = peer_u64(peer(&sh.top[tid % a.top], tid / a.top));
+            __syncthreads();
+            int at = 0;
+            for (int j = 0; j < n; ++j) at += sh.all[j] > x;
+            if (tid < n && x != 0 && at < a.top) sh.keep[at] = x;
+            __syncthreads();
+            if (tid < a.top) sh.top[tid] = sh.keep[tid];
+        }
+        if (warp == 0) {
+            if (cluster > 1) {
+                const int c = lane % cluster;
+                st.m = peer_float(peer(&sh.stat[0], c)), st.z = peer_float(peer(&sh.stat[1], c)), st.w = peer_float(peer(&sh.stat[2], c));
+                join_lanes(cluster);
             }
-        }
-        const float log_z = logf(all.z);
-        if (tid == 0) {
-            const long long tok = a.tokens64 ? static_cast<const long long*>(a.tokens)[r] : static_cast<const int*>(a.tokens)[r];
-            const bool known = tok >= 0 && tok < a.vocab;
-            const float x = known ? to_float(row[tok]) : -INFINITY;
-            a.logprobs[r] = (x - all.m) - log_z;
-            a.entropy[r] = log_z - all.w / all.z;
-        }
-        if (tid < a.top) {
-            const int idx = static_cast<int>(0x7fffffffu - static_cast<unsigned>(sh.top[tid]));
-            a.top_tokens[r * a.top + tid] = idx;
-            a.top_logprobs[r * a.top + tid] = (to_float(row[idx]) - all.m) - log_z;
+            __syncwarp();
+            const float log_z = logf(st.z);
+            if (lane == 0) {
+                a.logprobs[r] = (asked - st.m) - log_z;
+                a.entropy[r] = log_z - st.w / st.z;
+            }
+            if (lane < a.top) {
+                const unsigned long long x = sh.top[lane];
+                a.top_tokens[r * a.top + lane] = static_cast<int>(0x7fffffffu - static_cast<unsigned>(x));
+                a.top_logprobs[r * a.top + lane] = (key_value(static_cast<unsigned>(x >> 32)) - st.m) - log_z;
+            }
         }
     }
     if (cluster > 1) cluster_sync();  // a peer's shared memory is read until here
