@@ -30,36 +30,33 @@ template <class T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <class T> __device__ __forceinline__ void load4(const T* p, float (&x)[4]) {
-    const uint2 raw = *reinterpret_cast<const uint2*>(p);
-    const T* e = reinterpret_cast<const T*>(&raw);
+// Both kernels: half a warp for a (token, head), lane l of the half holds dims 8 l .. 8 l + 7 (16 bytes) of the key and the
+// value, four lanes a group.  A warp then moves 2 KB of keys and values with two loads a lane, and the index arithmetic, the
+// group reductions (two shuffles) and the parameters' divisions are paid once for 64 values.
+constexpr int CT = 256;          // threads of a CTA
+constexpr int ITEMS = CT / 16;   // (token, head) pairs of a CTA
+
+template <class T> __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+    const uint2 raw[2] = {*reinterpret_cast<const uint2*>(p), *reinterpret_cast<const uint2*>(p + 4)};  // rows are 8-byte aligned
+    const T* e = reinterpret_cast<const T*>(raw);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = to_float<T>(e[i]);
-}
-template <class T> __device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
-    uint2 raw;
-    T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = from_float<T>(x[i]);
-    *reinterpret_cast<uint2*>(p) = raw;
+    for (int i = 0; i < 8; ++i) x[i] = to_float<T>(e[i]);
 }
 
-// codes of this lane's four values (16 bits), scale and minimum of its group; the eight lanes of a group work together
-__device__ __forceinline__ unsigned quantise4(const float (&x)[4], bool real, __half* scale, __half* low) {
-    float lo = 65504.f, hi = -65504.f, v[4];
-    bool finite = true;
+// Codes of this lane's eight values (nibble i: value i), scale and minimum of its group of four lanes.
+__device__ __forceinline__ unsigned quantise8(const float (&x)[8], bool real, __half* scale, __half* low) {
+    float lo = 65504.f, hi = -65504.f, v[8];
+    unsigned bad = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        finite &= !real || fabsf(x[i]) <= 3.4028234663852886e38f;  // false for NaN and the infinities
+    for (int i = 0; i < 8; ++i) {
+        bad |= !(fabsf(x[i]) <= 3.4028234663852886e38f);  // NaN and the infinities
         v[i] = fminf(fmaxf(x[i], -65504.f), 65504.f);
-        if (real) {
-            lo = fminf(lo, v[i]);
-            hi = fmaxf(hi, v[i]);
-        }
+        lo = fminf(lo, v[i]);
+        hi = fmaxf(hi, v[i]);
     }
-    unsigned bad = !finite;
+    if (!real) lo = 65504.f, hi = -65504.f, bad = 0;
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
+    for (int o = 1; o < 4; o <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         bad |= __shfl_xor_sync(0xffffffffu, bad, o);
@@ -67,83 +64,97 @@ __device__ __forceinline__ unsigned quantise4(const float (&x)[4], bool real, __
     const __half m = __float2half_rn(lo);
     const float mf = __half2float(m);
     const __half s = __float2half_rn((hi - mf) / 15.f);
-    const float sf = __half2float(s);
+    const float sf = __half2float(s), r = 1.f / sf;
     unsigned codes = 0;
     if (real && sf > 0.f) {
+        // rint((v - m) / s) by the reciprocal: off by a few 2^-24 of at most 16, which matters only next to a half; there it is divided
+        float q[8];
+        bool near_half = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float c = rintf((v[i] - mf) / sf);
-            codes |= static_cast<unsigned>(fminf(fmaxf(c, 0.f), 15.f)) << (4 * i);
+        for (int i = 0; i < 8; ++i) {
+            q[i] = (v[i] - mf) * r;
+            near_half |= fabsf(fabsf(q[i] - rintf(q[i])) - 0.5f) < 1e-5f;
         }
+        if (near_half)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = (v[i] - mf) / sf;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) codes |= static_cast<unsigned>(__float2int_rn(fminf(fmaxf(q[i], 0.f), 15.f))) << (4 * i);
     }
     *scale = bad ? __ushort_as_half(0x7fff) : s;
     *low = m;
     return bad ? 0u : codes;
 }
 
-// One warp for a (token, head); lane l holds dims 4 l .. 4 l + 3 of the key and the value.
+// the tile that holds a row, and the row in it
+__device__ __forceinline__ long long tile_of(int slot, int head, int heads, int tiles_a_page) {
+    const unsigned tile = static_cast<unsigned>(slot) / KV4_TILE, page = tile / tiles_a_page;
+    return (static_cast<long long>(page) * heads + head) * tiles_a_page + (tile - page * tiles_a_page);
+}
+
 template <class T>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const T* __restrict__ key, const T* __restrict__ value, const int* __restrict__ slot_map,
-                                                         uint8_t* __restrict__ cache, long long tokens, int heads, int D, int page, long long slots,
-                                                         long long k_ts, long long k_hs, long long v_ts, long long v_hs) {
-    const int G = kv4_groups(D), lane = threadIdx.x & 31;
-    const long long item = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    if (item >= tokens * heads) return;
-    const long long tok = item / heads;
-    const int head = static_cast<int>(item - tok * heads);
-    const int slot = slot_map[tok];
-    if (slot < 0) return;  // a padded row
-    if (slot >= slots) {
-        if (lane == 0) report_bad_slot();
-        return;
-    }
-    const int dim = 4 * lane;
-    const bool real = dim < D, stored = dim < 32 * G;
-    float xk[4] = {0.f, 0.f, 0.f, 0.f}, xv[4] = {0.f, 0.f, 0.f, 0.f};
+__global__ void __launch_bounds__(CT) kv4_append_kernel(const T* __restrict__ key, const T* __restrict__ value, const int* __restrict__ slot_map,
+                                                        uint8_t* __restrict__ cache, unsigned items, int heads, int D, int tiles_a_page, long long slots,
+                                                        long long k_ts, long long k_hs, long long v_ts, long long v_hs) {
+    const int G = kv4_groups(D), l = threadIdx.x & 15;
+    const unsigned item = blockIdx.x * ITEMS + threadIdx.x / 16;
+    const bool there = item < items;
+    const unsigned tok = there ? item / heads : 0;
+    const int head = there ? static_cast<int>(item - tok * heads) : 0;
+    const int slot = there ? slot_map[tok] : -1;
+    if (slot >= slots && l == 0) report_bad_slot();
+    const bool kept = slot >= 0 && slot < slots;  // a padded row is skipped
+    const int dim = 8 * l;
+    const bool real = kept && dim < D;
+    float xk[8], xv[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) xk[i] = xv[i] = 0.f;
     if (real) {
-        load4(key + tok * k_ts + head * k_hs + dim, xk);
-        load4(value + tok * v_ts + head * v_hs + dim, xv);
+        load8(key + tok * k_ts + head * k_hs + dim, xk);
+        load8(value + tok * v_ts + head * v_hs + dim, xv);
     }
     __half ks, km, vs, vm;
-    const unsigned kc = quantise4(xk, real, &ks, &km), vc = quantise4(xv, real, &vs, &vm);
-    if (!stored) return;
-    const int at = slot % page, row = at % KV4_TILE;
-    uint8_t* tile = cache + ((static_cast<long long>(slot / page) * heads + head) * (page / KV4_TILE) + at / KV4_TILE) * kv4_tile_bytes(G);
-    *reinterpret_cast<uint16_t*>(tile + kv4_key_half(G, row, dim)) = static_cast<uint16_t>(kc);
+    const unsigned kc = quantise8(xk, real, &ks, &km), vc = quantise8(xv, real, &vs, &vm);
+    if (!kept || dim >= 32 * G) return;
+    const int row = slot % KV4_TILE, which = l & 3;
+    uint8_t* tile = cache + tile_of(slot, head, heads, tiles_a_page) * kv4_tile_bytes(G);
+    *reinterpret_cast<uint32_t*>(tile + kv4_key_half(G, row, dim)) = kc;
     *reinterpret_cast<uint16_t*>(tile + kv4_value_half(G, row, dim)) = static_cast<uint16_t>(vc);
-    if ((lane & 7) < 4) {
-        const int which = lane & 3;
-        *reinterpret_cast<__half*>(tile + kv4_param(G, row, which, lane >> 3)) = which == 0 ? ks : which == 1 ? km : which == 2 ? vs : vm;
-    }
+    *reinterpret_cast<uint16_t*>(tile + kv4_value_half(G, row, dim + 4)) = static_cast<uint16_t>(vc >> 16);
+    *reinterpret_cast<__half*>(tile + kv4_param(G, row, which, l >> 2)) = which == 0 ? ks : which == 1 ? km : which == 2 ? vs : vm;
 }
 
-__device__ __forceinline__ void unpack4(unsigned codes, float s, float m, float (&x)[4]) {
+template <class T> __device__ __forceinline__ uint4 unpack8(unsigned codes, float s, float m) {
+    __align__(16) T e[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = fmaf(static_cast<float>((codes >> (4 * i)) & 15u), s, m);
+    for (int i = 0; i < 8; ++i) e[i] = from_float<T>(fmaf(static_cast<float>((codes >> (4 * i)) & 15u), s, m));
+    return *reinterpret_cast<const uint4*>(e);
 }
 
 template <class T>
-__global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ slot_map, T* __restrict__ key,
-                                                       T* __restrict__ value, long long tokens, int heads, int D, int page, long long slots) {
-    const int G = kv4_groups(D), lane = threadIdx.x & 31;
-    const long long item = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    if (item >= tokens * heads) return;
-    const long long tok = item / heads;
-    const int head = static_cast<int>(item - tok * heads);
-    const int slot = slot_map[tok], dim = 4 * lane;
-    if (dim >= D) return;
-    float xk[4] = {0.f, 0.f, 0.f, 0.f}, xv[4] = {0.f, 0.f, 0.f, 0.f};
+__global__ void __launch_bounds__(CT) kv4_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ slot_map, T* __restrict__ key,
+                                                      T* __restrict__ value, unsigned items, int heads, int D, int tiles_a_page, long long slots) {
+    const int G = kv4_groups(D), l = threadIdx.x & 15, dim = 8 * l;
+    const unsigned item = blockIdx.x * ITEMS + threadIdx.x / 16;
+    if (item >= items || dim >= D) return;
+    const unsigned tok = item / heads;
+    const int head = static_cast<int>(item - tok * heads), slot = slot_map[tok];
+    uint4 k = make_uint4(0, 0, 0, 0), v = k;
     if (slot >= 0 && slot < slots) {
-        const int at = slot % page, row = at % KV4_TILE, g = lane >> 3;
-        const uint8_t* tile = cache + ((static_cast<long long>(slot / page) * heads + head) * (page / KV4_TILE) + at / KV4_TILE) * kv4_tile_bytes(G);
+        const int row = slot % KV4_TILE, g = l >> 2;
+        const uint8_t* tile = cache + tile_of(slot, head, heads, tiles_a_page) * kv4_tile_bytes(G);
         auto par = [&](int which) { return __half2float(*reinterpret_cast<const __half*>(tile + kv4_param(G, row, which, g))); };
-        unpack4(*reinterpret_cast<const uint16_t*>(tile + kv4_key_half(G, row, dim)), par(0), par(1), xk);
-        unpack4(*reinterpret_cast<const uint16_t*>(tile + kv4_value_half(G, row, dim)), par(2), par(3), xv);
-    } else if (slot >= slots && lane == 0) {
+        const unsigned kc = *reinterpret_cast<const uint32_t*>(tile + kv4_key_half(G, row, dim));
+        const unsigned vc = *reinterpret_cast<const uint16_t*>(tile + kv4_value_half(G, row, dim)) |
+                            static_cast<unsigned>(*reinterpret_cast<const uint16_t*>(tile + kv4_value_half(G, row, dim + 4))) << 16;
+        k = unpack8<T>(kc, par(0), par(1));
+        v = unpack8<T>(vc, par(2), par(3));
+    } else if (slot >= slots && l == 0) {
         report_bad_slot();
     }
-    store4(key + (tok * heads + head) * D + dim, xk);
-    store4(value + (tok * heads + head) * D + dim, xv);
+    const long long at = static_cast<long long>(item) * D + dim;
+    *reinterpret_cast<uint4*>(key + at) = k;
+    *reinterpret_cast<uint4*>(value + at) = v;
 }
 
 int check_cache(int64_t pages, int64_t kv_heads, int64_t page, int64_t D) {
@@ -185,12 +196,12 @@ int cf_kv4_append(const void* key, const void* value, int dtype, int64_t tokens,
     if (!key || !value || !slot_map || !cache) return cf_host_fail(CF_ERR_INVALID, "null pointer");
     if (!aligned(key, 8) || !aligned(value, 8) || !aligned(cache, 16) || (key_token_stride | key_head_stride | value_token_stride | value_head_stride) % 4 != 0)
         return cf_host_fail(CF_ERR_INVALID, "keys and values need 8-byte aligned rows (strides in multiples of 4 elements), the cache 16 bytes");
-    const int64_t warps = tokens * kv_heads, grid = (warps + 7) / 8;
-    if (grid > 0x7fffffff) return cf_host_fail(CF_ERR_INVALID, "%lld tokens of %lld heads in one call", (long long)tokens, (long long)kv_heads);
+    const int64_t items = tokens * kv_heads, grid = (items + ITEMS - 1) / ITEMS;
+    if (items > 0x7fffffff) return cf_host_fail(CF_ERR_INVALID, "%lld tokens of %lld heads in one call", (long long)tokens, (long long)kv_heads);
     auto go = [&](auto* k, auto kernel) {
-        kernel<<<static_cast<unsigned>(grid), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-            k, static_cast<decltype(k)>(value), slot_map, static_cast<uint8_t*>(cache), tokens, static_cast<int>(kv_heads), static_cast<int>(head_dim),
-            static_cast<int>(page_size), pages * page_size, key_token_stride, key_head_stride, value_token_stride, value_head_stride);
+        kernel<<<static_cast<unsigned>(grid), CT, 0, static_cast<cudaStream_t>(stream)>>>(
+            k, static_cast<decltype(k)>(value), slot_map, static_cast<uint8_t*>(cache), static_cast<unsigned>(items), static_cast<int>(kv_heads), static_cast<int>(head_dim),
+            static_cast<int>(page_size / KV4_TILE), pages * page_size, key_token_stride, key_head_stride, value_token_stride, value_head_stride);
     };
     if (dtype == CF_DTYPE_FP16) go(static_cast<const __half*>(key), kv4_append_kernel<__half>);
     else go(static_cast<const __nv_bfloat16*>(key), kv4_append_kernel<__nv_bfloat16>);
@@ -205,12 +216,12 @@ int cf_kv4_read(const void* cache, int64_t pages, int64_t page_size, int64_t kv_
     if (tokens == 0) return CF_OK;
     if (!key || !value || !slot_map || !cache) return cf_host_fail(CF_ERR_INVALID, "null pointer");
     if (!aligned(key, 16) || !aligned(value, 16) || !aligned(cache, 16)) return cf_host_fail(CF_ERR_INVALID, "storage must be 16-byte aligned");
-    const int64_t warps = tokens * kv_heads, grid = (warps + 7) / 8;
-    if (grid > 0x7fffffff) return cf_host_fail(CF_ERR_INVALID, "%lld tokens of %lld heads in one call", (long long)tokens, (long long)kv_heads);
+    const int64_t items = tokens * kv_heads, grid = (items + ITEMS - 1) / ITEMS;
+    if (items > 0x7fffffff) return cf_host_fail(CF_ERR_INVALID, "%lld tokens of %lld heads in one call", (long long)tokens, (long long)kv_heads);
     auto go = [&](auto* k, auto kernel) {
-        kernel<<<static_cast<unsigned>(grid), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-            static_cast<const uint8_t*>(cache), slot_map, k, static_cast<decltype(k)>(value), tokens, static_cast<int>(kv_heads), static_cast<int>(head_dim),
-            static_cast<int>(page_size), pages * page_size);
+        kernel<<<static_cast<unsigned>(grid), CT, 0, static_cast<cudaStream_t>(stream)>>>(
+            static_cast<const uint8_t*>(cache), slot_map, k, static_cast<decltype(k)>(value), static_cast<unsigned>(items), static_cast<int>(kv_heads), static_cast<int>(head_dim),
+            static_cast<int>(page_size / KV4_TILE), pages * page_size);
     };
     if (dtype == CF_DTYPE_FP16) go(static_cast<__half*>(key), kv4_read_kernel<__half>);
     else go(static_cast<__nv_bfloat16*>(key), kv4_read_kernel<__nv_bfloat16>);
