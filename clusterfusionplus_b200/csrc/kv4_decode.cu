@@ -10,8 +10,10 @@
 //  - keys: S^T = K Q^T with the codes as the 16-row operand, 32 dims (one group) at a time from a zero accumulator, then one fp32
 //    multiply-add by the group's scale.  The minima contribute sum_g m_g (sum of q over group g): one more matrix instruction, the
 //    query sums as two fp16 numbers each (hi + lo, 22 bits).  Scores are exact to fp32's rounding.
-//  - values: O^T = V^T P^T, again codes as the 16-row operand (two tokens in one word's halves, so no re-pairing), P times the
-//    group's scale rounded to fp16 once; the minima in fp32 beside it.
+//  - values: O^T = V^T P^T, again codes as the 16-row operand (two tokens in one word's halves, so no re-pairing).  P is rounded to
+//    fp16, transposed, and multiplied by the groups' scales two tokens at a time (a second rounding).  One more instruction takes the
+//    minima and a row of ones times the same P: sum p m of every group and the softmax's denominator, fp32 sums of the P that the
+//    numerators use.
 // Queries are scaled by a power of two to at most 2^10 before they become fp16: exact for fp16 and bf16 inputs of any size
 // down to 2^-20 of their row's largest, off by less than 2^-30 of it below.  Probabilities are kept within (0, 4] (the running maximum is
 // two binary steps low) so that their product with a scale of up to 8734 (the widest fp16 range / 15) fits fp16 and small
@@ -35,7 +37,7 @@ namespace {
 
 constexpr int W = 4;                 // warps of a CTA
 constexpr int STAGES = 4;            // tiles of a warp's ring
-constexpr float LOWEST = -3.0e38f;   // start of the running maximum: finite, so that no difference of infinities is formed
+constexpr float LOWEST = -3.0e38f;   // reference of a result without tokens: finite, so that no difference of infinities is formed
 
 template <class T> __device__ __forceinline__ float2 to_float2(uint32_t v);
 template <> __device__ __forceinline__ float2 to_float2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
@@ -74,6 +76,34 @@ template <int N> __device__ __forceinline__ void load_halves(float (&x)[N], cons
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = __half2float(*reinterpret_cast<const __half*>(p + 2 * i));
     }
+}
+
+// word i: the i-th fp16 numbers at a (low half) and at b
+template <int N> __device__ __forceinline__ void pair_halves(uint32_t (&x)[N], const uint8_t* a, const uint8_t* b) {
+    if constexpr (N % 2 == 0) {
+        uint32_t u[N / 2], v[N / 2];
+        load_words<N / 2>(u, a);
+        load_words<N / 2>(v, b);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            x[2 * i] = __byte_perm(u[i], v[i], 0x5410);
+            x[2 * i + 1] = __byte_perm(u[i], v[i], 0x7632);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const uint16_t*>(a + 2 * i) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(b + 2 * i)) << 16;
+    }
+}
+
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+    const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// 0xffff in each half that holds a finite fp16 number, else 0
+__device__ __forceinline__ uint32_t finite_halves(uint32_t x) {
+    const uint32_t over = (((x & 0x7fff7fffu) + 0x04000400u) >> 15) & 0x00010001u;  // 1: exponent all ones
+    return ~(over * 0xffffu);
 }
 
 // G groups of 32 dims, NT tiles of 8 query rows
@@ -212,7 +242,8 @@ __global__ void __launch_bounds__(32 * W) kv4_few_kernel(const Kv4AttnArgs a, in
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s) issue();
 
-        float o[NT][2 * G][4], om[NT][G][2], m[NT][2], l[NT][2];
+        // numerators in units of 2^-24 and 2^-20; rows of `low`: group g's sum of p times the minimum (row g), the sum of p (row G)
+        float o[NT][2 * G][4], low[NT][4], m[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -220,10 +251,10 @@ __global__ void __launch_bounds__(32 * W) kv4_few_kernel(const Kv4AttnArgs a, in
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
 #pragma unroll
-            for (int g = 0; g < G; ++g) om[nt][g][0] = om[nt][g][1] = 0.f;
-            m[nt][0] = m[nt][1] = LOWEST;
-            l[nt][0] = l[nt][1] = 0.f;
+            for (int j = 0; j < 4; ++j) low[nt][j] = 0.f;
+            m[nt][0] = m[nt][1] = 0.f;
         }
+        bool first_tile = true;
 
         for (int i = 0; i < mine; ++i) {
             cp_async_wait<STAGES - 2>();
@@ -252,7 +283,7 @@ __global__ void __launch_bounds__(32 * W) kv4_few_kernel(const Kv4AttnArgs a, in
                         low1 |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(par1 + 2 * G + 4 * j + 2)) << 16;
                     }
                 }
-                if (t >= 2 * PAIRS) low0 = low1 = 0;
+                if (2 * PAIRS < 4 && t >= 2 * PAIRS) low0 = low1 = 0;
                 uint32_t k0[G], k1[G];
                 float s0[G], s1[G];
                 load_words<G>(k0, tile + g8 * 16 * G + t * 4 * G);
@@ -261,18 +292,17 @@ __global__ void __launch_bounds__(32 * W) kv4_few_kernel(const Kv4AttnArgs a, in
                 load_halves<G>(s1, par1);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma_16816(c, low0, low1, 0u, 0u, qm[nt], 0u);
+                    mma_16816_zero(x[nt], low0, low1, 0u, 0u, qm[nt], 0u);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[nt][j] = c[j] * 5.9604644775390625e-08f;  // 2^-24: the codes' unit
+                    for (int j = 0; j < 4; ++j) x[nt][j] *= 5.9604644775390625e-08f;  // 2^-24: the codes' unit
                 }
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     const uint32_t h0 = k0[g] >> 8, h1 = k1[g] >> 8;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        float c[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_16816(c, k0[g] & 0x000f000fu, k1[g] & 0x000f000fu, h0 & 0x000f000fu, h1 & 0x000f000fu, qa[nt][g][0], qa[nt][g][1]);
+                        float c[4];
+                        mma_16816_zero(c, k0[g] & 0x000f000fu, k1[g] & 0x000f000fu, h0 & 0x000f000fu, h1 & 0x000f000fu, qa[nt][g][0], qa[nt][g][1]);
                         mma_16816(c, k0[g] & 0x00f000f0u, k1[g] & 0x00f000f0u, h0 & 0x00f000f0u, h1 & 0x00f000f0u, qb[nt][g][0], qb[nt][g][1]);
                         x[nt][0] = fmaf(s0[g], c[0], x[nt][0]);
                         x[nt][1] = fmaf(s0[g], c[1], x[nt][1]);
@@ -281,17 +311,17 @@ __global__ void __launch_bounds__(32 * W) kv4_few_kernel(const Kv4AttnArgs a, in
                     }
                 }
             }
-            // ---- softmax
+            // ---- softmax: x becomes the binary logarithm of p, at most 2 above the running reference m
             const bool whole = token + KV4_TILE - 1 <= all_see;
-            bool rise = false;
+            bool rise = first_tile;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    x[nt][j] *= factor[nt][j & 1];
+                    x[nt][j] = fmaf(x[nt][j], factor[nt][j & 1], -m[nt][j & 1]);
                     if (!whole && token + g8 + (j >> 1) * 8 > last[nt][j & 1]) x[nt][j] = -INFINITY;
                 }
-                rise |= fmaxf(x[nt][0], x[nt][2]) - 2.f > m[nt][0] || fmaxf(x[nt][1], x[nt][3]) - 2.f > m[nt][1];
+                rise |= fmaxf(fmaxf(x[nt][0], x[nt][2]), fmaxf(x[nt][1], x[nt][3])) > 2.f;
             }
             if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
@@ -301,67 +331,68 @@ __global__ void __launch_bounds__(32 * W) kv4_few_kernel(const Kv4AttnArgs a, in
                         float top = fmaxf(x[nt][c], x[nt][c + 2]);
 #pragma unroll
                         for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-                        top = fmaxf(m[nt][c], top - 2.f);
-                        const float keep = ex2(m[nt][c] - top);
-                        m[nt][c] = top;
-                        l[nt][c] *= keep;
-#pragma unroll
-                        for (int g = 0; g < G; ++g) om[nt][g][c] *= keep;
+                        // a column's first tile sets its reference; one that sees nothing of its first tile sees nothing of later ones
+                        const float up = first_tile ? (top == -INFINITY ? 0.f : top - 2.f) : fmaxf(top - 2.f, 0.f);
+                        m[nt][c] += up;
+                        x[nt][c] -= up;
+                        x[nt][c + 2] -= up;
+                        const float keep = first_tile ? 1.f : ex2(-up);
+                        low[nt][c] *= keep;
 #pragma unroll
                         for (int q = 0; q < 2 * G; ++q) o[nt][q][c] *= keep, o[nt][q][c + 2] *= keep;
                     }
+                first_tile = false;
             }
-            // ---- values
+            // ---- values: scales of tokens 2 t, 2 t + 1 (sa) and 2 t + 8, 2 t + 9 (sb), group by group; minima likewise, of group g8
+            const uint8_t* pv = tile + 512 * G + 2 * t * 8 * G + 4 * G;
+            uint32_t sa[G], sb[G], ma = 0, mb = 0;
+            pair_halves<G>(sa, pv, pv + 8 * G);
+            pair_halves<G>(sb, pv + 64 * G, pv + 72 * G);
+            if (g8 < G) {
+                const uint8_t* pm = pv + 2 * G + 2 * g8;
+                ma = *reinterpret_cast<const uint16_t*>(pm) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(pm + 8 * G)) << 16;
+                mb = *reinterpret_cast<const uint16_t*>(pm + 64 * G) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(pm + 72 * G)) << 16;
+            } else if (g8 == G) ma = mb = 0x3c003c00u;  // ones
             uint32_t v0[G], v1[G];
-            float s0[G], s1[G], l0[G], l1[G];
             load_words<G>(v0, tile + 256 * G + lane * 4 * G);
             load_words<G>(v1, tile + 384 * G + lane * 4 * G);
-            load_halves<G>(s0, par0 + 4 * G);
-            load_halves<G>(l0, par0 + 6 * G);
-            load_halves<G>(s1, par1 + 4 * G);
-            load_halves<G>(l1, par1 + 6 * G);
-            if (!whole) {  // nothing that lies behind the last token may reach a sum, not even times 0
-                if (token + g8 > most)
+            if (!whole) {
+                // What a query does not see must not reach its sums, not even times 0: a token with a parameter that is not finite is taken
+                // out here, and the sums of those that do see it become NaN in that group.
+                const uint32_t ra = finite_halves(ma), rb = finite_halves(mb);
+                uint32_t bad = 0;  // of group g8: tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
-                    for (int g = 0; g < G; ++g) s0[g] = l0[g] = 0.f;
-                if (token + g8 + 8 > most)
+                for (int g = 0; g < G; ++g) {
+                    const uint32_t fa = finite_halves(sa[g]), fb = finite_halves(sb[g]);
+                    // the lanes of column t that hold group g's minima say whether those are finite
+                    const uint32_t ga = __shfl_sync(0xffffffffu, ra, g * 4 + t) & fa, gb = __shfl_sync(0xffffffffu, rb, g * 4 + t) & fb;
+                    sa[g] &= ga, sb[g] &= gb;
+                    if (g8 == g) bad = (~ga & 1u) | (~(ga >> 16) & 1u) << 1 | (~gb & 1u) << 8 | (~(gb >> 16) & 1u) << 9;
+                }
+                if (g8 < G) ma &= ra, mb &= rb;
+                if (__any_sync(0xffffffffu, bad != 0)) {
+                    uint32_t tokens = bad << (2 * t);  // bit k: token k of the tile, over the four lanes of a row
+                    tokens |= __shfl_xor_sync(0xffffffffu, tokens, 1);
+                    tokens |= __shfl_xor_sync(0xffffffffu, tokens, 2);
 #pragma unroll
-                    for (int g = 0; g < G; ++g) s1[g] = l1[g] = 0.f;
-            }
-            uint32_t p0[NT][G], p1[NT][G];
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float p[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) p[j] = ex2(x[nt][j] - m[nt][j & 1]);
-                l[nt][0] += p[0] + p[2];
-                l[nt][1] += p[1] + p[3];
-                if (whole) {
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        om[nt][g][0] = fmaf(p[0], l0[g], fmaf(p[2], l1[g], om[nt][g][0]));
-                        om[nt][g][1] = fmaf(p[1], l0[g], fmaf(p[3], l1[g], om[nt][g][1]));
-                        p0[nt][g] = transpose_8x8(pack_half2(p[0] * s0[g], p[1] * s0[g]));
-                        p1[nt][g] = transpose_8x8(pack_half2(p[2] * s1[g], p[3] * s1[g]));
-                    }
-                } else {  // a query that does not see a token takes nothing of it, whatever it holds
-                    const bool see[4] = {token + g8 <= last[nt][0], token + g8 <= last[nt][1], token + g8 + 8 <= last[nt][0], token + g8 + 8 <= last[nt][1]};
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        om[nt][g][0] += (see[0] ? p[0] * l0[g] : 0.f) + (see[2] ? p[2] * l1[g] : 0.f);
-                        om[nt][g][1] += (see[1] ? p[1] * l0[g] : 0.f) + (see[3] ? p[3] * l1[g] : 0.f);
-                        p0[nt][g] = transpose_8x8(pack_half2(see[0] ? p[0] * s0[g] : 0.f, see[1] ? p[1] * s0[g] : 0.f));
-                        p1[nt][g] = transpose_8x8(pack_half2(see[2] ? p[2] * s1[g] : 0.f, see[3] ? p[3] * s1[g] : 0.f));
-                    }
+                        for (int c = 0; c < 2; ++c) {
+                            const int see = last[nt][c] - token;  // tokens 0 .. see of the tile
+                            const uint32_t seen = see < 0 ? 0u : see >= 15 ? 0xffffu : (2u << see) - 1u;
+                            if (g8 < G && (tokens & seen)) low[nt][c] = __int_as_float(0x7fffffff);
+                        }
                 }
             }
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const uint32_t h0 = v0[g] >> 8, h1 = v1[g] >> 8;
+            for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t p0 = transpose_8x8(pack_half2(ex2(x[nt][0]), ex2(x[nt][1]))), p1 = transpose_8x8(pack_half2(ex2(x[nt][2]), ex2(x[nt][3])));
+                mma_16816(low[nt], ma, 0u, mb, 0u, p0, p1);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma_16816(o[nt][2 * g], v0[g] & 0x000f000fu, h0 & 0x000f000fu, v1[g] & 0x000f000fu, h1 & 0x000f000fu, p0[nt][g], p1[nt][g]);
-                    mma_16816(o[nt][2 * g + 1], v0[g] & 0x00f000f0u, h0 & 0x00f000f0u, v1[g] & 0x00f000f0u, h1 & 0x00f000f0u, p0[nt][g], p1[nt][g]);
+                for (int g = 0; g < G; ++g) {
+                    const uint32_t h0 = v0[g] >> 8, h1 = v1[g] >> 8, q0 = mul_half2(p0, sa[g]), q1 = mul_half2(p1, sb[g]);
+                    mma_16816(o[nt][2 * g], v0[g] & 0x000f000fu, h0 & 0x000f000fu, v1[g] & 0x000f000fu, h1 & 0x000f000fu, q0, q1);
+                    mma_16816(o[nt][2 * g + 1], v0[g] & 0x00f000f0u, h0 & 0x00f000f0u, v1[g] & 0x00f000f0u, h1 & 0x00f000f0u, q0, q1);
                 }
             }
         }
@@ -375,22 +406,18 @@ __global__ void __launch_bounds__(32 * W) kv4_few_kernel(const Kv4AttnArgs a, in
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float* line = merge + (nt * 8 + 2 * t + c) * LINE;
-                float sum = l[nt][c];
-#pragma unroll
-                for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+                const float sum = __shfl_sync(0xffffffffu, low[nt][c], G * 4 + t);
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    float low = om[nt][g][c];
-#pragma unroll
-                    for (int w = 4; w < 32; w <<= 1) low += __shfl_xor_sync(0xffffffffu, low, w);
+                    const float least = __shfl_sync(0xffffffffu, low[nt][c], g * 4 + t);
                     float4 y;
-                    y.x = fmaf(o[nt][2 * g][c], 16777216.f, low);
-                    y.y = fmaf(o[nt][2 * g + 1][c], 1048576.f, low);
-                    y.z = fmaf(o[nt][2 * g][c + 2], 16777216.f, low);
-                    y.w = fmaf(o[nt][2 * g + 1][c + 2], 1048576.f, low);
+                    y.x = fmaf(o[nt][2 * g][c], 16777216.f, least);
+                    y.y = fmaf(o[nt][2 * g + 1][c], 1048576.f, least);
+                    y.z = fmaf(o[nt][2 * g][c + 2], 16777216.f, least);
+                    y.w = fmaf(o[nt][2 * g + 1][c + 2], 1048576.f, least);
                     *reinterpret_cast<float4*>(line + 32 * g + 4 * g8) = y;
                 }
-                if (g8 == 0) line[DP] = m[nt][c], line[DP + 1] = sum;
+                if (g8 == 0) line[DP] = sum == 0.f ? LOWEST : m[nt][c], line[DP + 1] = sum;  // nothing seen: no reference either
             }
         __syncthreads();
         const int cols = min(COLS, rows - r0);
