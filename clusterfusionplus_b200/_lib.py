@@ -115,7 +115,9 @@ SIGNATURES = {
     "cf_kv4_append": (C.c_int, [C.c_void_p] * 2 + [C.c_int] + [C.c_int64] * 7 + [C.c_void_p] * 2 + [C.c_int64] * 2 + [C.c_void_p]),
     "cf_kv4_read": (C.c_int, [C.c_void_p] + [C.c_int64] * 4 + [C.c_void_p, C.c_int64] + [C.c_void_p] * 2 + [C.c_int, C.c_void_p]),
     "cf_kv4_attention": (C.c_int, [C.c_void_p, C.c_int] + [C.c_int64] * 5 + [C.c_void_p] + [C.c_int64] * 3 + [C.c_void_p]
-                         + [C.c_int64] * 2 + [C.c_void_p] * 2 + [C.c_int64] * 2 + [C.c_float] + [C.c_void_p] * 2),
+                         + [C.c_int64] * 2 + [C.c_void_p] * 2 + [C.c_int64] * 2 + [C.c_float, C.c_void_p, C.c_int64]
+                         + [C.c_void_p] * 2),
+    "cf_kv4_attention_workspace": (C.c_int64, [C.c_int64] * 6),
     "cf_token_logprobs": (C.c_int, [C.c_void_p, C.c_int] + [C.c_int64] * 3 + [C.c_void_p, C.c_int, C.c_int64]
                           + [C.c_void_p] * 5),
 }

@@ -16,9 +16,13 @@ struct Kv4AttnArgs {
     int batch, heads, kv_heads, D, page, pages;
     float scale_log2;  // of q . k, times log2(e)
     int* status;       // device status word
+    void* workspace;   // null: none
 };
 
-// few query rows a request: the cache is streamed once for up to 8 or 16 of them
+// few query rows a request: the cache is streamed once for up to 8 or 16 of them.  The workspace (its size in bytes; whether it is of use
+// where a request has at most `tokens`) spreads requests of different lengths evenly over the GPU.
+long long kv4_few_workspace(long long heads, long long kv_heads, int D, long long max_q_len);
+bool kv4_few_uses_workspace(long long batch, long long heads, long long kv_heads, long long tokens, long long max_q_len);
 cudaError_t kv4_attention_few(const Kv4AttnArgs& a, bool bf16, long long max_q_len, cudaStream_t st);
 
 }  // namespace cfb

@@ -19,9 +19,12 @@
 // two binary steps low) so that their product with a scale of up to 8734 (the widest fp16 range / 15) fits fp16 and small
 // scales keep their bits.
 //
-// The work of one (request, cached head) is dealt out tile by tile to the warps of a cluster of up to 8 CTAs, each warp streaming its tiles
-// through its own ring of shared memory by cp.async.  The partial results meet in distributed shared memory in a fixed
-// order: no workspace, one launch, the same bits every time.
+// Two ways to deal out the work, both without a wait between CTAs and with the same bits every time:
+//  - little work: a cluster of up to 8 CTAs takes a (request, cached head), its tiles go round the warps, the partial results meet in
+//    distributed shared memory.  One launch, no workspace.
+//  - much work: the tiles of all requests in one line, cut into equal pieces, one for each CTA that fits on the GPU, so that requests of any
+//    lengths keep every SM busy to the end; what a cut divides goes to a workspace and a second launch joins it.
+// Each warp streams its tiles through its own ring of shared memory by cp.async.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -36,7 +39,9 @@ namespace cfb {
 namespace {
 
 constexpr int W = 4;                 // warps of a CTA
-constexpr int STAGES = 4;            // tiles of a warp's ring
+constexpr int STAGES = 2;            // pairs of tiles in a warp's ring
+constexpr long long LINE_FROM = 4096;  // tiles of a call from which on the line pays
+constexpr int MAX_CLUSTER = 8;
 constexpr float LOWEST = -3.0e38f;   // reference of a result without tokens: finite, so that no difference of infinities is formed
 
 template <class T> __device__ __forceinline__ float2 to_float2(uint32_t v);
@@ -48,22 +53,27 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // e in -126 .. 127
 
-// N consecutive 32-bit words of shared memory (4 N-byte aligned for N = 1, 2, 4)
-template <int N> __device__ __forceinline__ void load_words(uint32_t (&x)[N], const uint8_t* p) {
+// Shared memory by the offset in the CTA's dynamic part: a pointer that may be null loses its address space, and generic loads with 64-bit
+// arithmetic cost a tenth of the instructions of a tile.
+extern __shared__ __align__(16) uint8_t smem[];
+
+template <int N> __device__ __forceinline__ void load_words(uint32_t (&x)[N], uint32_t p) {  // N 32-bit words, 4 N-byte aligned for N = 1, 2, 4
     if constexpr (N == 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        const uint4 v = *reinterpret_cast<const uint4*>(smem + p);
         x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
     } else if constexpr (N == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        const uint2 v = *reinterpret_cast<const uint2*>(smem + p);
         x[0] = v.x, x[1] = v.y;
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
+        for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const uint32_t*>(smem + p + 4 * i);
     }
 }
+__device__ __forceinline__ uint32_t load_word(uint32_t p) { return *reinterpret_cast<const uint32_t*>(smem + p); }
+__device__ __forceinline__ uint32_t load_half(uint32_t p) { return *reinterpret_cast<const uint16_t*>(smem + p); }
 
 // N consecutive fp16 numbers as floats (2 N-byte aligned for even N)
-template <int N> __device__ __forceinline__ void load_halves(float (&x)[N], const uint8_t* p) {
+template <int N> __device__ __forceinline__ void load_halves(float (&x)[N], uint32_t p) {
     if constexpr (N % 2 == 0) {
         uint32_t w[N / 2];
         load_words<N / 2>(w, p);
@@ -74,12 +84,12 @@ template <int N> __device__ __forceinline__ void load_halves(float (&x)[N], cons
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = __half2float(*reinterpret_cast<const __half*>(p + 2 * i));
+        for (int i = 0; i < N; ++i) x[i] = __half2float(__ushort_as_half(static_cast<unsigned short>(load_half(p + 2 * i))));
     }
 }
 
 // word i: the i-th fp16 numbers at a (low half) and at b
-template <int N> __device__ __forceinline__ void pair_halves(uint32_t (&x)[N], const uint8_t* a, const uint8_t* b) {
+template <int N> __device__ __forceinline__ void pair_halves(uint32_t (&x)[N], uint32_t a, uint32_t b) {
     if constexpr (N % 2 == 0) {
         uint32_t u[N / 2], v[N / 2];
         load_words<N / 2>(u, a);
@@ -91,7 +101,7 @@ template <int N> __device__ __forceinline__ void pair_halves(uint32_t (&x)[N], c
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const uint16_t*>(a + 2 * i) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(b + 2 * i)) << 16;
+        for (int i = 0; i < N; ++i) x[i] = load_half(a + 2 * i) | load_half(b + 2 * i) << 16;
     }
 }
 
@@ -106,144 +116,138 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t x) {
     return ~(over * 0xffffu);
 }
 
-// G groups of 32 dims, NT tiles of 8 query rows
-template <class T, int G, int NT>
-__global__ void __launch_bounds__(32 * W) kv4_few_kernel(const Kv4AttnArgs a, int cluster) {
-    constexpr int TB = kv4_tile_bytes(G), DP = 32 * G, COLS = 8 * NT, LINE = DP + 4;
-    constexpr int PAIRS = (G + 1) / 2;
-    extern __shared__ __align__(16) uint8_t smem[];  // the rings, later the warps' partial results
-    __shared__ float part[COLS][LINE];               // this CTA's partial result: DP numerators, maximum, denominator
+// what a request is made of
+struct Request {
+    int first, rows, per;    // first query row; query rows times heads of one cached head; heads of one cached head
+    long long before, cap;   // tokens ahead of its queries; tokens that its table can name
+    const int* table;
 
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, t = lane & 3;
-    const int rank = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-    const long long item = blockIdx.x / cluster;
-    const int b = static_cast<int>(item / a.kv_heads), kvh = static_cast<int>(item % a.kv_heads);
-    const int per = a.heads / a.kv_heads, tiles_a_page = a.page / KV4_TILE;
-    int first = b, n = 1;
-    if (a.qo_indptr) {
-        first = a.qo_indptr[b];
-        n = first < 0 ? 0 : min(a.qo_indptr[b + 1], static_cast<int>(a.rows)) - first;
+    __device__ __forceinline__ Request(const Kv4AttnArgs& a, int b) {
+        int n = 1;
+        first = b;
+        if (a.qo_indptr) {
+            first = a.qo_indptr[b];
+            n = first < 0 ? 0 : min(a.qo_indptr[b + 1], static_cast<int>(a.rows)) - first;
+        }
+        per = a.heads / a.kv_heads;
+        rows = n > 0 ? n * per : 0;  // at most rows * heads of the call: fits
+        cap = a.table_width * a.page;
+        before = static_cast<long long>(a.kv_lens[b]) - n;
+        table = a.table + b * a.table_stride;
     }
-    const int rows = n > 0 ? n * per : 0;  // at most rows * heads of the call: fits
-    const long long cap = a.table_width * a.page;
-    const long long before = static_cast<long long>(a.kv_lens[b]) - n;  // tokens ahead of the request's queries
-    const int* table = a.table + b * a.table_stride;
+    // tiles that the queries of the request see, at least 1
+    __device__ __forceinline__ int tiles() const {
+        const long long seen = min(before + rows / per, cap);
+        return seen <= 0 ? 1 : static_cast<int>((seen - 1) / KV4_TILE) + 1;
+    }
+};
 
-    for (int r0 = blockIdx.y * COLS; r0 < rows; r0 += gridDim.y * COLS) {
-        // ---- queries: B operands, and what the columns of S^T need
-        uint32_t qa[NT][G][2], qb[NT][G][2], qm[NT];
-        float factor[NT][2];
-        int last[NT][2];  // the last token that a column's query sees (before the cap), -1 for none
-        int all_see = 0x7fffffff, most = -1;
+template <class T> __device__ __forceinline__ void write_out(const Kv4AttnArgs& a, int first, int per, int kvh, int r, int d, float num, float den) {
+    if (d < a.D)  // no token seen: zeros; a NaN stays one
+        static_cast<T*>(a.out)[(static_cast<long long>(first + r / per) * a.heads + kvh * per + r % per) * a.D + d] = from_float<T>(den == 0.f ? 0.f : num / den);
+}
+
+// ---------------------------------------------------------------------------------------------------- query rows
+// Up to 8 NT rows of one (request, cached head): row r is query r / per, head kvh * per + r % per.
+template <int G, int NT> struct Rows {
+    uint32_t qa[NT][G][2], qb[NT][G][2], qm[NT];  // B operands: even dims, odd dims / 16, sums of the groups
+    float factor[NT][2];                          // of a column's scores
+    int last[NT][2];                              // the last token that a column's query sees, -1 for none
+    int all_see, most;                            // tokens up to all_see are seen by every row, none after `most` by any
+
+    template <class T> __device__ __forceinline__ void load(const Kv4AttnArgs& a, const Request& own, int kvh, int r0);
+};
+
+template <int G, int NT>
+template <class T>
+__device__ __forceinline__ void Rows<G, NT>::load(const Kv4AttnArgs& a, const Request& own, int kvh, int r0) {
+    constexpr int PAIRS = (G + 1) / 2;
+    const int lane = threadIdx.x & 31, g8 = lane >> 2, t = lane & 3, per = own.per, rows = own.rows;
+    all_see = 0x7fffffff, most = -1;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int r = r0 + nt * 8 + g8;
-            const bool real = r < rows;
-            float q[G][8], top = 0.f;
-            if (real) {
-                const T* src = static_cast<const T*>(a.query) + static_cast<long long>(first + r / per) * a.q_ts + (kvh * per + r % per) * a.q_hs;
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const int dim = 32 * g + 8 * t;
-                    uint4 raw = make_uint4(0, 0, 0, 0);
-                    if (dim < a.D) raw = *reinterpret_cast<const uint4*>(src + dim);
-                    const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 f = to_float2<T>(words[i]);
-                        q[g][2 * i] = f.x, q[g][2 * i + 1] = f.y;
-                        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int g = 0; g < G; ++g)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) q[g][i] = 0.f;
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100);  // 2^e <= top < 2^(e + 1)
-            const float up = power_of_two(min(9 - e, 127));
-            float sums[G];
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = r0 + nt * 8 + g8;
+        const bool real = r < rows;
+        float q[G][8], top = 0.f;
+        if (real) {
+            const T* src = static_cast<const T*>(a.query) + static_cast<long long>(own.first + r / per) * a.q_ts + (kvh * per + r % per) * a.q_hs;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                sums[g] = 0.f;
+                const int dim = 32 * g + 8 * t;
+                uint4 raw = make_uint4(0, 0, 0, 0);
+                if (dim < a.D) raw = *reinterpret_cast<const uint4*>(src + dim);
+                const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    q[g][i] *= up;
-                    sums[g] += q[g][i];
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = to_float2<T>(words[i]);
+                    q[g][2 * i] = f.x, q[g][2 * i + 1] = f.y;
+                    top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
                 }
-                qa[nt][g][0] = pack_half2(q[g][0], q[g][4]);
-                qa[nt][g][1] = pack_half2(q[g][2], q[g][6]);
-                qb[nt][g][0] = pack_half2(q[g][1] * 0.0625f, q[g][5] * 0.0625f);
-                qb[nt][g][1] = pack_half2(q[g][3] * 0.0625f, q[g][7] * 0.0625f);
-                sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
-                sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
             }
-            qm[nt] = 0;  // row pair t of the minima's product: sums of groups 2 j, 2 j + 1 rounded (t = j), and what the rounding left (t = j + PAIRS)
+        } else {
 #pragma unroll
-            for (int j = 0; j < PAIRS; ++j) {
-                const float x = sums[2 * j], y = 2 * j + 1 < G ? sums[2 * j + 1] : 0.f;
-                const float xh = __half2float(__float2half_rn(x)), yh = __half2float(__float2half_rn(y));
-                if (t == j) qm[nt] = pack_half2(x, y);
-                if (t == j + PAIRS) qm[nt] = pack_half2(x - xh, y - yh);
-            }
-            // fp32 factor of a column's scores: 2^24 of the codes, the query's power of two, the softmax scale in binary logarithms
-            const float f = fminf(fmaxf(a.scale_log2 * 16777216.f * power_of_two(e - 9), -3.4e38f), 3.4e38f);
-            const long long see = before + r / per;
-            const int end = real ? static_cast<int>(min(see, cap - 1)) : -1;
+            for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                factor[nt][c] = __shfl_sync(0xffffffffu, f, (2 * t + c) * 4);
-                last[nt][c] = __shfl_sync(0xffffffffu, end < 0 ? -1 : end, (2 * t + c) * 4);
-            }
-            if (real) {
-                most = max(most, end);
-                all_see = min(all_see, end);
-            }
+                for (int i = 0; i < 8; ++i) q[g][i] = 0.f;
         }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100);  // 2^e <= top < 2^(e + 1)
+        const float up = power_of_two(min(9 - e, 127));
+        float sums[G];
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-            all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, o));
-        }
-
-        // ---- this warp's tiles: unit, unit + units, ...
-        const int units = cluster * W, unit = rank * W + warp;
-        const int tiles = most < 0 ? 0 : most / KV4_TILE + 1;
-        const int mine = tiles > unit ? (tiles - unit + units - 1) / units : 0;
-        uint8_t* ring = smem + warp * STAGES * TB;
-        int col = unit / tiles_a_page, in_page = unit % tiles_a_page, issued = 0;
-        const int step_col = units / tiles_a_page, step_in = units % tiles_a_page;
-        int held = mine > 0 ? table[col] : -1;
-        unsigned there = 0;  // bit s: the tile in stage s exists (its page lies in the cache)
-        auto issue = [&] {
-            if (issued < mine) {
-                const int stage = issued % STAGES;
-                const bool ok = held >= 0 && held < a.pages;
-                there = (there & ~(1u << stage)) | (static_cast<unsigned>(ok) << stage);
-                if (ok) {
-                    const uint8_t* src = a.cache + ((static_cast<long long>(held) * a.kv_heads + kvh) * tiles_a_page + in_page) * TB;
-                    const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(ring + stage * TB));
+        for (int g = 0; g < G; ++g) {
+            sums[g] = 0.f;
 #pragma unroll
-                    for (int i = 0; i < (TB / 16 + 31) / 32; ++i)
-                        if (i * 32 + lane < TB / 16) cp_async_16(dst + (i * 32 + lane) * 16, src + (i * 32 + lane) * 16);
-                } else if (lane == 0) {
-                    atomicCAS(a.status, 0, ST_BAD_SLOT);
-                }
-                ++issued;
-                col += step_col, in_page += step_in;
-                if (in_page >= tiles_a_page) in_page -= tiles_a_page, ++col;
-                held = issued < mine ? table[col] : -1;
+            for (int i = 0; i < 8; ++i) {
+                q[g][i] *= up;
+                sums[g] += q[g][i];
             }
-            cp_async_commit();
-        };
+            qa[nt][g][0] = pack_half2(q[g][0], q[g][4]);
+            qa[nt][g][1] = pack_half2(q[g][2], q[g][6]);
+            qb[nt][g][0] = pack_half2(q[g][1] * 0.0625f, q[g][5] * 0.0625f);
+            qb[nt][g][1] = pack_half2(q[g][3] * 0.0625f, q[g][7] * 0.0625f);
+            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
+            sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+        }
+        qm[nt] = 0;  // row pair t of the minima's product: sums of groups 2 j, 2 j + 1 rounded (t = j), and what the rounding left (t = j + PAIRS)
 #pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s) issue();
+        for (int j = 0; j < PAIRS; ++j) {
+            const float x = sums[2 * j], y = 2 * j + 1 < G ? sums[2 * j + 1] : 0.f;
+            const float xh = __half2float(__float2half_rn(x)), yh = __half2float(__float2half_rn(y));
+            if (t == j) qm[nt] = pack_half2(x, y);
+            if (t == j + PAIRS) qm[nt] = pack_half2(x - xh, y - yh);
+        }
+        // fp32 factor of a column's scores: 2^24 of the codes, the query's power of two, the softmax scale in binary logarithms
+        const float f = fminf(fmaxf(a.scale_log2 * 16777216.f * power_of_two(e - 9), -3.4e38f), 3.4e38f);
+        const long long see = own.before + r / per;
+        const int end = real ? static_cast<int>(min(see, own.cap - 1)) : -1;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            factor[nt][c] = __shfl_sync(0xffffffffu, f, (2 * t + c) * 4);
+            last[nt][c] = __shfl_sync(0xffffffffu, end < 0 ? -1 : end, (2 * t + c) * 4);
+        }
+        if (real) {
+            most = max(most, end);
+            all_see = min(all_see, end);
+        }
+    }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, o));
+    }
+}
 
-        // numerators in units of 2^-24 and 2^-20; rows of `low`: group g's sum of p times the minimum (row g), the sum of p (row G)
-        float o[NT][2 * G][4], low[NT][4], m[NT][2];
+// ---------------------------------------------------------------------------------------------------- accumulators
+template <int G, int NT> struct Acc {
+    static constexpr int DP = 32 * G, LINE = DP + 4;
+    float o[NT][2 * G][4];  // numerators in units of 2^-24 and 2^-20
+    float low[NT][4];       // row g: group g's sum of p times the minimum; row G: the sum of p
+    float m[NT][2];         // reference of a column: p = 2^(score - m), at most 4
+    bool first_tile;
+
+    __device__ __forceinline__ void reset() {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -254,245 +258,567 @@ __global__ void __launch_bounds__(32 * W) kv4_few_kernel(const Kv4AttnArgs a, in
             for (int j = 0; j < 4; ++j) low[nt][j] = 0.f;
             m[nt][0] = m[nt][1] = 0.f;
         }
-        bool first_tile = true;
+        first_tile = true;
+    }
+    template <int K> __device__ __forceinline__ void step(const int (&tile)[K], int token, const Rows<G, NT>& r, int lane);
+    __device__ __forceinline__ void store(float* lines) const;
+};
 
-        for (int i = 0; i < mine; ++i) {
-            cp_async_wait<STAGES - 2>();
-            __syncwarp();
-            const int stage = i % STAGES, token = (unit + i * units) * KV4_TILE;
-            const bool ok = (there >> stage) & 1;
-            issue();  // into the stage that the whole warp is done with
-            if (!ok) continue;
-            const uint8_t* tile = ring + stage * TB;
-            const uint8_t* par0 = tile + 512 * G + g8 * 8 * G;  // parameters of tokens g8 and g8 + 8
-            const uint8_t* par1 = par0 + 64 * G;
+// K tiles of 16 tokens in a row, the first token of all `token`, the tiles at these offsets of shared memory
+template <int G, int NT>
+template <int K>
+__device__ __forceinline__ void Acc<G, NT>::step(const int (&tile)[K], int token, const Rows<G, NT>& r, int lane) {
+    constexpr int PAIRS = (G + 1) / 2;
+    const int g8 = lane >> 2, t = lane & 3;
 
-            // ---- scores
-            float x[NT][4];
-            {
-                uint32_t low0 = 0, low1 = 0;
-                if constexpr (G % 2 == 0) {
-                    low0 = *reinterpret_cast<const uint32_t*>(par0 + 2 * G + 4 * (t % PAIRS));
-                    low1 = *reinterpret_cast<const uint32_t*>(par1 + 2 * G + 4 * (t % PAIRS));
-                } else {
-                    const int j = t % PAIRS;
-                    low0 = *reinterpret_cast<const uint16_t*>(par0 + 2 * G + 4 * j);
-                    low1 = *reinterpret_cast<const uint16_t*>(par1 + 2 * G + 4 * j);
-                    if (2 * j + 1 < G) {
-                        low0 |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(par0 + 2 * G + 4 * j + 2)) << 16;
-                        low1 |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(par1 + 2 * G + 4 * j + 2)) << 16;
-                    }
-                }
-                if (2 * PAIRS < 4 && t >= 2 * PAIRS) low0 = low1 = 0;
-                uint32_t k0[G], k1[G];
-                float s0[G], s1[G];
-                load_words<G>(k0, tile + g8 * 16 * G + t * 4 * G);
-                load_words<G>(k1, tile + (g8 + 8) * 16 * G + t * 4 * G);
-                load_halves<G>(s0, par0);
-                load_halves<G>(s1, par1);
+    // ---- scores
+    float x[K][NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma_16816_zero(x[nt], low0, low1, 0u, 0u, qm[nt], 0u);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[nt][j] *= 5.9604644775390625e-08f;  // 2^-24: the codes' unit
-                }
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const uint32_t h0 = k0[g] >> 8, h1 = k1[g] >> 8;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float c[4];
-                        mma_16816_zero(c, k0[g] & 0x000f000fu, k1[g] & 0x000f000fu, h0 & 0x000f000fu, h1 & 0x000f000fu, qa[nt][g][0], qa[nt][g][1]);
-                        mma_16816(c, k0[g] & 0x00f000f0u, k1[g] & 0x00f000f0u, h0 & 0x00f000f0u, h1 & 0x00f000f0u, qb[nt][g][0], qb[nt][g][1]);
-                        x[nt][0] = fmaf(s0[g], c[0], x[nt][0]);
-                        x[nt][1] = fmaf(s0[g], c[1], x[nt][1]);
-                        x[nt][2] = fmaf(s1[g], c[2], x[nt][2]);
-                        x[nt][3] = fmaf(s1[g], c[3], x[nt][3]);
-                    }
-                }
-            }
-            // ---- softmax: x becomes the binary logarithm of p, at most 2 above the running reference m
-            const bool whole = token + KV4_TILE - 1 <= all_see;
-            bool rise = first_tile;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    x[nt][j] = fmaf(x[nt][j], factor[nt][j & 1], -m[nt][j & 1]);
-                    if (!whole && token + g8 + (j >> 1) * 8 > last[nt][j & 1]) x[nt][j] = -INFINITY;
-                }
-                rise |= fmaxf(fmaxf(x[nt][0], x[nt][2]), fmaxf(x[nt][1], x[nt][3])) > 2.f;
-            }
-            if (__any_sync(0xffffffffu, rise)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float top = fmaxf(x[nt][c], x[nt][c + 2]);
-#pragma unroll
-                        for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-                        // a column's first tile sets its reference; one that sees nothing of its first tile sees nothing of later ones
-                        const float up = first_tile ? (top == -INFINITY ? 0.f : top - 2.f) : fmaxf(top - 2.f, 0.f);
-                        m[nt][c] += up;
-                        x[nt][c] -= up;
-                        x[nt][c + 2] -= up;
-                        const float keep = first_tile ? 1.f : ex2(-up);
-                        low[nt][c] *= keep;
-#pragma unroll
-                        for (int q = 0; q < 2 * G; ++q) o[nt][q][c] *= keep, o[nt][q][c + 2] *= keep;
-                    }
-                first_tile = false;
-            }
-            // ---- values: scales of tokens 2 t, 2 t + 1 (sa) and 2 t + 8, 2 t + 9 (sb), group by group; minima likewise, of group g8
-            const uint8_t* pv = tile + 512 * G + 2 * t * 8 * G + 4 * G;
-            uint32_t sa[G], sb[G], ma = 0, mb = 0;
-            pair_halves<G>(sa, pv, pv + 8 * G);
-            pair_halves<G>(sb, pv + 64 * G, pv + 72 * G);
-            if (g8 < G) {
-                const uint8_t* pm = pv + 2 * G + 2 * g8;
-                ma = *reinterpret_cast<const uint16_t*>(pm) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(pm + 8 * G)) << 16;
-                mb = *reinterpret_cast<const uint16_t*>(pm + 64 * G) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(pm + 72 * G)) << 16;
-            } else if (g8 == G) ma = mb = 0x3c003c00u;  // ones
-            uint32_t v0[G], v1[G];
-            load_words<G>(v0, tile + 256 * G + lane * 4 * G);
-            load_words<G>(v1, tile + 384 * G + lane * 4 * G);
-            if (!whole) {
-                // What a query does not see must not reach its sums, not even times 0: a token with a parameter that is not finite is taken
-                // out here, and the sums of those that do see it become NaN in that group.
-                const uint32_t ra = finite_halves(ma), rb = finite_halves(mb);
-                uint32_t bad = 0;  // of group g8: tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const uint32_t fa = finite_halves(sa[g]), fb = finite_halves(sb[g]);
-                    // the lanes of column t that hold group g's minima say whether those are finite
-                    const uint32_t ga = __shfl_sync(0xffffffffu, ra, g * 4 + t) & fa, gb = __shfl_sync(0xffffffffu, rb, g * 4 + t) & fb;
-                    sa[g] &= ga, sb[g] &= gb;
-                    if (g8 == g) bad = (~ga & 1u) | (~(ga >> 16) & 1u) << 1 | (~gb & 1u) << 8 | (~(gb >> 16) & 1u) << 9;
-                }
-                if (g8 < G) ma &= ra, mb &= rb;
-                if (__any_sync(0xffffffffu, bad != 0)) {
-                    uint32_t tokens = bad << (2 * t);  // bit k: token k of the tile, over the four lanes of a row
-                    tokens |= __shfl_xor_sync(0xffffffffu, tokens, 1);
-                    tokens |= __shfl_xor_sync(0xffffffffu, tokens, 2);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const int see = last[nt][c] - token;  // tokens 0 .. see of the tile
-                            const uint32_t seen = see < 0 ? 0u : see >= 15 ? 0xffffu : (2u << see) - 1u;
-                            if (g8 < G && (tokens & seen)) low[nt][c] = __int_as_float(0x7fffffff);
-                        }
-                }
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const uint32_t p0 = transpose_8x8(pack_half2(ex2(x[nt][0]), ex2(x[nt][1]))), p1 = transpose_8x8(pack_half2(ex2(x[nt][2]), ex2(x[nt][3])));
-                mma_16816(low[nt], ma, 0u, mb, 0u, p0, p1);
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const uint32_t h0 = v0[g] >> 8, h1 = v1[g] >> 8, q0 = mul_half2(p0, sa[g]), q1 = mul_half2(p1, sb[g]);
-                    mma_16816(o[nt][2 * g], v0[g] & 0x000f000fu, h0 & 0x000f000fu, v1[g] & 0x000f000fu, h1 & 0x000f000fu, q0, q1);
-                    mma_16816(o[nt][2 * g + 1], v0[g] & 0x00f000f0u, h0 & 0x00f000f0u, v1[g] & 0x00f000f0u, h1 & 0x00f000f0u, q0, q1);
-                }
+    for (int u = 0; u < K; ++u) {
+        const uint32_t par0 = tile[u] + 512 * G + g8 * 8 * G, par1 = par0 + 64 * G;  // parameters of tokens g8 and g8 + 8
+        uint32_t low0 = 0, low1 = 0;
+        const int j = t % PAIRS;
+        if constexpr (G % 2 == 0) {
+            low0 = load_word(par0 + 2 * G + 4 * j);
+            low1 = load_word(par1 + 2 * G + 4 * j);
+        } else {
+            low0 = load_half(par0 + 2 * G + 4 * j);
+            low1 = load_half(par1 + 2 * G + 4 * j);
+            if (2 * j + 1 < G) {
+                low0 |= load_half(par0 + 2 * G + 4 * j + 2) << 16;
+                low1 |= load_half(par1 + 2 * G + 4 * j + 2) << 16;
             }
         }
-        cp_async_wait<0>();
-
-        // ---- the warps' results, then the CTAs': columns of numerators, maximum and denominator
-        __syncthreads();  // the rings are free
-        float* merge = reinterpret_cast<float*>(smem) + warp * COLS * LINE;
+        if (2 * PAIRS < 4 && t >= 2 * PAIRS) low0 = low1 = 0;
+        uint32_t k0[G], k1[G];
+        float s0[G], s1[G];
+        load_words<G>(k0, tile[u] + g8 * 16 * G + t * 4 * G);
+        load_words<G>(k1, tile[u] + (g8 + 8) * 16 * G + t * 4 * G);
+        load_halves<G>(s0, par0);
+        load_halves<G>(s1, par1);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            mma_16816_zero(x[u][nt], low0, low1, 0u, 0u, r.qm[nt], 0u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[u][nt][i] *= 5.9604644775390625e-08f;  // 2^-24: the codes' unit
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const uint32_t h0 = k0[g] >> 8, h1 = k1[g] >> 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float c[4];
+                mma_16816_zero(c, k0[g] & 0x000f000fu, k1[g] & 0x000f000fu, h0 & 0x000f000fu, h1 & 0x000f000fu, r.qa[nt][g][0], r.qa[nt][g][1]);
+                mma_16816(c, k0[g] & 0x00f000f0u, k1[g] & 0x00f000f0u, h0 & 0x00f000f0u, h1 & 0x00f000f0u, r.qb[nt][g][0], r.qb[nt][g][1]);
+                x[u][nt][0] = fmaf(s0[g], c[0], x[u][nt][0]);
+                x[u][nt][1] = fmaf(s0[g], c[1], x[u][nt][1]);
+                x[u][nt][2] = fmaf(s1[g], c[2], x[u][nt][2]);
+                x[u][nt][3] = fmaf(s1[g], c[3], x[u][nt][3]);
+            }
+        }
+    }
+    // ---- softmax: x becomes the binary logarithm of p.  The reference is set so that the greatest p is 2 and moves when one exceeds 4: seldom
+    // after the first tiles.  (Lower would move less often, but p times a small scale would leave the range of normal fp16 numbers sooner.)
+    const bool whole = token + K * KV4_TILE - 1 <= r.all_see;
+    bool rise = first_tile;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int u = 0; u < K; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[u][nt][j] = fmaf(x[u][nt][j], r.factor[nt][j & 1], -m[nt][j & 1]);
+    if (!whole) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int u = 0; u < K; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (token + u * KV4_TILE + g8 + (j >> 1) * 8 > r.last[nt][j & 1]) x[u][nt][j] = -INFINITY;
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        float top = fmaxf(fmaxf(x[0][nt][0], x[0][nt][2]), fmaxf(x[0][nt][1], x[0][nt][3]));
+        if constexpr (K == 2) top = fmaxf(top, fmaxf(fmaxf(x[K - 1][nt][0], x[K - 1][nt][2]), fmaxf(x[K - 1][nt][1], x[K - 1][nt][3])));
+        rise |= top > 2.f;
+    }
+    if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float* line = merge + (nt * 8 + 2 * t + c) * LINE;
-                const float sum = __shfl_sync(0xffffffffu, low[nt][c], G * 4 + t);
+                float top = fmaxf(x[0][nt][c], x[0][nt][c + 2]);
+                if constexpr (K == 2) top = fmaxf(top, fmaxf(x[K - 1][nt][c], x[K - 1][nt][c + 2]));
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const float least = __shfl_sync(0xffffffffu, low[nt][c], g * 4 + t);
-                    float4 y;
-                    y.x = fmaf(o[nt][2 * g][c], 16777216.f, least);
-                    y.y = fmaf(o[nt][2 * g + 1][c], 1048576.f, least);
-                    y.z = fmaf(o[nt][2 * g][c + 2], 16777216.f, least);
-                    y.w = fmaf(o[nt][2 * g + 1][c + 2], 1048576.f, least);
-                    *reinterpret_cast<float4*>(line + 32 * g + 4 * g8) = y;
-                }
-                if (g8 == 0) line[DP] = sum == 0.f ? LOWEST : m[nt][c], line[DP + 1] = sum;  // nothing seen: no reference either
+                for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                // a column's first tiles set its reference; one that sees nothing of them sees nothing of later ones
+                const float up = (first_tile || top > 2.f) && top != -INFINITY ? top - 1.f : 0.f;
+                m[nt][c] += up;
+#pragma unroll
+                for (int u = 0; u < K; ++u) x[u][nt][c] -= up, x[u][nt][c + 2] -= up;
+                const float keep = first_tile ? 1.f : ex2(-up);
+                low[nt][c] *= keep;
+#pragma unroll
+                for (int q = 0; q < 2 * G; ++q) o[nt][q][c] *= keep, o[nt][q][c + 2] *= keep;
             }
+        first_tile = false;
+    }
+    // ---- values: scales of tokens 2 t, 2 t + 1 (sa) and 2 t + 8, 2 t + 9 (sb), group by group; minima likewise, of group g8
+#pragma unroll
+    for (int u = 0; u < K; ++u) {
+        const uint32_t pv = tile[u] + 512 * G + 2 * t * 8 * G + 4 * G;
+        uint32_t sa[G], sb[G], ma = 0, mb = 0;
+        pair_halves<G>(sa, pv, pv + 8 * G);
+        pair_halves<G>(sb, pv + 64 * G, pv + 72 * G);
+        if (g8 < G) {
+            const uint32_t pm = pv + 2 * G + 2 * g8;
+            ma = load_half(pm) | load_half(pm + 8 * G) << 16;
+            mb = load_half(pm + 64 * G) | load_half(pm + 72 * G) << 16;
+        } else if (g8 == G) ma = mb = 0x3c003c00u;  // ones
+        uint32_t v0[G], v1[G];
+        load_words<G>(v0, tile[u] + 256 * G + lane * 4 * G);
+        load_words<G>(v1, tile[u] + 384 * G + lane * 4 * G);
+        if (!whole) {
+            // What a query does not see must not reach its sums, not even times 0: a token with a parameter that is not finite is taken
+            // out here, and the sums of those that do see it become NaN in that group.
+            const uint32_t ra = finite_halves(ma), rb = finite_halves(mb);
+            uint32_t bad = 0;  // of group g8: tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const uint32_t fa = finite_halves(sa[g]), fb = finite_halves(sb[g]);
+                // the lanes of column t that hold group g's minima say whether those are finite
+                const uint32_t ga = __shfl_sync(0xffffffffu, ra, g * 4 + t) & fa, gb = __shfl_sync(0xffffffffu, rb, g * 4 + t) & fb;
+                sa[g] &= ga, sb[g] &= gb;
+                if (g8 == g) bad = (~ga & 1u) | (~(ga >> 16) & 1u) << 1 | (~gb & 1u) << 8 | (~(gb >> 16) & 1u) << 9;
+            }
+            if (g8 < G) ma &= ra, mb &= rb;
+            if (__any_sync(0xffffffffu, bad != 0)) {
+                uint32_t tokens = bad << (2 * t);  // bit k: token k of the tile, over the four lanes of a row
+                tokens |= __shfl_xor_sync(0xffffffffu, tokens, 1);
+                tokens |= __shfl_xor_sync(0xffffffffu, tokens, 2);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int see = r.last[nt][c] - token - u * KV4_TILE;  // tokens 0 .. see of the tile
+                        const uint32_t seen = see < 0 ? 0u : see >= 15 ? 0xffffu : (2u << see) - 1u;
+                        if (g8 < G && (tokens & seen)) low[nt][c] = __int_as_float(0x7fffffff);
+                    }
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t p0 = transpose_8x8(pack_half2(ex2(x[u][nt][0]), ex2(x[u][nt][1]))), p1 = transpose_8x8(pack_half2(ex2(x[u][nt][2]), ex2(x[u][nt][3])));
+            mma_16816(low[nt], ma, 0u, mb, 0u, p0, p1);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const uint32_t h0 = v0[g] >> 8, h1 = v1[g] >> 8, q0 = mul_half2(p0, sa[g]), q1 = mul_half2(p1, sb[g]);
+                mma_16816(o[nt][2 * g], v0[g] & 0x000f000fu, h0 & 0x000f000fu, v1[g] & 0x000f000fu, h1 & 0x000f000fu, q0, q1);
+                mma_16816(o[nt][2 * g + 1], v0[g] & 0x00f000f0u, h0 & 0x00f000f0u, v1[g] & 0x00f000f0u, h1 & 0x00f000f0u, q0, q1);
+            }
+        }
+    }
+}
+
+// this warp's result: COLS lines of DP numerators, reference and denominator
+template <int G, int NT> __device__ __forceinline__ void Acc<G, NT>::store(float* lines) const {
+    const int lane = threadIdx.x & 31, g8 = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float* line = lines + (nt * 8 + 2 * t + c) * LINE;
+            const float sum = __shfl_sync(0xffffffffu, low[nt][c], G * 4 + t);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const float least = __shfl_sync(0xffffffffu, low[nt][c], g * 4 + t);
+                float4 y;
+                y.x = fmaf(o[nt][2 * g][c], 16777216.f, least);
+                y.y = fmaf(o[nt][2 * g + 1][c], 1048576.f, least);
+                y.z = fmaf(o[nt][2 * g][c + 2], 16777216.f, least);
+                y.w = fmaf(o[nt][2 * g + 1][c + 2], 1048576.f, least);
+                *reinterpret_cast<float4*>(line + 32 * g + 4 * g8) = y;
+            }
+            if (g8 == 0) line[DP] = sum == 0.f ? LOWEST : m[nt][c], line[DP + 1] = sum;  // nothing seen: no reference either
+        }
+}
+
+// ---------------------------------------------------------------------------------------------------- a warp's tiles
+// Tiles from .. to of a request go round the units (warps) in pairs, through each warp's ring.  Lane l looks up the l-th of 32 tiles at a
+// time in the block table, 32 tiles ahead of their use.  Two tiles a step: the waits, the bookkeeping and the vote on the
+// maximum are paid once for both.
+template <int G> struct Feed {
+    static constexpr int TB = kv4_tile_bytes(G);
+    const Kv4AttnArgs& a;
+    const int lane;
+    const uint32_t ring;  // offset in shared memory
+    const int* table;
+    int kvh, start, step, count, issued, in, out;  // tiles of this warp; tiles asked for; the stages to be filled and used next
+    unsigned there;       // bits 2 s, 2 s + 1: the tiles in stage s exist (their pages lie in the cache)
+    long long now, next;  // this lane's tile of the present 32 and of the next: its index in the cache, -1 for none
+
+    __device__ __forceinline__ Feed(const Kv4AttnArgs& args, int warp) : a(args), lane(threadIdx.x & 31), ring(warp * STAGES * 2 * TB) {}
+    __device__ __forceinline__ long long look(int base) const {
+        const int i = base + lane;
+        if (i >= count) return -1;
+        const int tiles_a_page = a.page / KV4_TILE, tile = start + (i >> 1) * step + (i & 1), col = tile / tiles_a_page, held = table[col];
+        if (held < 0 || held >= a.pages) {
+            atomicCAS(a.status, 0, ST_BAD_SLOT);
+            return -1;
+        }
+        return (static_cast<long long>(held) * a.kv_heads + kvh) * tiles_a_page + (tile - col * tiles_a_page);
+    }
+    // returns the pairs of this warp; pair i begins with tile from + 2 (unit + i units)
+    __device__ __forceinline__ int begin(const int* t, int head, int from, int to, int unit, int units) {
+        const int pairs = (to - from + 1) / 2, mine = pairs > unit ? (pairs - unit + units - 1) / units : 0;
+        table = t, kvh = head, start = from + 2 * unit, step = 2 * units, issued = in = out = 0, there = 0;
+        count = 2 * mine - (mine > 0 && ((to - from) & 1) && unit + (mine - 1) * units == pairs - 1);
+        now = look(0);
+        next = look(32);
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) issue();
+        return mine;
+    }
+    __device__ __forceinline__ void issue() {
+        if (issued < count) {
+            const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + ring + in * 2 * TB + lane * 16;
+            there &= ~(3u << 2 * in);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const long long tile = __shfl_sync(0xffffffffu, now, (issued & 31) + u);  // past the last: -1
+                if (tile >= 0) {
+                    there |= 1u << (2 * in + u);
+                    const uint8_t* src = a.cache + tile * TB + lane * 16;
+#pragma unroll
+                    for (int i = 0; i < (TB / 16 + 31) / 32; ++i)
+                        if (i * 32 + lane < TB / 16) cp_async_16(dst + u * TB + i * 512, src + i * 512);
+                }
+            }
+            in = in == STAGES - 1 ? 0 : in + 1;
+            issued += 2;
+            if ((issued & 31) == 0) {
+                now = next;
+                next = look(issued + 32);
+            }
+        }
+        cp_async_commit();
+    }
+    // waits for the next pair and gives it to `acc`; `token`: its first
+    template <int NT> __device__ __forceinline__ void take(Acc<G, NT>& acc, int token, const Rows<G, NT>& rows) {
+        cp_async_wait<STAGES - 2>();
+        __syncwarp();
+        const int tile = static_cast<int>(ring + out * 2 * TB);
+        const unsigned both = there >> 2 * out & 3u;
+        out = out == STAGES - 1 ? 0 : out + 1;
+        issue();  // into the stage that the whole warp is done with
+        if (both == 3u) acc.template step<2>({tile, tile + TB}, token, rows, lane);
+        else if (both == 1u) acc.template step<1>({tile}, token, rows, lane);
+        else if (both == 2u) acc.template step<1>({tile + TB}, token + KV4_TILE, rows, lane);
+    }
+};
+
+// The results of the CTA's warps for element e = (column, dim), joined: numerator, denominator, reference
+template <int G, int NT> __device__ __forceinline__ void join_warps(const float* lines, int c, int d, float& num, float& den, float& top) {
+    constexpr int DP = 32 * G, COLS = 8 * NT, LINE = DP + 4;
+    top = LOWEST, num = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, lines[(w * COLS + c) * LINE + DP]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const float* line = lines + (w * COLS + c) * LINE;
+        const float k = ex2(line[DP] - top);
+        num = fmaf(k, line[d], num);
+        den = fmaf(k, line[DP + 1], den);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- little work
+template <class T, int G, int NT>
+__global__ void __launch_bounds__(32 * W, NT == 1 ? 4 : 2) kv4_few_kernel(const Kv4AttnArgs a, int cluster) {
+    constexpr int DP = 32 * G, COLS = 8 * NT, LINE = DP + 4;
+    // what the CTAs of the cluster send one another: pieces of 128 numerators go to CTA (piece % cluster), every column's reference
+    // and denominator to all
+    constexpr int PIECES = (COLS * DP + 32 * W - 1) / (32 * W);
+    __shared__ float received[(PIECES + MAX_CLUSTER) * 32 * W];
+    __shared__ float terms[MAX_CLUSTER][COLS][2];
+
+    const int warp = threadIdx.x >> 5;
+    const int rank = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+    const int item = static_cast<int>(blockIdx.x / cluster), b = item / a.kv_heads, kvh = item - b * a.kv_heads;
+    const Request own(a, b);
+    const int units = cluster * W, unit = rank * W + warp;
+
+    for (int r0 = blockIdx.y * COLS; r0 < own.rows; r0 += gridDim.y * COLS) {
+        const long long end = min(own.before + (min(r0 + COLS, own.rows) - 1) / own.per, own.cap - 1);  // the last token that these rows see
+        const int tiles = end < 0 ? 0 : static_cast<int>(end / KV4_TILE) + 1;
+        Feed<G> feed(a, warp);
+        const int pairs = feed.begin(own.table, kvh, 0, tiles, unit, units);
+        Rows<G, NT> rows;
+        rows.template load<T>(a, own, kvh, r0);
+        Acc<G, NT> acc;
+        acc.reset();
+        for (int i = 0; i < pairs; ++i) feed.take(acc, 2 * (unit + i * units) * KV4_TILE, rows);
+        cp_async_wait<0>();
+        __syncthreads();  // the rings are free
+        float* lines = reinterpret_cast<float*>(smem);
+        acc.store(lines + warp * COLS * LINE);
         __syncthreads();
-        const int cols = min(COLS, rows - r0);
-        const float* all = reinterpret_cast<const float*>(smem);
+        const int cols = min(COLS, own.rows - r0);
+        const int owned = (PIECES + cluster - 1) / cluster;  // pieces of one CTA, at most
         for (int e = threadIdx.x; e < cols * DP; e += 32 * W) {
             const int c = e / DP, d = e % DP;
-            float top = LOWEST, num = 0.f, den = 0.f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) top = fmaxf(top, all[(w * COLS + c) * LINE + DP]);
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float* line = all + (w * COLS + c) * LINE;
-                const float k = ex2(line[DP] - top);
-                num = fmaf(k, line[d], num);
-                den = fmaf(k, line[DP + 1], den);
-            }
-            part[c][d] = num;
-            if (d == 0) part[c][DP] = top, part[c][DP + 1] = den;
-        }
-        if (cluster > 1) cluster_sync_all();
-        else __syncthreads();
-        for (int e = rank * 32 * W + threadIdx.x; e < cols * DP; e += cluster * 32 * W) {
-            const int c = e / DP, d = e % DP;
-            float num, den;
+            float num, den, top;
+            join_warps<G, NT>(lines, c, d, num, den, top);
             if (cluster == 1) {
-                num = part[c][d];
-                den = part[c][DP + 1];
+                write_out<T>(a, own.first, own.per, kvh, r0 + c, d, num, den);
             } else {
-                float top = LOWEST;
-                num = den = 0.f;
-                for (int k = 0; k < cluster; ++k) top = fmaxf(top, cluster_ld_float(cluster_map(&part[c][DP], k)));
-                for (int k = 0; k < cluster; ++k) {
-                    const float f = ex2(cluster_ld_float(cluster_map(&part[c][DP], k)) - top);
-                    num = fmaf(f, cluster_ld_float(cluster_map(&part[c][d], k)), num);
-                    den = fmaf(f, cluster_ld_float(cluster_map(&part[c][DP + 1], k)), den);
+                const int piece = e / (32 * W), owner = piece % cluster;
+                cluster_st_float(cluster_map(&received[(rank * owned + piece / cluster) * 32 * W + threadIdx.x], owner), num);
+                if (d < cluster) {
+                    cluster_st_float(cluster_map(&terms[rank][c][0], d), top);
+                    cluster_st_float(cluster_map(&terms[rank][c][1], d), den);
                 }
             }
-            if (d < a.D) {
-                const int r = r0 + c;
-                // no token seen: zeros; a NaN stays one
-                static_cast<T*>(a.out)[(static_cast<long long>(first + r / per) * a.heads + kvh * per + r % per) * a.D + d] = from_float<T>(den == 0.f ? 0.f : num / den);
+        }
+        if (cluster > 1) {
+            cluster_sync_all();
+            for (int piece = rank; piece * 32 * W < cols * DP; piece += cluster) {
+                const int e = piece * 32 * W + threadIdx.x, c = e / DP;
+                if (e >= cols * DP) break;
+                float top = LOWEST, num = 0.f, den = 0.f;
+                for (int k = 0; k < cluster; ++k) top = fmaxf(top, terms[k][c][0]);
+                for (int k = 0; k < cluster; ++k) {
+                    const float f = ex2(terms[k][c][0] - top);
+                    num = fmaf(f, received[(k * owned + piece / cluster) * 32 * W + threadIdx.x], num);
+                    den = fmaf(f, terms[k][c][1], den);
+                }
+                write_out<T>(a, own.first, own.per, kvh, r0 + c, e % DP, num, den);
+            }
+            if (r0 + gridDim.y * COLS < own.rows) cluster_sync_all();  // the next rows' results go to the same place
+        } else {
+            __syncthreads();
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- much work
+// The line: request by request, cached head by cached head, 8 NT rows by 8 NT rows, AHEAD units for what each of these costs besides its
+// tiles (queries, the first loads' latency, joining the warps: about 2 us, in which the CTA's warps do a dozen tiles), then
+// its tiles, one unit each.  CTA c takes units c * chunk .. (c + 1) * chunk.
+constexpr int AHEAD = 12;
+
+struct Cut {  // what the CTA's first tile belongs to, for the join
+    long long begin, end, chunk;  // of its tiles in the line; begin = -1: the CTA has no tiles
+    int first, per, kvh, r0, cols, pad;
+};
+
+__host__ __device__ constexpr long long cuts_bytes(int ctas) { return (static_cast<long long>(ctas) * sizeof(Cut) + 15) / 16 * 16; }
+
+__device__ __forceinline__ long long block_sum_before(long long v, long long* total, long long* buf) {  // exclusive prefix over the CTA's threads
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+    }
+    if (lane == 31) buf[warp] = inc;
+    __syncthreads();
+    long long before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        if (w < warp) before += buf[w];
+        all += buf[w];
+    }
+    *total = all;
+    return before + inc - v;
+}
+
+template <class T, int G, int NT>
+__global__ void __launch_bounds__(32 * W, NT == 1 ? 4 : 2) kv4_line_kernel(const Kv4AttnArgs a, int least) {
+    constexpr int DP = 32 * G, COLS = 8 * NT, LINE = DP + 4;
+    __shared__ long long sums[W], found[2];
+    const int tid = threadIdx.x, warp = tid >> 5;
+    asm volatile("griddepcontrol.launch_dependents;");  // the join may be set up; it waits for this grid's end by itself
+
+    // ---- where this CTA's piece lies
+    auto weight = [&](const Request& q) { return static_cast<long long>(a.kv_heads) * ((q.rows + COLS - 1) / COLS) * (q.tiles() + AHEAD); };
+    const int share = (a.batch + 32 * W - 1) / (32 * W);
+    const int b0 = min(tid * share, a.batch), b1 = min(b0 + share, a.batch);
+    long long mine = 0, total;
+    for (int b = b0; b < b1; ++b) mine += weight(Request(a, b));
+    const long long before = block_sum_before(mine, &total, sums);
+    const long long chunk = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(least));
+    long long pos = blockIdx.x * chunk;
+    const long long stop = min(pos + chunk, total);
+    Cut* cut = static_cast<Cut*>(a.workspace) + blockIdx.x;
+    if (pos >= stop) {
+        if (tid == 0) cut->begin = -1;
+        return;
+    }
+    if (before <= pos && pos < before + mine) {
+        long long at = before;
+        int b = b0;
+        for (;; ++b) {
+            const long long w = weight(Request(a, b));
+            if (pos < at + w) break;
+            at += w;
+        }
+        found[0] = b, found[1] = at;
+    }
+    __syncthreads();
+    int b = static_cast<int>(found[0]);
+    long long base = found[1];  // of request b in the line
+    float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + cuts_bytes(gridDim.x)) + static_cast<long long>(blockIdx.x) * 2 * COLS * LINE;
+    float* lines = reinterpret_cast<float*>(smem);  // the warps' results, where the rings are
+
+    // ---- piece by piece
+    bool first_piece = true;
+    if (tid == 0) cut->begin = -1;
+    while (pos < stop) {
+        const Request own(a, b);
+        const long long w = weight(own);
+        if (pos >= base + w) {
+            base += w;
+            ++b;
+            continue;
+        }
+        const int nb = own.tiles(), q_tiles = (own.rows + COLS - 1) / COLS;
+        const int item = static_cast<int>((pos - base) / (nb + AHEAD));
+        const long long begin = base + static_cast<long long>(item) * (nb + AHEAD) + AHEAD;  // its first tile
+        const int kvh = item / q_tiles, r0 = (item - kvh * q_tiles) * COLS, cols = min(COLS, own.rows - r0);
+        const int from = static_cast<int>(max(pos - begin, 0ll)), to = static_cast<int>(min(static_cast<long long>(nb), stop - begin));
+        const int count = to - from;
+        if (to <= 0) break;  // the piece ends ahead of its tiles
+        Feed<G> feed(a, warp);
+        // no query of the request sees a token: its one tile is not looked at
+        const int pairs = feed.begin(own.table, kvh, from, own.before + own.rows / own.per <= 0 ? from : to, warp, W);
+        Rows<G, NT> rows;
+        rows.template load<T>(a, own, kvh, r0);
+        Acc<G, NT> acc;
+        acc.reset();
+        for (int i = 0; i < pairs; ++i) feed.take(acc, (from + 2 * (warp + i * W)) * KV4_TILE, rows);
+        cp_async_wait<0>();
+        __syncthreads();  // the rings are free
+        acc.store(lines + warp * COLS * LINE);
+        __syncthreads();
+        if (first_piece && tid == 0) *cut = Cut{begin, begin + nb, chunk, own.first, own.per, kvh, r0, cols, 0};
+        const bool whole = count == nb;
+        float* part = parts + (begin > blockIdx.x * chunk ? COLS * LINE : 0);  // a piece that begins here, or one begun before
+        for (int e = tid; e < cols * DP; e += 32 * W) {
+            const int c = e / DP, d = e % DP;
+            float num, den, top;
+            join_warps<G, NT>(lines, c, d, num, den, top);
+            if (whole) {
+                write_out<T>(a, own.first, own.per, kvh, r0 + c, d, num, den);
+            } else {
+                part[c * LINE + d] = num;
+                if (d == 0) part[c * LINE + DP] = top, part[c * LINE + DP + 1] = den;
             }
         }
-        if (cluster > 1) cluster_sync_all();  // until here the other CTAs read this one's part
-        else __syncthreads();
+        __syncthreads();
+        pos = begin + to;
+        first_piece = false;
     }
+}
+
+constexpr int JT = 256;  // threads of a joining CTA
+
+// CTA c - 1 belongs to the start of CTA c's piece of the line.  If that cuts a (request, head, rows) in two, it joins a share of its
+// elements: all the cuts inside take one share each.
+template <class T, int G, int NT>
+__global__ void __launch_bounds__(JT) kv4_join_kernel(const Kv4AttnArgs a, int ctas) {
+    constexpr int DP = 32 * G, COLS = 8 * NT, LINE = DP + 4;
+    __shared__ float part[3][JT];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int c = blockIdx.x + 1, tid = threadIdx.x;
+    const Cut cut = static_cast<const Cut*>(a.workspace)[c];
+    if (cut.begin < 0 || cut.begin >= c * cut.chunk) return;  // no tiles, or no cut
+    const int first = static_cast<int>(cut.begin / cut.chunk), n = static_cast<int>((cut.end - 1) / cut.chunk) - first + 1;  // n CTAs share it: n - 1 cuts
+    const int all = cut.cols * DP, share = (all + n - 2) / (n - 1);
+    const int from = min((c - first - 1) * share, all), to = min(from + share, all);
+    const float* parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.workspace) + cuts_bytes(ctas)) + static_cast<long long>(first) * 2 * COLS * LINE;
+    const int second = cut.begin > first * cut.chunk ? COLS * LINE : 0;  // the first CTA's part lies behind that of its piece's start
+    int width = 1;
+    while (width < to - from && width < JT) width *= 2;
+    const int groups = JT / width, lane = tid % width, group = tid / width;
+    for (int e0 = from; e0 < to; e0 += width) {
+        const int e = e0 + lane, col = e / DP, d = e % DP;
+        float top = LOWEST, num = 0.f, den = 0.f;
+        if (e < to) {
+#pragma unroll 4
+            for (int k = group; k < n; k += groups) {
+                const float* line = parts + static_cast<long long>(k) * 2 * COLS * LINE + (k == 0 ? second : 0) + col * LINE;
+                const float m = line[DP], l = line[DP + 1], x = line[d], t = fmaxf(top, m), keep = ex2(top - t), f = ex2(m - t);
+                num = fmaf(f, x, num * keep);
+                den = fmaf(f, l, den * keep);
+                top = t;
+            }
+        }
+        for (int half = groups / 2; half > 0; half /= 2) {  // the upper half of the groups hands over to the lower
+            part[0][tid] = top, part[1][tid] = num, part[2][tid] = den;
+            __syncthreads();
+            if (group < half) {
+                const int at = tid + half * width;
+                const float m = part[0][at], t = fmaxf(top, m), keep = ex2(top - t), f = ex2(m - t);
+                num = fmaf(f, part[1][at], num * keep);
+                den = fmaf(f, part[2][at], den * keep);
+                top = t;
+            }
+            __syncthreads();
+        }
+        if (group == 0 && e < to) write_out<T>(a, cut.first, cut.per, cut.kvh, cut.r0 + col, d, num, den);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- launches
+constexpr int SMS = 148;
+constexpr int LEAST = 2 * W;  // tiles of a CTA's piece, at least: below that the join costs more than it saves
+template <int NT> constexpr int line_ctas() { return SMS * (NT == 1 ? 4 : 2); }
+
+template <class K> cudaError_t allow_smem(K kernel, int bytes) {
+    return bytes > 32 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : cudaSuccess;  // more than 48 KB with the static part
 }
 
 template <class T, int G, int NT> cudaError_t launch(const Kv4AttnArgs& a, long long max_q_len, cudaStream_t st) {
     constexpr int COLS = 8 * NT;
-    constexpr int ring = W * STAGES * kv4_tile_bytes(G), merge = W * COLS * (32 * G + 4) * 4;
-    constexpr int smem = ring > merge ? ring : merge;
+    constexpr int ring = W * STAGES * 2 * kv4_tile_bytes(G), merge = W * COLS * (32 * G + 4) * 4, smem = ring > merge ? ring : merge;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    cfg.blockDim = dim3(32 * W);
+    cfg.stream = st;
+    cfg.attrs = at;
+    if (a.workspace) {
+        constexpr int ctas = line_ctas<NT>();
+        cudaError_t e = allow_smem(kv4_line_kernel<T, G, NT>, smem);
+        if (e != cudaSuccess) return e;
+        cfg.gridDim = dim3(ctas);
+        cfg.dynamicSmemBytes = smem;
+        e = cudaLaunchKernelEx(&cfg, kv4_line_kernel<T, G, NT>, a, LEAST);
+        if (e != cudaSuccess) return e;
+        cfg.gridDim = dim3(ctas - 1);
+        cfg.blockDim = dim3(JT);
+        cfg.dynamicSmemBytes = 0;
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, G, NT>, a, ctas);
+    }
     const long long items = static_cast<long long>(a.batch) * a.kv_heads;
     const long long q_tiles = (max_q_len * (a.heads / a.kv_heads) + COLS - 1) / COLS;
     const long long tiles = (a.table_width * a.page + KV4_TILE - 1) / KV4_TILE;
-    // as many CTAs to a (request, head) as fill the GPU (4 to an SM), but at least four tiles to a warp
+    // as many CTAs to a (request, head) as fill the GPU (4 to an SM), but at least two tiles to a warp
     int cluster = 1;
-    while (cluster < 8 && items * q_tiles * cluster < 4 * 148 && tiles >= 8 * W * cluster) cluster *= 2;
-    auto kernel = kv4_few_kernel<T, G, NT>;
-    if (smem + merge / W > 48 * 1024) {  // with the static part
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return e;
-    }
-    cudaLaunchConfig_t cfg = {};
+    while (cluster < MAX_CLUSTER && items * q_tiles * cluster < 4 * SMS && tiles >= 4 * W * cluster) cluster *= 2;
+    const cudaError_t e = allow_smem(kv4_few_kernel<T, G, NT>, smem);
+    if (e != cudaSuccess) return e;
     cfg.gridDim = dim3(static_cast<unsigned>(items * cluster), static_cast<unsigned>(q_tiles < 65535 ? q_tiles : 65535));
-    cfg.blockDim = dim3(32 * W);
     cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = cluster;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, a, cluster);
+    return cudaLaunchKernelEx(&cfg, kv4_few_kernel<T, G, NT>, a, cluster);
 }
 
 template <class T, int G> cudaError_t by_rows(const Kv4AttnArgs& a, long long max_q_len, cudaStream_t st) {
@@ -509,6 +835,16 @@ template <class T> cudaError_t by_groups(const Kv4AttnArgs& a, long long max_q_l
 }
 
 }  // namespace
+
+long long kv4_few_workspace(long long heads, long long kv_heads, int D, long long max_q_len) {
+    const int nt = max_q_len * (heads / kv_heads) <= 8 ? 1 : 2, ctas = nt == 1 ? line_ctas<1>() : line_ctas<2>();
+    return cuts_bytes(ctas) + static_cast<long long>(ctas) * 2 * 8 * nt * (32 * kv4_groups(D) + 4) * 4;
+}
+
+bool kv4_few_uses_workspace(long long batch, long long heads, long long kv_heads, long long tokens, long long max_q_len) {
+    const long long rows = max_q_len * (heads / kv_heads), cols = rows <= 8 ? 8 : 16;
+    return batch * kv_heads * ((rows + cols - 1) / cols) * ((tokens + KV4_TILE - 1) / KV4_TILE) >= LINE_FROM;
+}
 
 cudaError_t kv4_attention_few(const Kv4AttnArgs& a, bool bf16, long long max_q_len, cudaStream_t st) {
     return bf16 ? by_groups<__nv_bfloat16>(a, max_q_len, st) : by_groups<__half>(a, max_q_len, st);

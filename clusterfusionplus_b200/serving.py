@@ -15,6 +15,7 @@ caller.  Like the rest of the package these functions validate, allocate their r
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -176,6 +177,11 @@ def kv4_read(cache, slot_map, head_dim: int, dtype=torch.float16) -> Tuple[torch
     return key, value
 
 
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(batch: int, heads: int, kv_heads: int, head_dim: int, max_tokens: int, max_q_len: int) -> int:
+    return lib.cf_kv4_attention_workspace(batch, heads, kv_heads, head_dim, max_tokens, max_q_len)
+
+
 def kv4_attention(query, cache, block_table, kv_lens, qo_indptr=None, max_q_len: int = 1, scale: Optional[float] = None, out=None) -> torch.Tensor:
     """Causal attention of query [rows, heads, head_dim] (fp16 or bf16, a slice of a fused projection is fine) over the paged 4-bit cache;
     [rows, heads, head_dim].  heads is a multiple of the cache's heads.
@@ -196,8 +202,10 @@ def kv4_attention(query, cache, block_table, kv_lens, qo_indptr=None, max_q_len:
         out = torch.empty((rows, heads, dim), dtype=query.dtype, device=query.device)
     elif not isinstance(out, torch.Tensor) or out.get_device() != dev or out.shape != query.shape or out.dtype is not query.dtype or not out.is_contiguous():
         _complain(out, "out", dev, 3, (query.dtype,), f"a contiguous {tuple(query.shape)}")
+    need = _attention_workspace(batch, heads, kv_heads, dim, width * page, int(max_q_len))
+    work = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None  # of this call alone: graphs and streams share nothing
     check(lib.cf_kv4_attention(qp, _HALVES[query.dtype], rows, heads, dim, q0, q1, cp, pages, page, kv_heads, tp, width, apart, lp, ip, batch, int(max_q_len),
-                               dim ** -0.5 if scale is None else float(scale), out.data_ptr(), _raw_stream(dev)))
+                               dim ** -0.5 if scale is None else float(scale), work.data_ptr() if need else None, need, out.data_ptr(), _raw_stream(dev)))
     return out
 
 

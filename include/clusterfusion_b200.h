@@ -466,12 +466,17 @@ int cf_kv4_read(const void* cache, int64_t pages, int64_t page_size, int64_t kv_
  * tokens, which lie in the pages block_table[b][0 ..].  A query that sees no token gives zeros.  Rows of out that no
  * request owns stay as they are.  A page number outside the cache is skipped as if its tokens were not there, and recorded
  * (cf_get_status 8); tokens beyond table_width pages are not there either.  max_q_len: the most query rows a request
- * has, for the choice and the size of the launch; the result does not depend on it.  scale: of q . k (1 / sqrt(head_dim)
- * as a rule). */
+ * has, for the choice and the size of the launch; what the call computes does not depend on it.  scale: of q . k (1 /
+ * sqrt(head_dim) as a rule).  workspace: scratch of cf_kv4_attention_workspace(...) bytes, 16-byte aligned, of any content, which no
+ * call that may overlap uses; with it requests of different lengths share the GPU evenly (a second launch joins the parts).
+ * NULL works too, and is the faster way where that function gives 0 (max_tokens: table_width * page_size). */
+int64_t cf_kv4_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens,
+                                   int64_t max_q_len);
 int cf_kv4_attention(const void* query, int dtype, int64_t rows, int64_t heads, int64_t head_dim, int64_t query_token_stride,
                      int64_t query_head_stride, const void* cache, int64_t pages, int64_t page_size, int64_t kv_heads,
                      const int* block_table, int64_t table_width, int64_t table_stride, const int* kv_lens,
-                     const int* qo_indptr, int64_t batch, int64_t max_q_len, float scale, void* out, void* stream);
+                     const int* qo_indptr, int64_t batch, int64_t max_q_len, float scale, void* workspace,
+                     int64_t workspace_bytes, void* out, void* stream);
 
 /* Log probabilities from logits [rows][vocab] (fp16, bf16 or fp32, row_stride elements apart, natural alignment):
  *   logprobs[r] = log softmax(logits[r])[tokens[r]] (tokens int32 or int64, token_bytes 4 or 8; -inf for a token outside the

@@ -59,10 +59,11 @@ def test_read_refusals(kw, match):
 @pytest.mark.parametrize("kw,match", [
     (dict(dim=100), "head_dim"), (dict(heads=5), "query heads"), (dict(heads=2), "query heads"), (dict(rows=-1), "rows"), (dict(batch=0), "batch"), (dict(qo=None), "query rows"),
     (dict(max_q=0), "max_q_len"), (dict(width=0), "block table"), (dict(stride=3), "block table"), (dict(query=None), "null"), (dict(out=None), "null"),
-    (dict(qts=1020), "strides"), (dict(query=ctypes.c_void_p(8)), "aligned"), (dict(dtype=2), "dtype"), (dict(page=17), "page size")])
+    (dict(qts=1020), "strides"), (dict(query=ctypes.c_void_p(8)), "aligned"), (dict(dtype=2), "dtype"), (dict(page=17), "page size"),
+    (dict(work=ONE, work_bytes=16, width=1 << 14, stride=1 << 14), "workspace"), (dict(work=ctypes.c_void_p(8), work_bytes=1 << 30, width=1 << 14, stride=1 << 14), "workspace")])
 def test_attention_refusals(kw, match):
     a = dict(query=ONE, dtype=0, rows=3, heads=8, dim=128, qts=1024, qhs=128, cache=ONE, pages=4, page=16, kv_heads=4, table=ONE, width=8, stride=8, kv_lens=ONE, qo=ONE, batch=4,
-             max_q=1, scale=0.1, out=ONE, stream=None)
+             max_q=1, scale=0.1, work=None, work_bytes=0, out=ONE, stream=None)
     refused("cf_kv4_attention", list((a | kw).values()), match)
 
 
@@ -79,7 +80,7 @@ def test_nothing_to_do_is_fine():
     lib = _lib.lib
     assert lib.cf_kv4_append(None, None, 0, 0, 2, 128, 256, 128, 256, 128, None, None, 4, 16, None) == 0
     assert lib.cf_kv4_read(None, 4, 16, 2, 128, None, 0, None, None, 0, None) == 0
-    assert lib.cf_kv4_attention(None, 0, 0, 8, 128, 1024, 128, None, 4, 16, 4, None, 8, 8, None, ONE, 4, 1, 0.1, None, None) == 0
+    assert lib.cf_kv4_attention(None, 0, 0, 8, 128, 1024, 128, None, 4, 16, 4, None, 8, 8, None, ONE, 4, 1, 0.1, None, 0, None, None) == 0
     assert lib.cf_token_logprobs(None, 0, 0, 100, 100, None, 8, 0, None, None, None, None, None) == 0
 
 

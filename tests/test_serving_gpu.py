@@ -294,6 +294,14 @@ def attention_case(lens, counts, heads, kv_heads, D, page, dtype, seed, extra_co
     return qkv[:, :heads], cache, table, starts
 
 
+@pytest.fixture(params=["by_size", "line"])
+def schedule(request, monkeypatch):
+    """Both ways of dealing out the work: the one that the sizes choose (little work: clusters), and the line of tiles with a workspace."""
+    if request.param == "line":
+        from clusterfusionplus_b200 import serving
+        monkeypatch.setattr(serving, "_attention_workspace", lambda *a: 64 << 20)
+
+
 def check_attention(lens, counts, heads, kv_heads, D, page, dtype, seed=1, scale=None, max_q=None):
     import clusterfusionplus_b200 as cf
     q, cache, table, starts = attention_case(lens, counts, heads, kv_heads, D, page, dtype, seed)
@@ -307,14 +315,14 @@ def check_attention(lens, counts, heads, kv_heads, D, page, dtype, seed=1, scale
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("lens", [[1], [15, 16, 17], [0, 1, 300], [257, 64, 1000, 31]])
 @pytest.mark.parametrize("heads,kv_heads,D,page", [(4, 4, 128, 16), (8, 2, 64, 32), (8, 1, 128, 64), (5, 1, 80, 16), (3, 3, 96, 128), (16, 1, 16, 48), (6, 3, 120, 16), (24, 1, 128, 16), (40, 1, 64, 16)])
-def test_attention_of_single_tokens(cuda_device, dtype, lens, heads, kv_heads, D, page):
+def test_attention_of_single_tokens(cuda_device, schedule, dtype, lens, heads, kv_heads, D, page):
     check_attention(lens, [1] * len(lens), heads, kv_heads, D, page, dtype, seed=sum(lens) + heads)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("lens,counts", [([5], [5]), ([40, 3, 0, 129], [2, 3, 0, 7]), ([130, 200], [130, 1]), ([64, 500], [33, 17]), ([3, 20], [6, 1]), ([300], [200]), ([0, 2], [4, 0])])
 @pytest.mark.parametrize("heads,kv_heads,D,page", [(4, 4, 128, 16), (8, 2, 64, 32), (5, 1, 80, 16), (8, 1, 128, 64), (2, 2, 96, 16), (40, 2, 128, 16)])
-def test_attention_of_several_queries_a_request(cuda_device, dtype, lens, counts, heads, kv_heads, D, page):
+def test_attention_of_several_queries_a_request(cuda_device, schedule, dtype, lens, counts, heads, kv_heads, D, page):
     """Drafted tokens, whole prompts, chunks behind a history; more queries than cached tokens leave rows that see nothing."""
     got = check_attention(lens, counts, heads, kv_heads, D, page, dtype, seed=sum(lens) + sum(counts))
     row = 0
@@ -327,28 +335,41 @@ def test_attention_of_several_queries_a_request(cuda_device, dtype, lens, counts
 
 @pytest.mark.parametrize("max_q", [1, 3, 1000])
 @pytest.mark.parametrize("lens,counts", [([40, 300], [2, 150]), ([600, 7], [1, 1])])
-def test_attention_does_not_depend_on_the_hint(cuda_device, max_q, lens, counts):
+def test_attention_does_not_depend_on_the_hint(cuda_device, schedule, max_q, lens, counts):
     check_attention(lens, counts, 8, 2, 128, 16, torch.float16, max_q=max_q)
 
 
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.25, 3.0])
-def test_attention_scale(cuda_device, scale):
+def test_attention_scale(cuda_device, schedule, scale):
     check_attention([70, 9], [3, 1], 4, 2, 64, 16, torch.float16, scale=scale)
 
 
 @pytest.mark.parametrize("counts", [[1], [9], [140]])
-def test_attention_long_cache(cuda_device, counts):
+def test_attention_long_cache(cuda_device, schedule, counts):
     check_attention([20000], counts, 2, 1, 64, 64, torch.float16)
 
 
-def test_attention_many_requests(cuda_device):
+def test_attention_many_requests(cuda_device, schedule):
     rng = random.Random(4)
     lens = [rng.randint(0, 90) for _ in range(700)]
     check_attention(lens, [min(1, n) for n in lens], 2, 1, 64, 16, torch.float16)
 
 
+def test_attention_of_uneven_requests(cuda_device, schedule):
+    """Pieces of the line that begin and end everywhere: one long request among many short ones, ends on and off the tiles' borders."""
+    check_attention([1, 5000, 16, 0, 17, 300, 1600, 1], [1, 1, 1, 1, 1, 1, 1, 0], 8, 4, 128, 16, torch.float16, seed=2)
+    check_attention([64] * 40, [1] * 40, 4, 4, 64, 32, torch.bfloat16, seed=3)
+    check_attention([7000, 3, 900], [2, 3, 1], 16, 2, 96, 48, torch.float16, seed=4)
+
+
+def test_attention_chooses_the_line_by_itself(cuda_device):
+    from clusterfusionplus_b200 import serving
+    assert serving._attention_workspace(16, 8, 8, 128, 16384, 1) > 0 and serving._attention_workspace(1, 8, 8, 128, 1024, 1) == 0
+    check_attention([16000, 3000, 10, 9000], [1, 1, 1, 1], 8, 8, 128, 64, torch.float16, seed=6)
+
+
 @pytest.mark.parametrize("counts", [[1, 1, 1], [5, 70, 1]])
-def test_attention_leaves_other_rows(cuda_device, counts):
+def test_attention_leaves_other_rows(cuda_device, schedule, counts):
     """Rows before the first request's and behind the last one's stay as they were, and padded requests own none."""
     import clusterfusionplus_b200 as cf
     q, cache, table, starts = attention_case([30, 90, 2], counts, 4, 2, 64, 16, torch.float16, 3)
@@ -362,7 +383,7 @@ def test_attention_leaves_other_rows(cuda_device, counts):
 
 
 @pytest.mark.parametrize("counts", [[1, 1], [20, 90]])
-def test_attention_skips_and_reports_bad_pages(cuda_device, counts):
+def test_attention_skips_and_reports_bad_pages(cuda_device, schedule, counts):
     import clusterfusionplus_b200 as cf
     q, cache, table, starts = attention_case([100, 130], counts, 4, 2, 128, 16, torch.float16, 8)
     table[0][2], table[1][1], table[1][5] = -5, cache.shape[0], 2147483647
@@ -377,7 +398,7 @@ def test_attention_skips_and_reports_bad_pages(cuda_device, counts):
 
 
 @pytest.mark.parametrize("count", [1, 7, 80])
-def test_attention_ignores_what_lies_behind_the_last_token(cuda_device, count):
+def test_attention_ignores_what_lies_behind_the_last_token(cuda_device, schedule, count):
     """Stale NaN and infinities in the rows behind a request's end and in its page's other rows."""
     import clusterfusionplus_b200 as cf
     q, cache, table, starts = attention_case([83], [count], 4, 2, 128, 32, torch.float16, 21)
@@ -393,7 +414,7 @@ def test_attention_ignores_what_lies_behind_the_last_token(cuda_device, count):
 
 
 @pytest.mark.parametrize("count", [1, 40])
-def test_attention_passes_on_nan_that_it_sees(cuda_device, count):
+def test_attention_passes_on_nan_that_it_sees(cuda_device, schedule, count):
     import clusterfusionplus_b200 as cf
     q, cache, table, starts = attention_case([60, 60], [count, count], 2, 2, 64, 16, torch.float16, 22)
     x = rows_of(1, 2, 64, torch.float16, 3)
@@ -405,7 +426,7 @@ def test_attention_passes_on_nan_that_it_sees(cuda_device, count):
 
 @pytest.mark.parametrize("size", [2.0 ** -14, 2.0 ** -6, 200.0, 5000.0])
 @pytest.mark.parametrize("count", [1, 30])
-def test_attention_of_small_and_large_values(cuda_device, size, count):
+def test_attention_of_small_and_large_values(cuda_device, schedule, size, count):
     """Values from fp16's smallest normal number to thousands; keys of unit size."""
     import clusterfusionplus_b200 as cf
     D, T = 128, 150
@@ -421,7 +442,7 @@ def test_attention_of_small_and_large_values(cuda_device, size, count):
 
 
 @pytest.mark.parametrize("size", [1e-3, 40.0, 3000.0])
-def test_attention_of_small_and_large_queries(cuda_device, size):
+def test_attention_of_small_and_large_queries(cuda_device, schedule, size):
     """Large queries make one-hot probabilities; bf16 queries reach beyond fp16."""
     import clusterfusionplus_b200 as cf
     D = 64
