@@ -23,12 +23,6 @@ __device__ int g_kv4_status = 0;
 
 __device__ __forceinline__ void report_bad_slot() { atomicCAS(&g_kv4_status, 0, ST_BAD_SLOT); }
 
-template <class T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <class T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // Both kernels: half a warp for a (token, head), lane l of the half holds dims 8 l .. 8 l + 7 (16 bytes) of the key and the
 // value, four lanes a group.  A warp then moves 2 KB of keys and values with two loads a lane, and the index arithmetic, the
@@ -36,54 +30,73 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 constexpr int CT = 256;          // threads of a CTA
 constexpr int ITEMS = CT / 16;   // (token, head) pairs of a CTA
 
-template <class T> __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-    const uint2 raw[2] = {*reinterpret_cast<const uint2*>(p), *reinterpret_cast<const uint2*>(p + 4)};  // rows are 8-byte aligned
-    const T* e = reinterpret_cast<const T*>(raw);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_float<T>(e[i]);
-}
+// pairs of the 16-bit types
+template <class T> struct Two;
+template <> struct Two<__half> {
+    using P = __half2;
+    static constexpr uint32_t INF = 0x04000400u;  // what carries an exponent of all ones into bit 15
+    static __device__ __forceinline__ float2 floats(P v) { return __half22float2(v); }
+};
+template <> struct Two<__nv_bfloat16> {
+    using P = __nv_bfloat162;
+    static constexpr uint32_t INF = 0x00800080u;
+    static __device__ __forceinline__ float2 floats(P v) { return __bfloat1622float2(v); }
+};
 
-// Codes of this lane's eight values (nibble i: value i), scale and minimum of its group of four lanes.
-__device__ __forceinline__ unsigned quantise8(const float (&x)[8], bool real, __half* scale, __half* low) {
-    float lo = 65504.f, hi = -65504.f, v[8];
-    unsigned bad = 0;
+// Codes of this lane's eight values (raw words, nibble i: value i), scale and minimum of its group of four lanes.  Extremes and the test
+// for NaN and infinities work on the 16-bit pairs; codes are rounded by adding 1.5 * 2^23, which leaves them in the low mantissa
+// bits (conversions run at a quarter of the rate), and put together by multiply-adds.
+template <class T> __device__ __forceinline__ unsigned quantise8(const uint32_t (&raw)[4], bool real, __half* scale, __half* low) {
+    using P = typename Two<T>::P;
+    const P* p = reinterpret_cast<const P*>(raw);
+    const float2 hi2 = Two<T>::floats(__hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]))), lo2 = Two<T>::floats(__hmin2(__hmin2(p[0], p[1]), __hmin2(p[2], p[3])));
+    float hi = real ? fminf(fmaxf(hi2.x, hi2.y), 65504.f) : -65504.f, lo = real ? fmaxf(fminf(lo2.x, lo2.y), -65504.f) : 65504.f;
+    uint32_t over = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        bad |= !(fabsf(x[i]) <= 3.4028234663852886e38f);  // NaN and the infinities
-        v[i] = fminf(fmaxf(x[i], -65504.f), 65504.f);
-        lo = fminf(lo, v[i]);
-        hi = fmaxf(hi, v[i]);
-    }
-    if (!real) lo = 65504.f, hi = -65504.f, bad = 0;
+    for (int i = 0; i < 4; ++i) over |= (raw[i] & 0x7fff7fffu) + Two<T>::INF;
+    unsigned bad = real && (over & 0x80008000u);
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         bad |= __shfl_xor_sync(0xffffffffu, bad, o);
     }
+    lo = fminf(lo, 65504.f), hi = fmaxf(hi, -65504.f);  // bf16 beyond fp16 on one side only
     const __half m = __float2half_rn(lo);
     const float mf = __half2float(m);
     const __half s = __float2half_rn((hi - mf) / 15.f);
-    const float sf = __half2float(s), r = 1.f / sf;
+    const float sf = __half2float(s);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(sf));
     unsigned codes = 0;
-    if (real && sf > 0.f) {
-        // rint((v - m) / s) by the reciprocal: off by a few 2^-24 of at most 16, which matters only next to a half; there it is divided
-        float q[8];
-        bool near_half = false;
+    if (real && sf > 0.f && !bad) {
+        // rint((v - m) / s) by the reciprocal: off by a few 2^-24 of at most 22, which matters only next to a half; there it is divided
+        constexpr float MAGIC = 12582912.f;
+        float q[8], off = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            q[i] = (v[i] - mf) * r;
-            near_half |= fabsf(fabsf(q[i] - rintf(q[i])) - 0.5f) < 1e-5f;
+        for (int i = 0; i < 4; ++i) {
+            float2 v = Two<T>::floats(p[i]);
+            if (sizeof(T) == 2 && Two<T>::INF == 0x00800080u) v.x = fminf(fmaxf(v.x, -65504.f), 65504.f), v.y = fminf(fmaxf(v.y, -65504.f), 65504.f);
+            q[2 * i] = (v.x - mf) * r;
+            q[2 * i + 1] = (v.y - mf) * r;
         }
-        if (near_half)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = (v[i] - mf) / sf;
+        for (int i = 0; i < 8; ++i) off = fmaxf(off, fabsf(q[i] - ((q[i] + MAGIC) - MAGIC)));
+        if (off > 0.49999f) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) codes |= static_cast<unsigned>(__float2int_rn(fminf(fmaxf(q[i], 0.f), 15.f))) << (4 * i);
+            for (int i = 0; i < 4; ++i) {
+                const float2 v = Two<T>::floats(p[i]);
+                q[2 * i] = (fminf(fmaxf(v.x, -65504.f), 65504.f) - mf) / sf;
+                q[2 * i + 1] = (fminf(fmaxf(v.y, -65504.f), 65504.f) - mf) / sf;
+            }
+        }
+#pragma unroll
+        for (int i = 7; i >= 0; --i) codes = codes * 16 + __float_as_uint(fminf(fmaxf(q[i], 0.f), 15.f) + MAGIC);
+        codes -= 0x4b400000u * 0x11111111u;
     }
     *scale = bad ? __ushort_as_half(0x7fff) : s;
     *low = m;
-    return bad ? 0u : codes;
+    return codes;
 }
 
 // the tile that holds a row, and the row in it
@@ -106,15 +119,15 @@ __global__ void __launch_bounds__(CT) kv4_append_kernel(const T* __restrict__ ke
     const bool kept = slot >= 0 && slot < slots;  // a padded row is skipped
     const int dim = 8 * l;
     const bool real = kept && dim < D;
-    float xk[8], xv[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) xk[i] = xv[i] = 0.f;
+    uint2 k0 = make_uint2(0, 0), k1 = k0, v0 = k0, v1 = k0;  // rows are 8-byte aligned
     if (real) {
-        load8(key + tok * k_ts + head * k_hs + dim, xk);
-        load8(value + tok * v_ts + head * v_hs + dim, xv);
+        const uint2* kp = reinterpret_cast<const uint2*>(key + tok * k_ts + head * k_hs + dim);
+        const uint2* vp = reinterpret_cast<const uint2*>(value + tok * v_ts + head * v_hs + dim);
+        k0 = kp[0], k1 = kp[1], v0 = vp[0], v1 = vp[1];
     }
+    const uint32_t xk[4] = {k0.x, k0.y, k1.x, k1.y}, xv[4] = {v0.x, v0.y, v1.x, v1.y};
     __half ks, km, vs, vm;
-    const unsigned kc = quantise8(xk, real, &ks, &km), vc = quantise8(xv, real, &vs, &vm);
+    const unsigned kc = quantise8<T>(xk, real, &ks, &km), vc = quantise8<T>(xv, real, &vs, &vm);
     if (!kept || dim >= 32 * G) return;
     const int row = slot % KV4_TILE, which = l & 3;
     uint8_t* tile = cache + tile_of(slot, head, heads, tiles_a_page) * kv4_tile_bytes(G);
@@ -124,10 +137,41 @@ __global__ void __launch_bounds__(CT) kv4_append_kernel(const T* __restrict__ ke
     *reinterpret_cast<__half*>(tile + kv4_param(G, row, which, l >> 2)) = which == 0 ? ks : which == 1 ? km : which == 2 ? vs : vm;
 }
 
-template <class T> __device__ __forceinline__ uint4 unpack8(unsigned codes, float s, float m) {
-    __align__(16) T e[8];
+// Eight values: the codes as fp16 numbers 1024 + code two at a time (codes i and i + 4), back to 0 .. 15 exactly, times the scale plus
+// the minimum with one rounding (fp16: fused in fp16; bf16: fused in fp32, then rounded)
+template <class T> __device__ __forceinline__ uint4 unpack8(unsigned codes, __half s, __half m);
+__device__ __forceinline__ void codes_as_halves(unsigned codes, __half2 (&c)[4]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_float<T>(fmaf(static_cast<float>((codes >> (4 * i)) & 15u), s, m));
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = ((codes >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+        c[i] = __hsub2(*reinterpret_cast<const __half2*>(&w), __floats2half2_rn(1024.f, 1024.f));
+    }
+}
+template <> __device__ __forceinline__ uint4 unpack8<__half>(unsigned codes, __half s, __half m) {
+    __half2 c[4];
+    codes_as_halves(codes, c);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 v = __hfma2(c[i], __half2half2(s), __half2half2(m));
+        w[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    return make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+}
+template <> __device__ __forceinline__ uint4 unpack8<__nv_bfloat16>(unsigned codes, __half s, __half m) {
+    __half2 c[4];
+    codes_as_halves(codes, c);
+    const float sf = __half2float(s), mf = __half2float(m);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(c[i]);
+        v[i] = fmaf(f.x, sf, mf);
+        v[i + 4] = fmaf(f.y, sf, mf);
+    }
+    __align__(16) __nv_bfloat162 e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
     return *reinterpret_cast<const uint4*>(e);
 }
 
@@ -143,7 +187,7 @@ __global__ void __launch_bounds__(CT) kv4_read_kernel(const uint8_t* __restrict_
     if (slot >= 0 && slot < slots) {
         const int row = slot % KV4_TILE, g = l >> 2;
         const uint8_t* tile = cache + tile_of(slot, head, heads, tiles_a_page) * kv4_tile_bytes(G);
-        auto par = [&](int which) { return __half2float(*reinterpret_cast<const __half*>(tile + kv4_param(G, row, which, g))); };
+        auto par = [&](int which) { return *reinterpret_cast<const __half*>(tile + kv4_param(G, row, which, g)); };
         const unsigned kc = *reinterpret_cast<const uint32_t*>(tile + kv4_key_half(G, row, dim));
         const unsigned vc = *reinterpret_cast<const uint16_t*>(tile + kv4_value_half(G, row, dim)) |
                             static_cast<unsigned>(*reinterpret_cast<const uint16_t*>(tile + kv4_value_half(G, row, dim + 4))) << 16;

@@ -40,7 +40,6 @@ namespace {
 
 constexpr int W = 4;                 // warps of a CTA
 constexpr int STAGES = 2;            // pairs of tiles in a warp's ring
-constexpr long long LINE_FROM = 4096;  // tiles of a call from which on the line pays
 constexpr int MAX_CLUSTER = 8;
 constexpr float LOWEST = -3.0e38f;   // reference of a result without tokens: finite, so that no difference of infinities is formed
 
@@ -841,9 +840,14 @@ long long kv4_few_workspace(long long heads, long long kv_heads, int D, long lon
     return cuts_bytes(ctas) + static_cast<long long>(ctas) * 2 * 8 * nt * (32 * kv4_groups(D) + 4) * 4;
 }
 
+// The line pays where requests of any length have to keep the GPU busy for long (from about 100 000 tiles of 16 tokens: 250 MB at
+// head_dim 128; below, its second launch and its look at all lengths cost what the even spread gives: 32 heads x 4096 tokens 15 us
+// against 9 us), and where there are too few (request, head) pairs for clusters of 8 CTAs to reach half the GPU and each is long
+// (8 heads x 32768 tokens: 21 us against 33 us).
 bool kv4_few_uses_workspace(long long batch, long long heads, long long kv_heads, long long tokens, long long max_q_len) {
     const long long rows = max_q_len * (heads / kv_heads), cols = rows <= 8 ? 8 : 16;
-    return batch * kv_heads * ((rows + cols - 1) / cols) * ((tokens + KV4_TILE - 1) / KV4_TILE) >= LINE_FROM;
+    const long long items = batch * kv_heads * ((rows + cols - 1) / cols), tiles = (tokens + KV4_TILE - 1) / KV4_TILE;
+    return items * tiles >= 100000 || (items * MAX_CLUSTER < 2 * SMS && tiles >= 512);
 }
 
 cudaError_t kv4_attention_few(const Kv4AttnArgs& a, bool bf16, long long max_q_len, cudaStream_t st) {

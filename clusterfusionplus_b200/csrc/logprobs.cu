@@ -82,24 +82,73 @@ __device__ __forceinline__ void extremes(const uint4& v, float& hi, float& lo, _
     extremes_of_pairs<__nv_bfloat162>(v, hi, lo, [](__nv_bfloat162 x) { return __bfloat1622float2(x); });
 }
 
-// running statistics; m starts at the lowest finite number so that no difference of infinities is ever formed
+// Two fp32 numbers in one register pair: sm_100 adds and multiplies both with one instruction
+struct Pair {
+    unsigned long long v;
+    __device__ __forceinline__ Pair() {}
+    __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ float2 both() const {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+        return f;
+    }
+};
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+// Running statistics of a thread relative to a reference m within 4 of its greatest element (e^4 costs no precision, and the
+// reference hardly ever moves).  m starts at the lowest finite number so that no difference of infinities is ever formed.
 struct Stat {
+    float m = -FLT_MAX;
+    Pair z = Pair(0.f, 0.f), w = Pair(0.f, 0.f);
+    __device__ __forceinline__ void meet(float top) {  // before elements up to `top` are added
+        if (top > m + 4.f) {
+            const float d = fmaxf(m - top, -150.f), r = ex2(d * LOG2E);  // e^-150 is 0 here
+            w = Pair(r, r) * fma2(Pair(d, d), z, w);
+            z = Pair(r, r) * z;
+            m = top;
+        }
+    }
+    // CLAMP where x - m may be -inf (0 times infinity in w); NaN goes through
+    template <bool CLAMP> __device__ __forceinline__ void add(float x, float y) {
+        Pair d = Pair(x, y) + Pair(-m, -m);
+        if (CLAMP) {
+            const float2 f = d.both();
+            d = Pair(max_nan(f.x, -150.f), max_nan(f.y, -150.f));
+        }
+        const float2 l = (d * Pair(LOG2E, LOG2E)).both();
+        const Pair e(ex2(l.x), ex2(l.y));
+        z = z + e;
+        w = fma2(e, d, w);
+    }
+};
+
+// a sum of statistics: reference, z, w
+struct Sum {
     float m = -FLT_MAX, z = 0.f, w = 0.f;
+    __device__ __forceinline__ Sum() {}
+    __device__ __forceinline__ Sum(float m_, float z_, float w_) : m(m_), z(z_), w(w_) {}
     __device__ __forceinline__ void refer_to(float top) {  // top >= m
-        const float d = fmaxf(m - top, -150.f), r = ex2(d * LOG2E);  // e^-150 is 0 here
+        const float d = fmaxf(m - top, -150.f), r = ex2(d * LOG2E);
         w = r * fmaf(d, z, w);
         z *= r;
         m = top;
     }
-    template <bool CLAMP> __device__ __forceinline__ void add(float x) {  // x <= m; NaN goes through; CLAMP where x may be -inf (0 times infinity in w)
-        const float d = CLAMP ? max_nan(x - m, -150.f) : x - m, e = ex2(d * LOG2E);
-        z += e;
-        w = fmaf(e, d, w);
-    }
-    __device__ __forceinline__ void join(float m2, float z2, float w2) {
-        Stat o;
-        o.m = m2, o.z = z2, o.w = w2;
-        const float top = fmaxf(m, m2);
+    __device__ __forceinline__ void join(Sum o) {
+        const float top = fmaxf(m, o.m);
         refer_to(top);
         o.refer_to(top);
         z += o.z;
@@ -206,8 +255,9 @@ template <class T> __device__ void block_top(const Walk<T>& w, unsigned long lon
     }
     __syncthreads();
     const unsigned long long bound = sh.bound;
+    const float bound_value = key_value(static_cast<unsigned>(bound >> 32));
     auto keep = [&](float x, int idx, int start) {
-        if (ranked(x, start) >= bound) {
+        if (!(x < bound_value) && ranked(x, start) >= bound) {
             const int at = atomicAdd(&sh.kept, 1);
             if (at < KEEP) sh.keep[at] = ranked(x, idx);
         }
@@ -291,31 +341,33 @@ __global__ void __launch_bounds__(LT, 6) token_logprobs_kernel(const LogprobArgs
         if (tok >= 0 && tok < a.vocab) asked = to_float(row[tok]);
     }
     Stat st;
+    float best_value = -FLT_MAX;
     int best_at = -1;  // start of the vector (or the single) that holds this thread's first maximum
     const int single = w.single(tid);
+    auto meet = [&](float top, int at) {
+        if (top > best_value || best_at < 0) {
+            best_value = fmaxf(top, best_value);
+            best_at = at;
+        }
+        st.meet(top);
+    };
     auto take_single = [&] {
         const float x = to_float(row[single]);
-        if (x > st.m) {
-            st.refer_to(x);
-            best_at = single;
-        } else if (best_at < 0) best_at = single;
-        st.template add<true>(x);
+        meet(x, single);
+        st.template add<true>(x, -INFINITY);
     };
     if (single >= 0 && tid < E) take_single();
     auto take = [&](const uint4& raw, int at) {
         const T* e = reinterpret_cast<const T*>(&raw);
         float hi, lo;
         extremes(raw, hi, lo, T());
-        if (hi > st.m) {
-            st.refer_to(hi);
-            best_at = at;
-        } else if (best_at < 0) best_at = at;
-        if (lo == -INFINITY) {
+        meet(hi, at);
+        if (lo < -1e37f) {  // masked by -inf or the lowest number
 #pragma unroll
-            for (int i = 0; i < E; ++i) st.template add<true>(to_float(e[i]));
+            for (int i = 0; i < E; i += 2) st.template add<true>(to_float(e[i]), to_float(e[i + 1]));
         } else {
 #pragma unroll
-            for (int i = 0; i < E; ++i) st.template add<false>(to_float(e[i]));
+            for (int i = 0; i < E; i += 2) st.template add<false>(to_float(e[i]), to_float(e[i + 1]));
         }
     };
     const uint4* vec = reinterpret_cast<const uint4*>(row + w.vec_at(0));
@@ -331,11 +383,16 @@ __global__ void __launch_bounds__(LT, 6) token_logprobs_kernel(const LogprobArgs
     for (; v < w.vecs; v += LT) take(__ldg(vec + v), w.vec_at(v));
     if (single >= 0 && tid >= E) take_single();
 
+    Sum sum;
+    {
+        const float2 z = st.z.both(), ww = st.w.both();
+        sum = Sum(st.m, z.x + z.y, ww.x + ww.y);
+    }
     if (a.top > 0) {
         unsigned long long best = 0;
         if (best_at >= 0) {
-            if (st.z == st.z && st.m > -FLT_MAX) {
-                best = ranked(st.m, best_at);
+            if (sum.z == sum.z && best_value > -FLT_MAX) {
+                best = ranked(best_value, best_at);
             } else {  // a NaN, an infinity or nothing above the lowest number among them: look at each
                 if (single >= 0) best = ranked(to_float(row[single]), single);
                 for (int u = tid; u < w.vecs; u += LT)
@@ -352,17 +409,16 @@ __global__ void __launch_bounds__(LT, 6) token_logprobs_kernel(const LogprobArgs
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             if (o >= width) continue;
-            const float m = __shfl_xor_sync(0xffffffffu, st.m, o), z = __shfl_xor_sync(0xffffffffu, st.z, o), ww = __shfl_xor_sync(0xffffffffu, st.w, o);
-            st.join(m, z, ww);
+            sum.join(Sum(__shfl_xor_sync(0xffffffffu, sum.m, o), __shfl_xor_sync(0xffffffffu, sum.z, o), __shfl_xor_sync(0xffffffffu, sum.w, o)));
         }
     };
     join_lanes(32);
-    if (lane == 0) sh.part[warp][0] = st.m, sh.part[warp][1] = st.z, sh.part[warp][2] = st.w;
+    if (lane == 0) sh.part[warp][0] = sum.m, sh.part[warp][1] = sum.z, sh.part[warp][2] = sum.w;
     __syncthreads();
     if (warp == 0) {
-        st.m = sh.part[lane % LW][0], st.z = sh.part[lane % LW][1], st.w = sh.part[lane % LW][2];
+        sum = Sum(sh.part[lane % LW][0], sh.part[lane % LW][1], sh.part[lane % LW][2]);
         join_lanes(LW);
-        if (lane == 0) sh.stat[0] = st.m, sh.stat[1] = st.z, sh.stat[2] = st.w;
+        if (lane == 0) sh.stat[0] = sum.m, sh.stat[1] = sum.z, sh.stat[2] = sum.w;
     }
     if (cluster > 1) cluster_sync();
     if (rank == 0) {
@@ -380,19 +436,19 @@ __global__ void __launch_bounds__(LT, 6) token_logprobs_kernel(const LogprobArgs
         if (warp == 0) {
             if (cluster > 1) {
                 const int c = lane % cluster;
-                st.m = peer_float(peer(&sh.stat[0], c)), st.z = peer_float(peer(&sh.stat[1], c)), st.w = peer_float(peer(&sh.stat[2], c));
+                sum = Sum(peer_float(peer(&sh.stat[0], c)), peer_float(peer(&sh.stat[1], c)), peer_float(peer(&sh.stat[2], c)));
                 join_lanes(cluster);
             }
             __syncwarp();
-            const float log_z = logf(st.z);
+            const float log_z = logf(sum.z);
             if (lane == 0) {
-                a.logprobs[r] = (asked - st.m) - log_z;
-                a.entropy[r] = log_z - st.w / st.z;
+                a.logprobs[r] = (asked - sum.m) - log_z;
+                a.entropy[r] = log_z - sum.w / sum.z;
             }
             if (lane < a.top) {
                 const unsigned long long x = sh.top[lane];
                 a.top_tokens[r * a.top + lane] = static_cast<int>(0x7fffffffu - static_cast<unsigned>(x));
-                a.top_logprobs[r * a.top + lane] = (key_value(static_cast<unsigned>(x >> 32)) - st.m) - log_z;
+                a.top_logprobs[r * a.top + lane] = (key_value(static_cast<unsigned>(x >> 32)) - sum.m) - log_z;
             }
         }
     }

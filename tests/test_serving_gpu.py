@@ -364,8 +364,8 @@ def test_attention_of_uneven_requests(cuda_device, schedule):
 
 def test_attention_chooses_the_line_by_itself(cuda_device):
     from clusterfusionplus_b200 import serving
-    assert serving._attention_workspace(16, 8, 8, 128, 16384, 1) > 0 and serving._attention_workspace(1, 8, 8, 128, 1024, 1) == 0
-    check_attention([16000, 3000, 10, 9000], [1, 1, 1, 1], 8, 8, 128, 64, torch.float16, seed=6)
+    assert serving._attention_workspace(2, 8, 8, 128, 16384, 1) > 0 and serving._attention_workspace(1, 8, 8, 128, 1024, 1) == 0
+    check_attention([16000, 9000], [1, 1], 8, 8, 128, 64, torch.float16, seed=6)
 
 
 @pytest.mark.parametrize("counts", [[1, 1, 1], [5, 70, 1]])
