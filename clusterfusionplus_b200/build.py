@@ -2,7 +2,7 @@
 
     python clusterfusionplus_b200/build.py [--force] [--verbose]
 
-Eight translation units, compiled separately (objects cached under lib/obj/) and linked into one
+Nine translation units, compiled separately (objects cached under lib/obj/) and linked into one
 shared library: the decode kernel with the C ABI, the batched Llama decode blocks (hand-written
 tcgen05 skinny GEMMs + paged attention), the elementwise kernels of the prompt pass, the plan of a step over a
 paged cache, the cache held in 4 bits, the log probabilities of tokens, and the tensor-core prefill GEMM, which is built from the CUTLASS / CuTe headers found in the Python environment (the `flashinfer` wheel
@@ -33,6 +33,7 @@ UNITS = {
     "serve_plan.cu": (["host_common.h", HEADER], False),
     "kv4_cache.cu": (["kv4_layout.cuh", "kv4_attention.h", "host_common.h", HEADER], False),
     "kv4_decode.cu": (["kv4_layout.cuh", "kv4_attention.h", "mma.cuh"], False),
+    "kv4_prompt.cu": (["kv4_layout.cuh", "kv4_attention.h", "mma.cuh", "pipeline.cuh"], False),
     "logprobs.cu": (["host_common.h", HEADER], False),
 }
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -25,4 +25,7 @@ long long kv4_few_workspace(long long heads, long long kv_heads, int D, long lon
 bool kv4_few_uses_workspace(long long batch, long long heads, long long kv_heads, long long tokens, long long max_q_len);
 cudaError_t kv4_attention_few(const Kv4AttnArgs& a, bool bf16, long long max_q_len, cudaStream_t st);
 
+// many query rows a request: 128 of them at a time on the tensor cores
+cudaError_t kv4_attention_prompt(const Kv4AttnArgs& a, bool bf16, long long max_q_len, cudaStream_t st);
+
 }  // namespace cfb

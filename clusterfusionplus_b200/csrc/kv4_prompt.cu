@@ -1,0 +1,541 @@
+// Attention over the 4-bit cache for many query rows a request: chunks of prompts.
+//
+// Here every cached token meets 128 query rows (queries times the heads of one cached head) and the work is two matrix products, 4 D flops
+// for each (row, token): it goes to the 5th-generation tensor cores, S = Q K^T and O += P V with 128 x 128 tiles, operands in shared
+// memory (K-major, 128-byte swizzle), accumulators in tensor memory.  At 4096 fp16 multiply-adds a clock a pair of tiles takes
+// ~1000 clocks of the tensor cores and as many of the exponential unit (16 a clock), and unpacking the codes takes ~600 issue slots
+// of each scheduler: three things that overlap, so each has its warps:
+//  - 8 warps unpack: 16 tokens each of a 128-token tile, to fp16 value = code * scale + minimum in one fused rounding (2^-11 of a key or
+//    value: the operands' type; scores and sums stay fp32).  Keys as rows of dims, values as rows of tokens, which is how the cache's
+//    words hold them: two neighbouring tokens in the halves of a word are two neighbouring elements of a row of V^T.
+//  - 4 warps do the softmax, one thread a query row: no exchange between threads.  The reference of a row moves only when it is exceeded
+//    by 2^8, so the accumulator in tensor memory is hardly ever rescaled.
+//  - 1 thread issues the products: S of the next tile before P V of this one, so that they run under the softmax.
+// Every wait is bounded; one that runs out ends the kernel with a device status.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "kv4_attention.h"
+#include "kv4_layout.cuh"
+#include "mma.cuh"
+#include "pipeline.cuh"
+
+namespace cfb {
+namespace {
+
+constexpr int ROWS = 128;            // query rows of a CTA
+constexpr int KEYS = 128;            // tokens of a tile
+constexpr int SOFT = 4, UNPACK = 8;  // warps; one more issues the products
+constexpr int THREADS = 32 * (SOFT + UNPACK + 1);
+constexpr int BLOCK = 128 * 128;     // bytes of a K-major operand block of 128 rows x 64 elements
+constexpr float SLACK = 8.f;         // binary steps that a score may lie above its row's reference
+
+// ------------------------------------------------------------------------------------------------ tensor cores
+__device__ __forceinline__ uint64_t operand(uint32_t saddr) {  // K-major, 128-byte swizzle: rows of 128 bytes, groups of 8 rows 1024 bytes apart
+    return static_cast<uint64_t>((saddr & 0x3ffffu) >> 4) | static_cast<uint64_t>(1u) << 16 | static_cast<uint64_t>(1024u >> 4) << 32 |
+           static_cast<uint64_t>(1u) << 46 | static_cast<uint64_t>(2u) << 61;
+}
+__device__ __forceinline__ constexpr uint32_t shape(int m, int n) {  // fp16 operands, fp32 accumulator, both K-major
+    return (1u << 4) | static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(m >> 4) << 24;
+}
+__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {  // arrives once every product issued so far is done
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }  // plain stores, for the tensor cores to read
+
+// 16 columns of this thread's row of tensor memory; the wait belongs to the load, so that nothing uses the registers before it
+__device__ __forceinline__ void tmem_load(uint32_t at, float (&x)[16]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(x[8]), "=f"(x[9]), "=f"(x[10]),
+          "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15])
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t at, float (&x)[32]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(x[8]), "=f"(x[9]), "=f"(x[10]),
+          "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15]), "=f"(x[16]), "=f"(x[17]), "=f"(x[18]), "=f"(x[19]), "=f"(x[20]),
+          "=f"(x[21]), "=f"(x[22]), "=f"(x[23]), "=f"(x[24]), "=f"(x[25]), "=f"(x[26]), "=f"(x[27]), "=f"(x[28]), "=f"(x[29]), "=f"(x[30]), "=f"(x[31])
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store(uint32_t at, const float (&x)[16]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n\t"
+        "tcgen05.wait::st.sync.aligned;" ::"r"(at), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]), "f"(x[8]),
+        "f"(x[9]), "f"(x[10]), "f"(x[11]), "f"(x[12]), "f"(x[13]), "f"(x[14]), "f"(x[15])
+        : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------ numbers
+template <class T> __device__ __forceinline__ float2 to_float2(uint32_t v);
+template <> __device__ __forceinline__ float2 to_float2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+template <> __device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
+template <class T> __device__ __forceinline__ uint32_t pack(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) { return pack_half2(a, b); }
+template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // e in -126 .. 127
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
+__device__ __forceinline__ uint32_t as_word(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+
+// codes 0, 4 | 1, 5 | 2, 6 | 3, 7 of a word as pairs of fp16 numbers: 1024 + code and 64 + code by the bits, less 1024 and 64
+__device__ __forceinline__ void code_pairs(uint32_t w, __half2 (&c)[4]) {
+    const uint32_t h = w >> 8;
+    const __half2 k1024 = as_half2(0x64006400u), k64 = as_half2(0x54005400u);
+    c[0] = __hsub2(as_half2((w & 0x000f000fu) | 0x64006400u), k1024);
+    c[1] = __hsub2(as_half2((w & 0x00f000f0u) | 0x54005400u), k64);
+    c[2] = __hsub2(as_half2((h & 0x000f000fu) | 0x64006400u), k1024);
+    c[3] = __hsub2(as_half2((h & 0x00f000f0u) | 0x54005400u), k64);
+}
+// A scale whose largest value minimum + 15 scale would round beyond fp16 (the scale was rounded up at the end of the range): one step lower
+__device__ __forceinline__ uint32_t within_range(uint32_t s, uint32_t m) {
+    return fmaf(15.f, __half2float(__ushort_as_half(static_cast<unsigned short>(s))), __half2float(__ushort_as_half(static_cast<unsigned short>(m)))) > 65504.f ? s - 1 : s;
+}
+__device__ __forceinline__ bool finite_half(uint32_t x) { return (x & 0x7c00u) != 0x7c00u; }
+
+// N consecutive words / 16-bit numbers of global memory; two and four words are aligned to all of them
+template <int N> __device__ __forceinline__ void global_words(uint32_t (&x)[N], const uint8_t* p) {
+    if constexpr (N == 4) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    } else if constexpr (N == 2) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        x[0] = v.x, x[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+    }
+}
+template <int N> __device__ __forceinline__ void global_halves(uint32_t (&x)[N], const uint8_t* p) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = __ldg(reinterpret_cast<const unsigned short*>(p) + i);
+}
+
+struct Shared {
+    unsigned long long q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full, pv_done, drain;
+    uint32_t tmem;
+    int abort;
+    unsigned there[4];          // [tile % 4] bit t: the 16 tokens t of the tile exist.  Four: keys are unpacked two tiles ahead of the softmax
+    uint32_t bad[2][4][4];      // [value buffer][group][token / 32]: tokens whose value parameters are not finite
+};
+
+template <class T, int G>
+__global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArgs a) {
+    constexpr int TB = kv4_tile_bytes(G), DP = 32 * G, DB = (DP + 63) / 64;  // blocks of 64 dims
+    constexpr int VBLOCK = DP * 128;                                         // bytes of V^T, 64 tokens
+    extern __shared__ uint8_t raw[];
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
+    uint8_t* s_q = base;
+    uint8_t* s_k = s_q + DB * BLOCK;            // [2]
+    uint8_t* s_v = s_k + 2 * DB * BLOCK;        // [2]
+    uint8_t* s_p = s_v + 2 * 2 * VBLOCK;
+    __shared__ Shared sh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    auto bar = [](unsigned long long& b) { return smem_u32(&b); };
+    if (tid == 0) {
+        mbar_init(bar(sh.q_full), 32 * SOFT);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(sh.k_full[i]), UNPACK);
+            mbar_init(bar(sh.k_empty[i]), 1);
+            mbar_init(bar(sh.v_full[i]), UNPACK);
+            mbar_init(bar(sh.v_empty[i]), 1);
+            mbar_init(bar(sh.s_full[i]), 1);
+        }
+        mbar_init(bar(sh.p_full), 32 * SOFT);
+        mbar_init(bar(sh.pv_done), 1);
+        mbar_init(bar(sh.drain), 1);
+        mbar_fence_init();
+        sh.abort = 0;
+        for (int i = 0; i < 4; ++i) sh.there[i] = 0;
+    }
+    if (tid < 32) (&sh.bad[0][0][0])[tid] = 0;
+    if (warp == SOFT + UNPACK) {  // scores twice 128 columns, numerators 128: 512 is the next size there is
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        fence_before();
+    }
+    __syncthreads();
+    fence_after();
+    const uint32_t tm_s = sh.tmem, tm_o = sh.tmem + 2 * KEYS;  // columns: scores of two tiles, numerators
+    const AbortCtl ctl{&sh.abort, a.status};
+    // one answer for the whole warp, which goes on together
+    auto wait = [&](unsigned long long& b, int phase, int code) { return __all_sync(0xffffffffu, mbar_wait(bar(b), phase & 1, ctl, code)) != 0; };
+
+    const int b = blockIdx.x / a.kv_heads, kvh = blockIdx.x - b * a.kv_heads, per = a.heads / a.kv_heads;
+    int first = b, n_q = 1;
+    if (a.qo_indptr) {
+        first = a.qo_indptr[b];
+        n_q = first < 0 ? 0 : min(a.qo_indptr[b + 1], static_cast<int>(a.rows)) - first;
+    }
+    const int rows = n_q > 0 ? n_q * per : 0, q_tiles = (rows + ROWS - 1) / ROWS;
+    const long long cap = a.table_width * a.page, before = static_cast<long long>(a.kv_lens[b]) - n_q;
+    const int* table = a.table + b * a.table_stride;
+    const int N = (a.D + 15) / 16 * 16;
+
+    int done = 0;   // tiles of tokens so far: the phase of every barrier follows from it
+    int items = 0;  // (request, head, 128 rows) so far
+    for (int y = blockIdx.y; y < q_tiles; y += gridDim.y) {
+        const int r0 = (q_tiles - 1 - y) * ROWS;  // the longest first
+        const long long end = min(before + (min(r0 + ROWS, rows) - 1) / per, cap - 1);  // the last token that these rows see
+        const int n = end < 0 ? 0 : static_cast<int>(end / KEYS) + 1;
+        bool ok = true;
+
+        if (warp < SOFT) {
+            // ================================================================ softmax: thread = row
+            const int r = r0 + tid;
+            const bool real = r < rows;
+            const int qi = real ? r / per : 0, head = kvh * per + (real ? r % per : 0);
+            const T* src = static_cast<const T*>(a.query) + static_cast<long long>(first + qi) * a.q_ts + head * a.q_hs;
+            const int last = real ? static_cast<int>(max(min(before + qi, cap - 1), -1ll)) : -1;
+            const int all_see = static_cast<int>(max(min(before + r0 / per, cap - 1), -1ll));  // every real row sees these
+            float top = 0.f;
+            if (n > 0) {
+                for (int d = 0; d < a.D; d += 8) {
+                    const uint4 v = real ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 f = to_float2<T>(w[i]);
+                        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    }
+                }
+                // a power of two takes the row to at most 2^10 (exact; bf16 reaches beyond fp16), the scale's sign goes along
+                const int e = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100);
+                const float up = copysignf(power_of_two(min(9 - e, 127)), a.scale_log2);
+                for (int d = 0; d < N; d += 8) {
+                    const uint4 v = real && d < a.D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    uint32_t o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 f = to_float2<T>(w[i]);
+                        o[i] = pack_half2(f.x * up, f.y * up);
+                    }
+                    *reinterpret_cast<uint4*>(s_q + d / 64 * BLOCK + tid * 128 + ((d % 64 / 8) ^ (tid & 7)) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+                fence_shared();
+                mbar_arrive(bar(sh.q_full));
+                const float factor = fminf(fabsf(a.scale_log2) * power_of_two(e - 9), 3.4e38f);
+                const uint32_t mine = static_cast<uint32_t>(warp * 32) << 16;  // this warp's lanes of tensor memory
+
+                float m = 0.f, l = 0.f;
+                unsigned broken = 0;  // groups in which this row meets a value that is not finite
+                for (int i = 0; ok && i < n; ++i) {
+                    const int at = done + i, buf = at & 1, key0 = i * KEYS;
+                    if (!(ok = wait(sh.s_full[buf], at >> 1, ST_TIMEOUT_FULL))) break;
+                    fence_after();
+                    const unsigned there = sh.there[at & 3];
+                    const bool whole = key0 + KEYS - 1 <= all_see && there == 0xffu;
+                    float x[32], high = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < KEYS; c += 32) {
+                        tmem_load(tm_s + buf * KEYS + c + mine, x);
+                        if (!whole) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (key0 + c + j > last || !(there >> ((c + j) / 16) & 1u)) x[j] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) high = fmaxf(high, x[j]);
+                    }
+                    high = high == -INFINITY ? -INFINITY : high * factor;
+                    // the reference: the first tile's greatest; later only if exceeded by SLACK
+                    const bool start = i == 0 || l == 0.f;
+                    const float up_by = start ? (high == -INFINITY ? 0.f : high - m) : (high > m + SLACK ? high - m : 0.f);
+                    if (i > 0) {  // the products before have read P and written O
+                        if (!(ok = wait(sh.pv_done, at - 1, ST_TIMEOUT_FULL))) break;
+                        fence_after();
+                        if (__any_sync(0xffffffffu, up_by != 0.f && l != 0.f)) {
+                            const float keep = l != 0.f ? ex2(-up_by) : 1.f;
+                            l *= keep;
+                            for (int c = 0; c < N; c += 16) {
+                                float o[16];
+                                tmem_load(tm_o + c + mine, o);
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) o[j] *= keep;
+                                tmem_store(tm_o + c + mine, o);
+                            }
+                        }
+                    }
+                    m += up_by;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int c = 0; c < KEYS; c += 32) {
+                        tmem_load(tm_s + buf * KEYS + c + mine, x);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) x[j] = fmaf(x[j], factor, -m);
+                        if (!whole) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (key0 + c + j > last || !(there >> ((c + j) / 16) & 1u)) x[j] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8) {
+                            float p[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                p[k] = ex2(x[j + k]);
+                                sum += p[k];
+                            }
+                            const int chunk = (c % 64 + j) / 8;
+                            *reinterpret_cast<uint4*>(s_p + c / 64 * BLOCK + tid * 128 + (chunk ^ (tid & 7)) * 16) =
+                                make_uint4(pack_half2(p[0], p[1]), pack_half2(p[2], p[3]), pack_half2(p[4], p[5]), pack_half2(p[6], p[7]));
+                        }
+                    }
+                    l += sum;
+                    if (!(ok = wait(sh.v_full[buf], at >> 1, ST_TIMEOUT_FULL))) break;  // for sh.bad; in time for P V anyway
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int see = last - key0 - 32 * k;
+                            const uint32_t seen = see < 0 ? 0u : see >= 31 ? 0xffffffffu : (2u << see) - 1u;
+                            if (sh.bad[buf][g][k] & seen) broken |= 1u << g;
+                        }
+                    fence_before();
+                    fence_shared();
+                    mbar_arrive(bar(sh.p_full));
+                }
+                if (ok && (ok = wait(sh.pv_done, done + n - 1, ST_TIMEOUT_FULL))) {
+                    fence_after();
+                    T* dst = static_cast<T*>(a.out) + (static_cast<long long>(first + qi) * a.heads + head) * a.D;
+                    const float inv = 1.f / l;
+                    for (int c = 0; c < N; c += 16) {
+                        float o[16];
+                        tmem_load(tm_o + c + mine, o);
+                        if (broken >> (c / 32) & 1u) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = __int_as_float(0x7fffffff);
+                        }
+                        if (l == 0.f) {  // no token seen
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = 0.f;
+                        }
+                        const float by = l == 0.f ? 1.f : inv;
+#pragma unroll
+                        for (int j = 0; j < 16; j += 8)
+                            if (real && c + j < a.D)
+                                *reinterpret_cast<uint4*>(dst + c + j) = make_uint4(pack<T>(o[j] * by, o[j + 1] * by), pack<T>(o[j + 2] * by, o[j + 3] * by),
+                                                                                    pack<T>(o[j + 4] * by, o[j + 5] * by), pack<T>(o[j + 6] * by, o[j + 7] * by));
+                    }
+                    fence_before();
+                }
+            } else if (real) {
+                T* dst = static_cast<T*>(a.out) + (static_cast<long long>(first + qi) * a.heads + head) * a.D;
+                for (int d = 0; d < a.D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
+            }
+        } else if (warp < SOFT + UNPACK) {
+            // ================================================================ unpacking: warp = 16 tokens of each tile
+            // What the next step needs is on its way while this one is unpacked: the block table an iteration ahead, keys behind the
+            // values before them, values behind the keys of their own tile.
+            const int part = warp - SOFT, tiles_a_page = a.page / KV4_TILE;
+            auto find = [&](int i) -> const uint8_t* {
+                const int tile = i * (KEYS / KV4_TILE) + part;
+                if (i >= n || tile * KV4_TILE > end) return nullptr;
+                const int col = tile / tiles_a_page, held = table[col];
+                if (held >= 0 && held < a.pages) return a.cache + ((static_cast<long long>(held) * a.kv_heads + kvh) * tiles_a_page + (tile - col * tiles_a_page)) * TB;
+                if (lane == 0) atomicCAS(a.status, 0, ST_BAD_SLOT);
+                return nullptr;
+            };
+            // keys: lane = row (16) and half of the t's; values: lane = (h, c) and half of the groups
+            const int row = lane & 15, th = lane >> 4, c8 = lane & 7, h = lane >> 3 & 1;
+            constexpr int GP = (G + 1) / 2;
+            const int g0 = (lane >> 4) * GP;
+            uint32_t kw[2][G], kp[2 * G];  // codes; scales and minima
+            auto load_keys = [&](const uint8_t* src) {
+                if (src) {
+                    global_words<G>(kw[0], src + (row * 4 + 2 * th) * 4 * G);
+                    global_words<G>(kw[1], src + (row * 4 + 2 * th + 1) * 4 * G);
+                    global_halves<2 * G>(kp, src + kv4_param(G, row, 0, 0));
+                }
+            };
+            const uint8_t* src = find(0);
+            load_keys(src);
+            for (int i = 0; ok && i < n; ++i) {
+                const int at = done + i, buf = at & 1, token0 = (i * (KEYS / KV4_TILE) + part) * KV4_TILE;
+                const uint8_t* next = find(i + 1);
+                uint32_t vw[4][GP], vs[8][GP], vm[8][GP];  // words of the token pairs; scales and minima of the tokens; groups g0 ..
+                if (src) {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const uint8_t* w = src + kv4_value_half(G, 8 * h + 2 * t, 32 * g0 + 4 * c8);
+                        if constexpr (G == 4) {
+                            global_words<GP>(vw[t], w);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < GP; ++k) vw[t][k] = g0 + k < G ? __ldg(reinterpret_cast<const uint32_t*>(w) + k) : 0u;
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) {
+                        const unsigned short* x = reinterpret_cast<const unsigned short*>(src + kv4_param(G, 8 * h + t, 2, g0));  // scale, G on the minimum
+#pragma unroll
+                        for (int k = 0; k < GP; ++k) {
+                            vs[t][k] = g0 + k < G ? __ldg(x + k) : 0u;
+                            vm[t][k] = g0 + k < G ? __ldg(x + G + k) : 0u;
+                        }
+                    }
+                }
+                if (!(ok = wait(sh.k_empty[buf], (at >> 1) + 1, ST_TIMEOUT_EMPTY))) break;
+                uint8_t* kd = s_k + buf * DB * BLOCK + (part * KV4_TILE + row) * 128;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const uint32_t s = src ? within_range(kp[g], kp[G + g]) : 0u, m = src ? kp[G + g] : 0u;
+                    const __half2 s2 = as_half2(s | s << 16), m2 = as_half2(m | m << 16);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        __half2 c[4];
+                        code_pairs(src ? kw[j][g] : 0u, c);
+                        uint32_t v[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[k] = as_word(__hfma2(c[k], s2, m2));
+                        const int d = 32 * g + 8 * (2 * th + j);
+                        *reinterpret_cast<uint4*>(kd + d / 64 * BLOCK + ((d % 64 / 8) ^ (row & 7)) * 16) =
+                            make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
+                    }
+                }
+                if (lane == 0) {
+                    if (src) atomicOr(&sh.there[at & 3], 1u << part);
+                    else atomicAnd(&sh.there[at & 3], ~(1u << part));
+                }
+                fence_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(sh.k_full[buf]));
+                load_keys(next);
+
+                if (!(ok = wait(sh.v_empty[buf], (at >> 1) + 1, ST_TIMEOUT_EMPTY))) break;
+#pragma unroll
+                for (int k = 0; k < GP; ++k) {
+                    const int g = g0 + k;
+                    if (g >= G) continue;
+                    uint32_t out[4][4];  // [dim][token pair]
+                    uint32_t bad = 0;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        uint32_t s[2] = {0u, 0u}, m[2] = {0u, 0u};
+                        if (src) {
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                // Nothing that is not finite goes into the products, where it would reach rows that do not see the token: it is
+                                // left out here and the rows that see it become NaN in this group.  Behind the last token, where anything
+                                // may lie, nothing is taken.
+                                const uint32_t x = vs[2 * t + j][k], y = vm[2 * t + j][k];
+                                const bool seen = token0 + 8 * h + 2 * t + j <= end, fine = finite_half(x) && finite_half(y);
+                                if (!fine && seen) bad |= 1u << (2 * t + j);
+                                s[j] = fine && seen ? within_range(x, y) : 0u;
+                                m[j] = fine && seen ? y : 0u;
+                            }
+                        }
+                        const __half2 s2 = as_half2(s[0] | s[1] << 16), m2 = as_half2(m[0] | m[1] << 16);
+                        __half2 c[4];
+                        code_pairs(src ? vw[t][k] : 0u, c);  // nibble n of both tokens
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) out[d][t] = as_word(__hfma2(c[d], s2, m2));
+                    }
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        const int dim = 32 * g + 4 * c8 + d, key = part * KV4_TILE + 8 * h;
+                        *reinterpret_cast<uint4*>(s_v + (buf * 2 + key / 64) * VBLOCK + dim * 128 + ((key % 64 / 8) ^ (dim & 7)) * 16) =
+                            make_uint4(out[d][0], out[d][1], out[d][2], out[d][3]);
+                    }
+                    if (c8 == 0) reinterpret_cast<uint8_t*>(&sh.bad[buf][g][0])[part * 2 + h] = static_cast<uint8_t>(bad);  // 8 tokens a byte
+                }
+                fence_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(sh.v_full[buf]));
+                src = next;
+            }
+        } else if (lane == 0 && n > 0) {
+            // ================================================================ products, one thread
+            const uint32_t d_s = shape(ROWS, KEYS), d_o = shape(ROWS, N);
+            const uint32_t q = smem_u32(s_q), k0 = smem_u32(s_k), v0 = smem_u32(s_v), p = smem_u32(s_p);
+            auto scores = [&](int i) {
+                const int at = done + i, buf = at & 1;
+                if (!mbar_wait(bar(sh.k_full[buf]), (at >> 1) & 1, ctl, ST_TIMEOUT_FULL)) return false;
+                fence_after();
+                for (int s = 0; s < N / 16; ++s)
+                    product(tm_s + buf * KEYS, operand(q + s / 4 * BLOCK + s % 4 * 32), operand(k0 + buf * DB * BLOCK + s / 4 * BLOCK + s % 4 * 32), d_s, s > 0);
+                commit(bar(sh.s_full[buf]));
+                commit(bar(sh.k_empty[buf]));
+                return true;
+            };
+            ok = mbar_wait(bar(sh.q_full), items & 1, ctl, ST_TIMEOUT_FULL) && scores(0);
+            for (int i = 0; ok && i < n; ++i) {
+                const int at = done + i, buf = at & 1;
+                if (i + 1 < n && !(ok = scores(i + 1))) break;
+                if (!(ok = mbar_wait(bar(sh.v_full[buf]), (at >> 1) & 1, ctl, ST_TIMEOUT_FULL) && mbar_wait(bar(sh.p_full), at & 1, ctl, ST_TIMEOUT_FULL))) break;
+                fence_after();
+                for (int s = 0; s < KEYS / 16; ++s)
+                    product(tm_o, operand(p + s / 4 * BLOCK + s % 4 * 32), operand(v0 + (buf * 2 + s / 4) * VBLOCK + s % 4 * 32), d_o, i > 0 || s > 0);
+                commit(bar(sh.pv_done));
+                commit(bar(sh.v_empty[buf]));
+            }
+        }
+        if (!ok || *ctl.flag) break;
+        done += n;
+        items += n > 0;
+    }
+    // every product has ended where the last P V was waited for; after a wait that ran out, wait for what was issued (bounded) before freeing
+    __syncwarp();
+    if (warp == SOFT + UNPACK) {
+        if (lane == 0 && *ctl.flag) {
+            commit(bar(sh.drain));
+            for (int spin = 0; spin < 1 << 20 && !mbar_try_wait(bar(sh.drain), 0); ++spin) {}
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+    if (warp == SOFT + UNPACK) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh.tmem) : "memory");
+    }
+}
+
+template <class T, int G> cudaError_t launch(const Kv4AttnArgs& a, long long max_q_len, cudaStream_t st) {
+    constexpr int DB = (32 * G + 63) / 64, smem = 1024 + 3 * DB * BLOCK + 4 * 32 * G * 128 + 2 * BLOCK;
+    const cudaError_t e = cudaFuncSetAttribute(kv4_prompt_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const long long q_tiles = (max_q_len * (a.heads / a.kv_heads) + ROWS - 1) / ROWS;
+    const dim3 grid(static_cast<unsigned>(a.batch * a.kv_heads), static_cast<unsigned>(q_tiles < 65535 ? q_tiles : 65535));
+    kv4_prompt_kernel<T, G><<<grid, THREADS, smem, st>>>(a);
+    return cudaGetLastError();
+}
+
+template <class T> cudaError_t by_groups(const Kv4AttnArgs& a, long long max_q_len, cudaStream_t st) {
+    switch (kv4_groups(a.D)) {
+        case 1: return launch<T, 1>(a, max_q_len, st);
+        case 2: return launch<T, 2>(a, max_q_len, st);
+        case 3: return launch<T, 3>(a, max_q_len, st);
+        default: return launch<T, 4>(a, max_q_len, st);
+    }
+}
+
+}  // namespace
+
+cudaError_t kv4_attention_prompt(const Kv4AttnArgs& a, bool bf16, long long max_q_len, cudaStream_t st) {
+    return bf16 ? by_groups<__nv_bfloat16>(a, max_q_len, st) : by_groups<__half>(a, max_q_len, st);
+}
+
+}  // namespace cfb

@@ -193,7 +193,8 @@ __device__ __forceinline__ unsigned cluster_rank() {
     return r;
 }
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t peer(const void* p, unsigned rank) {
     uint32_t a;
@@ -324,7 +325,7 @@ template <class T> __device__ void block_top(const Walk<T>& w, unsigned long lon
 }
 
 template <class T>
-__global__ void __launch_bounds__(LT, 6) token_logprobs_kernel(const LogprobArgs a, int cluster) {
+__global__ void __launch_bounds__(LT, 8) token_logprobs_kernel(const LogprobArgs a, int cluster) {
     __shared__ Shared sh;
     constexpr int E = Walk<T>::E;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;

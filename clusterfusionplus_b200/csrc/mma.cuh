@@ -50,7 +50,8 @@ __device__ __forceinline__ unsigned cluster_ctarank() {
     return r;
 }
 __device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t cluster_map(const void* p, unsigned rank) {
     uint32_t a;
