@@ -139,6 +139,8 @@ struct Shared {
     int abort;
     unsigned there[4];          // [tile % 4] bit t: the 16 tokens t of the tile exist.  Four: keys are unpacked two tiles ahead of the softmax
     uint32_t bad[2][4][4];      // [value buffer][group][token / 32]: tokens whose value parameters are not finite
+    __align__(16) uint16_t kpar[8][16][8];     // [unpacking warp][token][scales, minima of the keys]
+    __align__(16) uint16_t vpar[8][2][4][16];  // [unpacking warp][scale, minimum of the values][group][token]
 };
 
 template <class T, int G>
@@ -146,7 +148,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
     constexpr int TB = kv4_tile_bytes(G), DP = 32 * G, DB = (DP + 63) / 64;  // blocks of 64 dims
     constexpr int VBLOCK = DP * 128;                                         // bytes of V^T, 64 tokens
     extern __shared__ uint8_t raw[];
-    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
+    uint8_t* base = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;  // (by an offset: the compiler has to see that it is shared memory)
     uint8_t* s_q = base;
     uint8_t* s_k = s_q + DB * BLOCK;            // [2]
     uint8_t* s_v = s_k + 2 * DB * BLOCK;        // [2]
@@ -348,38 +350,42 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
             }
         } else if (warp < SOFT + UNPACK) {
             // ================================================================ unpacking: warp = 16 tokens of each tile
-            // What the next step needs is on its way while this one is unpacked: the block table an iteration ahead, keys behind the
-            // values before them, values behind the keys of their own tile.
+            // What a tile needs is asked for while the tile before it is unpacked: the block table's entry first, then codes and parameters, each
+            // as soon as its registers are free.  The parameters of the 16 tokens are looked over once, and handed round through shared memory in
+            // the order of their use.
             const int part = warp - SOFT, tiles_a_page = a.page / KV4_TILE;
-            auto find = [&](int i) -> const uint8_t* {
-                const int tile = i * (KEYS / KV4_TILE) + part;
-                if (i >= n || tile * KV4_TILE > end) return nullptr;
-                const int col = tile / tiles_a_page, held = table[col];
-                if (held >= 0 && held < a.pages) return a.cache + ((static_cast<long long>(held) * a.kv_heads + kvh) * tiles_a_page + (tile - col * tiles_a_page)) * TB;
-                if (lane == 0) atomicCAS(a.status, 0, ST_BAD_SLOT);
+            constexpr int NOT_NEEDED = -2;
+            auto entry = [&](int i) {
+                const long long tile = static_cast<long long>(i) * (KEYS / KV4_TILE) + part;
+                return i < n && tile * KV4_TILE <= end ? table[static_cast<int>(tile) / tiles_a_page] : NOT_NEEDED;
+            };
+            auto find = [&](int held, int i) -> const uint8_t* {
+                if (held >= 0 && held < a.pages)
+                    return a.cache + ((static_cast<long long>(held) * a.kv_heads + kvh) * tiles_a_page + (i * (KEYS / KV4_TILE) + part) % tiles_a_page) * TB;
+                if (held != NOT_NEEDED && lane == 0) atomicCAS(a.status, 0, ST_BAD_SLOT);
                 return nullptr;
             };
-            // keys: lane = row (16) and half of the t's; values: lane = (h, c) and half of the groups
-            const int row = lane & 15, th = lane >> 4, c8 = lane & 7, h = lane >> 3 & 1;
+            // keys: lane = row (16) and half of the t's; values: lane = (c, h) and half of the groups (neighbouring lanes differ in c & 1 and
+            // h, which spreads their stores over the banks); parameters: lane = token (16) and half of the groups
             constexpr int GP = (G + 1) / 2;
-            const int g0 = (lane >> 4) * GP;
-            uint32_t kw[2][G], kp[2 * G];  // codes; scales and minima
-            auto load_keys = [&](const uint8_t* src) {
-                if (src) {
-                    global_words<G>(kw[0], src + (row * 4 + 2 * th) * 4 * G);
-                    global_words<G>(kw[1], src + (row * 4 + 2 * th + 1) * 4 * G);
-                    global_halves<2 * G>(kp, src + kv4_param(G, row, 0, 0));
-                }
-            };
-            const uint8_t* src = find(0);
-            load_keys(src);
-            for (int i = 0; ok && i < n; ++i) {
-                const int at = done + i, buf = at & 1, token0 = (i * (KEYS / KV4_TILE) + part) * KV4_TILE;
-                const uint8_t* next = find(i + 1);
-                uint32_t vw[4][GP], vs[8][GP], vm[8][GP];  // words of the token pairs; scales and minima of the tokens; groups g0 ..
-                if (src) {
+            const int row = lane & 15, th = lane >> 4, h = lane >> 1 & 1, c8 = (lane & 1) | (lane >> 1 & 6), g0 = th * GP;
+            uint32_t kw[2][G], vw[4][GP], par[4][GP];  // codes; key scale, key minimum, value scale, value minimum of token `row`, groups g0 ..
+            auto load_par = [&](const uint8_t* src) {
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
+                for (int which = 0; which < 4; ++which)
+#pragma unroll
+                    for (int k = 0; k < GP; ++k)
+                        par[which][k] = src && g0 + k < G ? __ldg(reinterpret_cast<const unsigned short*>(src + kv4_param(G, row, which, g0)) + k) : 0u;
+            };
+            auto load_keys = [&](const uint8_t* src) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (src) global_words<G>(kw[j], src + (row * 4 + 2 * th + j) * 4 * G);
+            };
+            auto load_values = [&](const uint8_t* src) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    if (src) {
                         const uint8_t* w = src + kv4_value_half(G, 8 * h + 2 * t, 32 * g0 + 4 * c8);
                         if constexpr (G == 4) {
                             global_words<GP>(vw[t], w);
@@ -388,32 +394,63 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                             for (int k = 0; k < GP; ++k) vw[t][k] = g0 + k < G ? __ldg(reinterpret_cast<const uint32_t*>(w) + k) : 0u;
                         }
                     }
+            };
 #pragma unroll
-                    for (int t = 0; t < 8; ++t) {
-                        const unsigned short* x = reinterpret_cast<const unsigned short*>(src + kv4_param(G, 8 * h + t, 2, g0));  // scale, G on the minimum
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int k = 0; k < GP; ++k) {
-                            vs[t][k] = g0 + k < G ? __ldg(x + k) : 0u;
-                            vm[t][k] = g0 + k < G ? __ldg(x + G + k) : 0u;
-                        }
+                for (int g = 0; g < G; ++g) kw[j][g] = 0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int k = 0; k < GP; ++k) vw[t][k] = 0;
+            const uint8_t* src = find(entry(0), 0);
+            load_par(src);
+            load_keys(src);
+            load_values(src);
+            int held = entry(1);
+            for (int i = 0; ok && i < n; ++i) {
+                const int at = done + i, buf = at & 1;
+                const long long token0 = (static_cast<long long>(i) * (KEYS / KV4_TILE) + part) * KV4_TILE;
+                const uint8_t* next = find(held, i + 1);
+                held = entry(i + 2);
+                // ---- parameters (those of a missing page are 0: so are its keys and values)
+                uint32_t bad[GP];  // tokens of groups k (low half) and GP + k
+#pragma unroll
+                for (int k = 0; k < GP; ++k) {
+                    // Nothing that is not finite goes into P V, where it would reach rows that do not see the token: it is left out here and the
+                    // rows that see it become NaN in this group.  Behind the last token, where anything may lie, nothing is taken.
+                    const bool seen = token0 + row <= end, fine = finite_half(par[2][k]) && finite_half(par[3][k]);
+                    bad[k] = __ballot_sync(0xffffffffu, seen && !fine);
+                    if (g0 + k < G) {
+                        sh.kpar[part][row][g0 + k] = static_cast<uint16_t>(within_range(par[0][k], par[1][k]));
+                        sh.kpar[part][row][4 + g0 + k] = static_cast<uint16_t>(par[1][k]);
+                        sh.vpar[part][0][g0 + k][row] = static_cast<uint16_t>(seen && fine ? within_range(par[2][k], par[3][k]) : 0u);
+                        sh.vpar[part][1][g0 + k][row] = static_cast<uint16_t>(seen && fine ? par[3][k] : 0u);
                     }
                 }
+                load_par(next);
+                __syncwarp();
+                // ---- keys
                 if (!(ok = wait(sh.k_empty[buf], (at >> 1) + 1, ST_TIMEOUT_EMPTY))) break;
-                uint8_t* kd = s_k + buf * DB * BLOCK + (part * KV4_TILE + row) * 128;
+                {
+                    const uint4 sm = *reinterpret_cast<const uint4*>(sh.kpar[part][row]);
+                    const uint32_t pw[4] = {sm.x, sm.y, sm.z, sm.w};  // scales 0, 1 | 2, 3; minima 0, 1 | 2, 3
+                    uint8_t* kd = s_k + buf * DB * BLOCK + (part * KV4_TILE + row) * 128;
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const uint32_t s = src ? within_range(kp[g], kp[G + g]) : 0u, m = src ? kp[G + g] : 0u;
-                    const __half2 s2 = as_half2(s | s << 16), m2 = as_half2(m | m << 16);
+                    for (int g = 0; g < G; ++g) {
+                        const uint32_t both = g & 1 ? 0x3232 : 0x1010;
+                        const __half2 s2 = as_half2(__byte_perm(pw[g / 2], 0, both)), m2 = as_half2(__byte_perm(pw[2 + g / 2], 0, both));
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        __half2 c[4];
-                        code_pairs(src ? kw[j][g] : 0u, c);
-                        uint32_t v[4];
+                        for (int j = 0; j < 2; ++j) {
+                            __half2 c[4];
+                            code_pairs(kw[j][g], c);
+                            uint32_t v[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) v[k] = as_word(__hfma2(c[k], s2, m2));
-                        const int d = 32 * g + 8 * (2 * th + j);
-                        *reinterpret_cast<uint4*>(kd + d / 64 * BLOCK + ((d % 64 / 8) ^ (row & 7)) * 16) =
-                            make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
+                            for (int k = 0; k < 4; ++k) v[k] = as_word(__hfma2(c[k], s2, m2));
+                            const int d = 32 * g + 8 * (2 * th + j);
+                            *reinterpret_cast<uint4*>(kd + d / 64 * BLOCK + ((d % 64 / 8) ^ (row & 7)) * 16) =
+                                make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
+                        }
                     }
                 }
                 if (lane == 0) {
@@ -424,47 +461,35 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(sh.k_full[buf]));
                 load_keys(next);
-
+                // ---- values
                 if (!(ok = wait(sh.v_empty[buf], (at >> 1) + 1, ST_TIMEOUT_EMPTY))) break;
 #pragma unroll
                 for (int k = 0; k < GP; ++k) {
                     const int g = g0 + k;
-                    if (g >= G) continue;
-                    uint32_t out[4][4];  // [dim][token pair]
-                    uint32_t bad = 0;
+                    if (g < G) {
+                        const uint4 s8 = *reinterpret_cast<const uint4*>(&sh.vpar[part][0][g][8 * h]), m8 = *reinterpret_cast<const uint4*>(&sh.vpar[part][1][g][8 * h]);
+                        const uint32_t s2[4] = {s8.x, s8.y, s8.z, s8.w}, m2[4] = {m8.x, m8.y, m8.z, m8.w};  // token pairs
+                        uint32_t out[4][4];  // [dim][token pair]
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        uint32_t s[2] = {0u, 0u}, m[2] = {0u, 0u};
-                        if (src) {
+                        for (int t = 0; t < 4; ++t) {
+                            __half2 c[4];
+                            code_pairs(vw[t][k], c);  // nibble n of both tokens
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                // Nothing that is not finite goes into the products, where it would reach rows that do not see the token: it is
-                                // left out here and the rows that see it become NaN in this group.  Behind the last token, where anything
-                                // may lie, nothing is taken.
-                                const uint32_t x = vs[2 * t + j][k], y = vm[2 * t + j][k];
-                                const bool seen = token0 + 8 * h + 2 * t + j <= end, fine = finite_half(x) && finite_half(y);
-                                if (!fine && seen) bad |= 1u << (2 * t + j);
-                                s[j] = fine && seen ? within_range(x, y) : 0u;
-                                m[j] = fine && seen ? y : 0u;
-                            }
+                            for (int d = 0; d < 4; ++d) out[d][t] = as_word(__hfma2(c[d], as_half2(s2[t]), as_half2(m2[t])));
                         }
-                        const __half2 s2 = as_half2(s[0] | s[1] << 16), m2 = as_half2(m[0] | m[1] << 16);
-                        __half2 c[4];
-                        code_pairs(src ? vw[t][k] : 0u, c);  // nibble n of both tokens
 #pragma unroll
-                        for (int d = 0; d < 4; ++d) out[d][t] = as_word(__hfma2(c[d], s2, m2));
+                        for (int d = 0; d < 4; ++d) {
+                            const int dim = 32 * g + 4 * c8 + d, key = part * KV4_TILE + 8 * h;
+                            *reinterpret_cast<uint4*>(s_v + (buf * 2 + key / 64) * VBLOCK + dim * 128 + ((key % 64 / 8) ^ (dim & 7)) * 16) =
+                                make_uint4(out[d][0], out[d][1], out[d][2], out[d][3]);
+                        }
+                        if (row == 0) reinterpret_cast<uint16_t*>(&sh.bad[buf][g][0])[part] = static_cast<uint16_t>(bad[k] >> (16 * th));  // 16 tokens
                     }
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        const int dim = 32 * g + 4 * c8 + d, key = part * KV4_TILE + 8 * h;
-                        *reinterpret_cast<uint4*>(s_v + (buf * 2 + key / 64) * VBLOCK + dim * 128 + ((key % 64 / 8) ^ (dim & 7)) * 16) =
-                            make_uint4(out[d][0], out[d][1], out[d][2], out[d][3]);
-                    }
-                    if (c8 == 0) reinterpret_cast<uint8_t*>(&sh.bad[buf][g][0])[part * 2 + h] = static_cast<uint8_t>(bad);  // 8 tokens a byte
                 }
                 fence_shared();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(sh.v_full[buf]));
+                load_values(next);
                 src = next;
             }
         } else if (lane == 0 && n > 0) {
