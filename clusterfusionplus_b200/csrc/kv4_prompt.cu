@@ -8,8 +8,9 @@
 //  - 8 warps unpack: 16 tokens each of a 128-token tile, to fp16 value = code * scale + minimum in one fused rounding (2^-11 of a key or
 //    value: the operands' type; scores and sums stay fp32).  Keys as rows of dims, values as rows of tokens, which is how the cache's
 //    words hold them: two neighbouring tokens in the halves of a word are two neighbouring elements of a row of V^T.
-//  - 4 warps do the softmax, one thread a query row: no exchange between threads.  The reference of a row moves only when it is exceeded
-//    by 2^8, so the accumulator in tensor memory is hardly ever rescaled.
+//  - 4 warps do the softmax, one thread a query row: no exchange between threads, one pass over a tile's scores.  The reference of a row
+//    moves only when a score lies more than 8 binary steps above it, which after a row's first tile hardly ever happens: then the
+//    accumulator in tensor memory is rescaled and the pass repeated.
 //  - 1 thread issues the products: S of the next tile before P V of this one, so that they run under the softmax.
 // Every wait is bounded; one that runs out ends the kernel with a device status.
 #include <cuda_bf16.h>
@@ -18,6 +19,7 @@
 
 #include <cstdint>
 
+#include "f32x2.cuh"
 #include "kv4_attention.h"
 #include "kv4_layout.cuh"
 #include "mma.cuh"
@@ -65,17 +67,22 @@ __device__ __forceinline__ void tmem_load(uint32_t at, float (&x)[16]) {
         : "r"(at)
         : "memory");
 }
-__device__ __forceinline__ void tmem_load(uint32_t at, float (&x)[32]) {
+// the same in two steps: asked for now, there after tmem_wait (which names the registers, so that nothing uses them before it)
+__device__ __forceinline__ void tmem_ask(uint32_t at, float (&x)[16]) {
     __syncwarp();
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(x[8]), "=f"(x[9]), "=f"(x[10]),
-          "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15]), "=f"(x[16]), "=f"(x[17]), "=f"(x[18]), "=f"(x[19]), "=f"(x[20]),
-          "=f"(x[21]), "=f"(x[22]), "=f"(x[23]), "=f"(x[24]), "=f"(x[25]), "=f"(x[26]), "=f"(x[27]), "=f"(x[28]), "=f"(x[29]), "=f"(x[30]), "=f"(x[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(x[8]), "=f"(x[9]),
+          "=f"(x[10]), "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15])
         : "r"(at)
         : "memory");
+}
+__device__ __forceinline__ void tmem_wait(float (&x)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]), "+f"(x[4]), "+f"(x[5]), "+f"(x[6]), "+f"(x[7]), "+f"(x[8]), "+f"(x[9]),
+                   "+f"(x[10]), "+f"(x[11]), "+f"(x[12]), "+f"(x[13]), "+f"(x[14]), "+f"(x[15])
+                 :
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_store(uint32_t at, const float (&x)[16]) {
     __syncwarp();
@@ -100,14 +107,20 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e 
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 __device__ __forceinline__ uint32_t as_word(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 
+// (w & mask) | bits in one instruction
+__device__ __forceinline__ uint32_t select_or(uint32_t w, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+    return r;
+}
 // codes 0, 4 | 1, 5 | 2, 6 | 3, 7 of a word as pairs of fp16 numbers: 1024 + code and 64 + code by the bits, less 1024 and 64
 __device__ __forceinline__ void code_pairs(uint32_t w, __half2 (&c)[4]) {
     const uint32_t h = w >> 8;
     const __half2 k1024 = as_half2(0x64006400u), k64 = as_half2(0x54005400u);
-    c[0] = __hsub2(as_half2((w & 0x000f000fu) | 0x64006400u), k1024);
-    c[1] = __hsub2(as_half2((w & 0x00f000f0u) | 0x54005400u), k64);
-    c[2] = __hsub2(as_half2((h & 0x000f000fu) | 0x64006400u), k1024);
-    c[3] = __hsub2(as_half2((h & 0x00f000f0u) | 0x54005400u), k64);
+    c[0] = __hsub2(as_half2(select_or(w, 0x000f000fu, 0x64006400u)), k1024);
+    c[1] = __hsub2(as_half2(select_or(w, 0x00f000f0u, 0x54005400u)), k64);
+    c[2] = __hsub2(as_half2(select_or(h, 0x000f000fu, 0x64006400u)), k1024);
+    c[3] = __hsub2(as_half2(select_or(h, 0x00f000f0u, 0x54005400u)), k64);
 }
 // A scale whose largest value minimum + 15 scale would round beyond fp16 (the scale was rounded up at the end of the range): one step lower
 __device__ __forceinline__ uint32_t within_range(uint32_t s, uint32_t m) {
@@ -139,6 +152,7 @@ struct Shared {
     int abort;
     unsigned there[4];          // [tile % 4] bit t: the 16 tokens t of the tile exist.  Four: keys are unpacked two tiles ahead of the softmax
     uint32_t bad[2][4][4];      // [value buffer][group][token / 32]: tokens whose value parameters are not finite
+    uint32_t any_bad[2];        // a bit for each unpacking warp that found one
     __align__(16) uint16_t kpar[8][16][8];     // [unpacking warp][token][scales, minima of the keys]
     __align__(16) uint16_t vpar[8][2][4][16];  // [unpacking warp][scale, minimum of the values][group][token]
 };
@@ -173,6 +187,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
         for (int i = 0; i < 4; ++i) sh.there[i] = 0;
     }
     if (tid < 32) (&sh.bad[0][0][0])[tid] = 0;
+    if (tid < 2) sh.any_bad[tid] = 0;
     if (warp == SOFT + UNPACK) {  // scores twice 128 columns, numerators 128: 512 is the next size there is
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -250,28 +265,69 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                     fence_after();
                     const unsigned there = sh.there[at & 3];
                     const bool whole = key0 + KEYS - 1 <= all_see && there == 0xffu;
-                    float x[32], high = -INFINITY;
+                    // One pass: p by the reference that the row has, and the greatest score with it.  Only where that lies more than SLACK above the
+                    // reference (or the row had none) the reference moves, the numerators are rescaled and the pass is done again.
+                    for (bool again = false;; again = true) {
+                        constexpr int C = 16, CHUNKS = KEYS / C;
+                        float high = -INFINITY, x[2][C];
+                        Pair sum(0.f, 0.f);
+                        uint32_t held[CHUNKS / 2][C / 2];
+                        tmem_ask(tm_s + buf * KEYS + mine, x[0]);
 #pragma unroll
-                    for (int c = 0; c < KEYS; c += 32) {
-                        tmem_load(tm_s + buf * KEYS + c + mine, x);
-                        if (!whole) {
+                        for (int q = 0; q < CHUNKS; ++q) {
+                            float(&y)[C] = x[q & 1];
+                            tmem_wait(y);
+                            if (q + 1 < CHUNKS) tmem_ask(tm_s + buf * KEYS + C * (q + 1) + mine, x[(q + 1) & 1]);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (key0 + c + j > last || !(there >> ((c + j) / 16) & 1u)) x[j] = -INFINITY;
+                            for (int j = 0; j < C; j += 2) {
+                                const float2 f = fma2(Pair(y[j], y[j + 1]), Pair(factor, factor), Pair(-m, -m)).both();
+                                y[j] = f.x, y[j + 1] = f.y;
+                            }
+                            if (!whole) {
+                                const int see = there >> q & 1u ? last - key0 - C * q : -1;  // columns 0 .. see of the chunk (one 16-token tile)
+#pragma unroll
+                                for (int j = 0; j < C; ++j)
+                                    if (j > see) y[j] = -INFINITY;
+                            }
+#pragma unroll
+                            for (int j = 0; j < C; ++j) high = fmaxf(high, y[j]);
+                            uint32_t(&h)[C / 2] = held[q % (CHUNKS / 2)];
+#pragma unroll
+                            for (int j = 0; j < C; j += 2) {
+                                const Pair p(ex2(y[j]), ex2(y[j + 1]));
+                                sum = sum + p;
+                                const float2 f = p.both();
+                                h[j / 2] = pack_half2(f.x, f.y);
+                            }
+                            if (q + 1 < CHUNKS / 2) continue;
+                            // the products of the tile before read P: the first half waits in registers for their end
+                            if (q + 1 == CHUNKS / 2 && !again && i > 0) {
+                                if (!(ok = wait(sh.pv_done, at - 1, ST_TIMEOUT_FULL))) {
+                                    tmem_wait(x[(q + 1) & 1]);
+                                    break;
+                                }
+                                fence_after();
+                            }
+#pragma unroll
+                            for (int w = q + 1 == CHUNKS / 2 ? 0 : q; w <= q; ++w)
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) {
+                                    const uint32_t(&v)[C / 2] = held[w % (CHUNKS / 2)];
+                                    *reinterpret_cast<uint4*>(s_p + w / 4 * BLOCK + tid * 128 + ((w % 4 * 2 + j) ^ (tid & 7)) * 16) =
+                                        make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                                }
                         }
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) high = fmaxf(high, x[j]);
-                    }
-                    high = high == -INFINITY ? -INFINITY : high * factor;
-                    // the reference: the first tile's greatest; later only if exceeded by SLACK
-                    const bool start = i == 0 || l == 0.f;
-                    const float up_by = start ? (high == -INFINITY ? 0.f : high - m) : (high > m + SLACK ? high - m : 0.f);
-                    if (i > 0) {  // the products before have read P and written O
-                        if (!(ok = wait(sh.pv_done, at - 1, ST_TIMEOUT_FULL))) break;
-                        fence_after();
-                        if (__any_sync(0xffffffffu, up_by != 0.f && l != 0.f)) {
-                            const float keep = l != 0.f ? ex2(-up_by) : 1.f;
-                            l *= keep;
+                        if (!ok) break;
+                        const float2 both = sum.both();
+                        const bool move = !again && (high > SLACK || (l == 0.f && high != -INFINITY));
+                        if (!__any_sync(0xffffffffu, move)) {
+                            l += both.x + both.y;
+                            break;
+                        }
+                        const float up = move ? high : 0.f, keep = l != 0.f ? ex2(-up) : 1.f;
+                        m += up;
+                        l *= keep;
+                        if (i > 0)
                             for (int c = 0; c < N; c += 16) {
                                 float o[16];
                                 tmem_load(tm_o + c + mine, o);
@@ -279,43 +335,18 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                                 for (int j = 0; j < 16; ++j) o[j] *= keep;
                                 tmem_store(tm_o + c + mine, o);
                             }
-                        }
                     }
-                    m += up_by;
-                    float sum = 0.f;
+                    if (!ok || !(ok = wait(sh.v_full[buf], at >> 1, ST_TIMEOUT_FULL))) break;  // for sh.bad; in time for P V anyway
+                    if (sh.any_bad[buf]) {
 #pragma unroll
-                    for (int c = 0; c < KEYS; c += 32) {
-                        tmem_load(tm_s + buf * KEYS + c + mine, x);
+                        for (int g = 0; g < G; ++g)
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) x[j] = fmaf(x[j], factor, -m);
-                        if (!whole) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (key0 + c + j > last || !(there >> ((c + j) / 16) & 1u)) x[j] = -INFINITY;
-                        }
-#pragma unroll
-                        for (int j = 0; j < 32; j += 8) {
-                            float p[8];
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) {
-                                p[k] = ex2(x[j + k]);
-                                sum += p[k];
+                            for (int k = 0; k < 4; ++k) {
+                                const int see = last - key0 - 32 * k;
+                                const uint32_t seen = see < 0 ? 0u : see >= 31 ? 0xffffffffu : (2u << see) - 1u;
+                                if (sh.bad[buf][g][k] & seen) broken |= 1u << g;
                             }
-                            const int chunk = (c % 64 + j) / 8;
-                            *reinterpret_cast<uint4*>(s_p + c / 64 * BLOCK + tid * 128 + (chunk ^ (tid & 7)) * 16) =
-                                make_uint4(pack_half2(p[0], p[1]), pack_half2(p[2], p[3]), pack_half2(p[4], p[5]), pack_half2(p[6], p[7]));
-                        }
                     }
-                    l += sum;
-                    if (!(ok = wait(sh.v_full[buf], at >> 1, ST_TIMEOUT_FULL))) break;  // for sh.bad; in time for P V anyway
-#pragma unroll
-                    for (int g = 0; g < G; ++g)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int see = last - key0 - 32 * k;
-                            const uint32_t seen = see < 0 ? 0u : see >= 31 ? 0xffffffffu : (2u << see) - 1u;
-                            if (sh.bad[buf][g][k] & seen) broken |= 1u << g;
-                        }
                     fence_before();
                     fence_shared();
                     mbar_arrive(bar(sh.p_full));
@@ -463,6 +494,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                 load_keys(next);
                 // ---- values
                 if (!(ok = wait(sh.v_empty[buf], (at >> 1) + 1, ST_TIMEOUT_EMPTY))) break;
+                if (lane == 0) {
+                    uint32_t found = bad[0];
+#pragma unroll
+                    for (int k = 1; k < GP; ++k) found |= bad[k];
+                    if (found) atomicOr(&sh.any_bad[buf], 1u << part);
+                    else atomicAnd(&sh.any_bad[buf], ~(1u << part));
+                }
 #pragma unroll
                 for (int k = 0; k < GP; ++k) {
                     const int g = g0 + k;

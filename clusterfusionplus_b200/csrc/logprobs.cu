@@ -21,9 +21,13 @@
 #include <cstdint>
 
 #include "../../include/clusterfusion_b200.h"
+#include "f32x2.cuh"
 #include "host_common.h"
 
 namespace {
+
+using cfb::fma2;
+using cfb::Pair;
 
 constexpr int LT = 256;        // threads of a CTA
 constexpr int LW = LT / 32;
@@ -80,33 +84,6 @@ __device__ __forceinline__ void extremes(const uint4& v, float& hi, float& lo, _
 }
 __device__ __forceinline__ void extremes(const uint4& v, float& hi, float& lo, __nv_bfloat16) {
     extremes_of_pairs<__nv_bfloat162>(v, hi, lo, [](__nv_bfloat162 x) { return __bfloat1622float2(x); });
-}
-
-// Two fp32 numbers in one register pair: sm_100 adds and multiplies both with one instruction
-struct Pair {
-    unsigned long long v;
-    __device__ __forceinline__ Pair() {}
-    __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-    __device__ __forceinline__ float2 both() const {
-        float2 f;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-        return f;
-    }
-};
-__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
-    Pair r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
-    Pair r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-    Pair r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
 }
 
 // Running statistics of a thread relative to a reference m within 4 of its greatest element (e^4 costs no precision, and the
