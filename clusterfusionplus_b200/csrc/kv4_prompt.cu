@@ -8,9 +8,9 @@
 //  - 8 warps unpack: 16 tokens each of a 128-token tile, to fp16 value = code * scale + minimum in one fused rounding (2^-11 of a key or
 //    value: the operands' type; scores and sums stay fp32).  Keys as rows of dims, values as rows of tokens, which is how the cache's
 //    words hold them: two neighbouring tokens in the halves of a word are two neighbouring elements of a row of V^T.
-//  - 4 warps do the softmax, one thread a query row: no exchange between threads, one pass over a tile's scores.  The reference of a row
-//    moves only when a score lies more than 8 binary steps above it, which after a row's first tile hardly ever happens: then the
-//    accumulator in tensor memory is rescaled and the pass repeated.
+//  - 8 warps do the softmax, two threads a query row, in one pass over a tile's scores.  The reference of a row moves only when a score
+//    lies more than 8 binary steps above it, which after a row's first tile hardly ever happens: then the accumulator in tensor
+//    memory is rescaled and the pass repeated.
 //  - 1 thread issues the products: S of the next tile before P V of this one, so that they run under the softmax.
 // Every wait is bounded; one that runs out ends the kernel with a device status.
 #include <cuda_bf16.h>
@@ -30,7 +30,7 @@ namespace {
 
 constexpr int ROWS = 128;            // query rows of a CTA
 constexpr int KEYS = 128;            // tokens of a tile
-constexpr int SOFT = 4, UNPACK = 8;  // warps; one more issues the products
+constexpr int SOFT = 8, UNPACK = 8;  // warps; one more issues the products
 constexpr int THREADS = 32 * (SOFT + UNPACK + 1);
 constexpr int BLOCK = 128 * 128;     // bytes of a K-major operand block of 128 rows x 64 elements
 constexpr float SLACK = 8.f;         // binary steps that a score may lie above its row's reference
@@ -151,8 +151,9 @@ struct Shared {
     uint32_t tmem;
     int abort;
     unsigned there[4];          // [tile % 4] bit t: the 16 tokens t of the tile exist.  Four: keys are unpacked two tiles ahead of the softmax
-    uint32_t bad[2][4][4];      // [value buffer][group][token / 32]: tokens whose value parameters are not finite
-    uint32_t any_bad[2];        // a bit for each unpacking warp that found one
+    unsigned long long agreed[4], summed[4];  // of the two warps that share rows
+    float high[2][2][ROWS], sums[2][ROWS];    // [tile & 1][half][row]: greatest score; [half][row]: denominator
+    int not_finite;                           // a token that some row sees has value parameters that are not finite
     __align__(16) uint16_t kpar[8][16][8];     // [unpacking warp][token][scales, minima of the keys]
     __align__(16) uint16_t vpar[8][2][4][16];  // [unpacking warp][scale, minimum of the values][group][token]
 };
@@ -183,11 +184,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
         mbar_init(bar(sh.pv_done), 1);
         mbar_init(bar(sh.drain), 1);
         mbar_fence_init();
-        sh.abort = 0;
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(bar(sh.agreed[i]), 64);
+            mbar_init(bar(sh.summed[i]), 64);
+        }
+        sh.abort = sh.not_finite = 0;
         for (int i = 0; i < 4; ++i) sh.there[i] = 0;
     }
-    if (tid < 32) (&sh.bad[0][0][0])[tid] = 0;
-    if (tid < 2) sh.any_bad[tid] = 0;
     if (warp == SOFT + UNPACK) {  // scores twice 128 columns, numerators 128: 512 is the next size there is
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -220,15 +223,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
         bool ok = true;
 
         if (warp < SOFT) {
-            // ================================================================ softmax: thread = row
-            const int r = r0 + tid;
+            // ================================================================ softmax: two threads a row, 64 columns of a tile each
+            const int line = tid & (ROWS - 1), half = warp >> 2, pair = warp & 3, r = r0 + line;
             const bool real = r < rows;
             const int qi = real ? r / per : 0, head = kvh * per + (real ? r % per : 0);
             const T* src = static_cast<const T*>(a.query) + static_cast<long long>(first + qi) * a.q_ts + head * a.q_hs;
+            T* dst = static_cast<T*>(a.out) + (static_cast<long long>(first + qi) * a.heads + head) * a.D;
             const int last = real ? static_cast<int>(max(min(before + qi, cap - 1), -1ll)) : -1;
             const int all_see = static_cast<int>(max(min(before + r0 / per, cap - 1), -1ll));  // every real row sees these
-            float top = 0.f;
             if (n > 0) {
+                float top = 0.f;
                 for (int d = 0; d < a.D; d += 8) {
                     const uint4 v = real ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
                     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -241,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                 // a power of two takes the row to at most 2^10 (exact; bf16 reaches beyond fp16), the scale's sign goes along
                 const int e = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100);
                 const float up = copysignf(power_of_two(min(9 - e, 127)), a.scale_log2);
-                for (int d = 0; d < N; d += 8) {
+                for (int d = 8 * half; d < N; d += 16) {
                     const uint4 v = real && d < a.D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
                     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
                     uint32_t o[4];
@@ -250,41 +254,42 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                         const float2 f = to_float2<T>(w[i]);
                         o[i] = pack_half2(f.x * up, f.y * up);
                     }
-                    *reinterpret_cast<uint4*>(s_q + d / 64 * BLOCK + tid * 128 + ((d % 64 / 8) ^ (tid & 7)) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<uint4*>(s_q + d / 64 * BLOCK + line * 128 + ((d % 64 / 8) ^ (line & 7)) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
                 }
                 fence_shared();
                 mbar_arrive(bar(sh.q_full));
                 const float factor = fminf(fabsf(a.scale_log2) * power_of_two(e - 9), 3.4e38f);
-                const uint32_t mine = static_cast<uint32_t>(warp * 32) << 16;  // this warp's lanes of tensor memory
+                const uint32_t mine = static_cast<uint32_t>(pair * 32) << 16;  // this warp's lanes of tensor memory
 
-                float m = 0.f, l = 0.f;
-                unsigned broken = 0;  // groups in which this row meets a value that is not finite
+                float m = 0.f, l = 0.f;  // reference of the row, sum of this thread's p
+                bool set = false;        // the row has a reference
                 for (int i = 0; ok && i < n; ++i) {
-                    const int at = done + i, buf = at & 1, key0 = i * KEYS;
+                    const int at = done + i, buf = at & 1, key0 = i * KEYS + 64 * half;
                     if (!(ok = wait(sh.s_full[buf], at >> 1, ST_TIMEOUT_FULL))) break;
                     fence_after();
                     const unsigned there = sh.there[at & 3];
-                    const bool whole = key0 + KEYS - 1 <= all_see && there == 0xffu;
+                    const bool whole = i * KEYS + KEYS - 1 <= all_see && there == 0xffu;
                     // One pass: p by the reference that the row has, and the greatest score with it.  Only where that lies more than SLACK above the
                     // reference (or the row had none) the reference moves, the numerators are rescaled and the pass is done again.
                     for (bool again = false;; again = true) {
-                        constexpr int C = 16, CHUNKS = KEYS / C;
+                        constexpr int C = 16, CHUNKS = 64 / C;
                         float high = -INFINITY, x[2][C];
                         Pair sum(0.f, 0.f);
                         uint32_t held[CHUNKS / 2][C / 2];
-                        tmem_ask(tm_s + buf * KEYS + mine, x[0]);
+                        const uint32_t from = tm_s + buf * KEYS + 64 * half + mine;
+                        tmem_ask(from, x[0]);
 #pragma unroll
                         for (int q = 0; q < CHUNKS; ++q) {
                             float(&y)[C] = x[q & 1];
                             tmem_wait(y);
-                            if (q + 1 < CHUNKS) tmem_ask(tm_s + buf * KEYS + C * (q + 1) + mine, x[(q + 1) & 1]);
+                            if (q + 1 < CHUNKS) tmem_ask(from + C * (q + 1), x[(q + 1) & 1]);
 #pragma unroll
                             for (int j = 0; j < C; j += 2) {
                                 const float2 f = fma2(Pair(y[j], y[j + 1]), Pair(factor, factor), Pair(-m, -m)).both();
                                 y[j] = f.x, y[j + 1] = f.y;
                             }
                             if (!whole) {
-                                const int see = there >> q & 1u ? last - key0 - C * q : -1;  // columns 0 .. see of the chunk (one 16-token tile)
+                                const int see = there >> (4 * half + q) & 1u ? last - key0 - C * q : -1;  // columns 0 .. see of the chunk (16 tokens: one page's)
 #pragma unroll
                                 for (int j = 0; j < C; ++j)
                                     if (j > see) y[j] = -INFINITY;
@@ -313,22 +318,29 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
 #pragma unroll
                                 for (int j = 0; j < 2; ++j) {
                                     const uint32_t(&v)[C / 2] = held[w % (CHUNKS / 2)];
-                                    *reinterpret_cast<uint4*>(s_p + w / 4 * BLOCK + tid * 128 + ((w % 4 * 2 + j) ^ (tid & 7)) * 16) =
+                                    *reinterpret_cast<uint4*>(s_p + half * BLOCK + line * 128 + ((w * 2 + j) ^ (line & 7)) * 16) =
                                         make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                                 }
                         }
                         if (!ok) break;
-                        const float2 both = sum.both();
-                        const bool move = !again && (high > SLACK || (l == 0.f && high != -INFINITY));
+                        if (!again) {  // the row's other thread: both have to come to the same reference
+                            sh.high[at & 1][half][line] = high;
+                            mbar_arrive(bar(sh.agreed[pair]));
+                            if (!(ok = wait(sh.agreed[pair], at, ST_TIMEOUT_FULL))) break;
+                            high = fmaxf(high, sh.high[at & 1][half ^ 1][line]);
+                        }
+                        const bool move = !again && (high > SLACK || (!set && high != -INFINITY));
                         if (!__any_sync(0xffffffffu, move)) {
+                            const float2 both = sum.both();
                             l += both.x + both.y;
                             break;
                         }
-                        const float up = move ? high : 0.f, keep = l != 0.f ? ex2(-up) : 1.f;
-                        m += up;
+                        const float by = move ? high : 0.f, keep = set ? ex2(-by) : 1.f;
+                        m += by;
                         l *= keep;
+                        set |= move;
                         if (i > 0)
-                            for (int c = 0; c < N; c += 16) {
+                            for (int c = 16 * half; c < N; c += 32) {
                                 float o[16];
                                 tmem_load(tm_o + c + mine, o);
 #pragma unroll
@@ -336,48 +348,50 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                                 tmem_store(tm_o + c + mine, o);
                             }
                     }
-                    if (!ok || !(ok = wait(sh.v_full[buf], at >> 1, ST_TIMEOUT_FULL))) break;  // for sh.bad; in time for P V anyway
-                    if (sh.any_bad[buf]) {
-#pragma unroll
-                        for (int g = 0; g < G; ++g)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const int see = last - key0 - 32 * k;
-                                const uint32_t seen = see < 0 ? 0u : see >= 31 ? 0xffffffffu : (2u << see) - 1u;
-                                if (sh.bad[buf][g][k] & seen) broken |= 1u << g;
-                            }
-                    }
+                    if (!ok) break;
                     fence_before();
                     fence_shared();
                     mbar_arrive(bar(sh.p_full));
                 }
-                if (ok && (ok = wait(sh.pv_done, done + n - 1, ST_TIMEOUT_FULL))) {
+                if (ok) {
+                    sh.sums[half][line] = l;
+                    mbar_arrive(bar(sh.summed[pair]));
+                    ok = wait(sh.summed[pair], items, ST_TIMEOUT_FULL) && wait(sh.pv_done, done + n - 1, ST_TIMEOUT_FULL);
+                }
+                if (ok) {
                     fence_after();
-                    T* dst = static_cast<T*>(a.out) + (static_cast<long long>(first + qi) * a.heads + head) * a.D;
-                    const float inv = 1.f / l;
-                    for (int c = 0; c < N; c += 16) {
+                    l += sh.sums[half ^ 1][line];
+                    unsigned broken = 0;  // groups in which the row sees a value that is not finite: looked up only if there was one at all
+                    if (sh.not_finite) {
+                        const int tiles_a_page = a.page / KV4_TILE;
+                        for (int t = 0; t * KV4_TILE <= last; ++t) {
+                            const int held = table[t / tiles_a_page];
+                            if (held < 0 || held >= a.pages) continue;
+                            const uint8_t* tile = a.cache + ((static_cast<long long>(held) * a.kv_heads + kvh) * tiles_a_page + t % tiles_a_page) * TB;
+                            for (int k = 0; k < KV4_TILE && t * KV4_TILE + k <= last; ++k)
+                                for (int g = 0; g < G; ++g)
+                                    if (!finite_half(*reinterpret_cast<const unsigned short*>(tile + kv4_param(G, k, 2, g))) ||
+                                        !finite_half(*reinterpret_cast<const unsigned short*>(tile + kv4_param(G, k, 3, g))))
+                                        broken |= 1u << g;
+                        }
+                        __syncwarp();
+                    }
+                    const float by = l == 0.f ? 0.f : 1.f / l;  // no token seen: zeros; NaN stays
+                    for (int c = 16 * half; c < N; c += 32) {
                         float o[16];
                         tmem_load(tm_o + c + mine, o);
-                        if (broken >> (c / 32) & 1u) {
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) o[j] = __int_as_float(0x7fffffff);
-                        }
-                        if (l == 0.f) {  // no token seen
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) o[j] = 0.f;
-                        }
-                        const float by = l == 0.f ? 1.f : inv;
+                        for (int j = 0; j < 16; ++j) o[j] = broken >> (c / 32) & 1u ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : o[j] * by;
 #pragma unroll
                         for (int j = 0; j < 16; j += 8)
                             if (real && c + j < a.D)
-                                *reinterpret_cast<uint4*>(dst + c + j) = make_uint4(pack<T>(o[j] * by, o[j + 1] * by), pack<T>(o[j + 2] * by, o[j + 3] * by),
-                                                                                    pack<T>(o[j + 4] * by, o[j + 5] * by), pack<T>(o[j + 6] * by, o[j + 7] * by));
+                                *reinterpret_cast<uint4*>(dst + c + j) =
+                                    make_uint4(pack<T>(o[j], o[j + 1]), pack<T>(o[j + 2], o[j + 3]), pack<T>(o[j + 4], o[j + 5]), pack<T>(o[j + 6], o[j + 7]));
                     }
                     fence_before();
                 }
             } else if (real) {
-                T* dst = static_cast<T*>(a.out) + (static_cast<long long>(first + qi) * a.heads + head) * a.D;
-                for (int d = 0; d < a.D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
+                for (int d = 8 * half; d < a.D; d += 16) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
             }
         } else if (warp < SOFT + UNPACK) {
             // ================================================================ unpacking: warp = 16 tokens of each tile
@@ -445,14 +459,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                 const uint8_t* next = find(held, i + 1);
                 held = entry(i + 2);
                 // ---- parameters (those of a missing page are 0: so are its keys and values)
-                uint32_t bad[GP];  // tokens of groups k (low half) and GP + k
 #pragma unroll
                 for (int k = 0; k < GP; ++k) {
-                    // Nothing that is not finite goes into P V, where it would reach rows that do not see the token: it is left out here and the
-                    // rows that see it become NaN in this group.  Behind the last token, where anything may lie, nothing is taken.
-                    const bool seen = token0 + row <= end, fine = finite_half(par[2][k]) && finite_half(par[3][k]);
-                    bad[k] = __ballot_sync(0xffffffffu, seen && !fine);
+                    // Nothing that is not finite goes into P V, where it would reach rows that do not see the token: it is left out here, and the
+                    // rows that see it become NaN in this group at the end.  Behind the last token, where anything may lie, nothing is taken.
                     if (g0 + k < G) {
+                        const bool seen = token0 + row <= end, fine = finite_half(par[2][k]) && finite_half(par[3][k]);
+                        if (seen && !fine) sh.not_finite = 1;
                         sh.kpar[part][row][g0 + k] = static_cast<uint16_t>(within_range(par[0][k], par[1][k]));
                         sh.kpar[part][row][4 + g0 + k] = static_cast<uint16_t>(par[1][k]);
                         sh.vpar[part][0][g0 + k][row] = static_cast<uint16_t>(seen && fine ? within_range(par[2][k], par[3][k]) : 0u);
@@ -494,13 +507,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                 load_keys(next);
                 // ---- values
                 if (!(ok = wait(sh.v_empty[buf], (at >> 1) + 1, ST_TIMEOUT_EMPTY))) break;
-                if (lane == 0) {
-                    uint32_t found = bad[0];
-#pragma unroll
-                    for (int k = 1; k < GP; ++k) found |= bad[k];
-                    if (found) atomicOr(&sh.any_bad[buf], 1u << part);
-                    else atomicAnd(&sh.any_bad[buf], ~(1u << part));
-                }
 #pragma unroll
                 for (int k = 0; k < GP; ++k) {
                     const int g = g0 + k;
@@ -521,7 +527,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                             *reinterpret_cast<uint4*>(s_v + (buf * 2 + key / 64) * VBLOCK + dim * 128 + ((key % 64 / 8) ^ (dim & 7)) * 16) =
                                 make_uint4(out[d][0], out[d][1], out[d][2], out[d][3]);
                         }
-                        if (row == 0) reinterpret_cast<uint16_t*>(&sh.bad[buf][g][0])[part] = static_cast<uint16_t>(bad[k] >> (16 * th));  // 16 tokens
                     }
                 }
                 fence_shared();
