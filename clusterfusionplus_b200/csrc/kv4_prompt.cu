@@ -201,7 +201,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
     const uint32_t tm_s = sh.tmem, tm_o = sh.tmem + 2 * KEYS;  // columns: scores of two tiles, numerators
     const AbortCtl ctl{&sh.abort, a.status};
     // one answer for the whole warp, which goes on together
-    auto wait = [&](unsigned long long& b, int phase, int code) { return __all_sync(0xffffffffu, mbar_wait(bar(b), phase & 1, ctl, code)) != 0; };
+    auto wait_one = [&](unsigned long long& b, int phase, int code) { return mbar_wait(bar(b), phase & 1, ctl, code); };
+    auto wait = [&](unsigned long long& b, int phase, int code) { return __all_sync(0xffffffffu, wait_one(b, phase, code)) != 0; };
 
     const int b = blockIdx.x / a.kv_heads, kvh = blockIdx.x - b * a.kv_heads, per = a.heads / a.kv_heads;
     int first = b, n_q = 1;
@@ -248,12 +249,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                 for (int d = 8 * half; d < N; d += 16) {
                     const uint4 v = real && d < a.D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
                     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    float v8[8];
                     uint32_t o[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float2 f = to_float2<T>(w[i]);
-                        o[i] = pack_half2(f.x * up, f.y * up);
+                        v8[2 * i] = f.x * up, v8[2 * i + 1] = f.y * up;
                     }
+                    // dims 0, 4, 1, 5, 2, 6, 3, 7 of each eight: the order in which the keys come out of their words
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = pack_half2(v8[i], v8[i + 4]);
                     *reinterpret_cast<uint4*>(s_q + d / 64 * BLOCK + line * 128 + ((d % 64 / 8) ^ (line & 7)) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
                 }
                 fence_shared();
@@ -399,15 +404,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
             // as soon as its registers are free.  The parameters of the 16 tokens are looked over once, and handed round through shared memory in
             // the order of their use.
             const int part = warp - SOFT, tiles_a_page = a.page / KV4_TILE;
-            constexpr int NOT_NEEDED = -2;
-            auto entry = [&](int i) {
-                const long long tile = static_cast<long long>(i) * (KEYS / KV4_TILE) + part;
-                return i < n && tile * KV4_TILE <= end ? table[static_cast<int>(tile) / tiles_a_page] : NOT_NEEDED;
+            const int step_col = (KEYS / KV4_TILE) / tiles_a_page, step_in = (KEYS / KV4_TILE) % tiles_a_page;
+            int looked = 0, col = part / tiles_a_page, in = part % tiles_a_page;  // tiles looked up so far; column and place in the page of the next
+            const int wanted = n > 0 && part * KV4_TILE <= end ? static_cast<int>((end - part * KV4_TILE) / KEYS) + 1 : 0;  // tiles that exist for this warp
+            int held = -1, held_in = 0;  // page and place of the tile looked up last
+            auto look = [&] {
+                held_in = in;
+                held = looked < wanted ? table[col] : -1;
+                ++looked;
+                col += step_col, in += step_in;
+                if (in >= tiles_a_page) in -= tiles_a_page, ++col;
             };
-            auto find = [&](int held, int i) -> const uint8_t* {
-                if (held >= 0 && held < a.pages)
-                    return a.cache + ((static_cast<long long>(held) * a.kv_heads + kvh) * tiles_a_page + (i * (KEYS / KV4_TILE) + part) % tiles_a_page) * TB;
-                if (held != NOT_NEEDED && lane == 0) atomicCAS(a.status, 0, ST_BAD_SLOT);
+            auto find = [&]() -> const uint8_t* {  // of the tile looked up last
+                if (held >= 0 && held < a.pages) return a.cache + ((static_cast<long long>(held) * a.kv_heads + kvh) * tiles_a_page + held_in) * TB;
+                if (looked <= wanted && lane == 0) atomicCAS(a.status, 0, ST_BAD_SLOT);
                 return nullptr;
             };
             // keys: lane = row (16) and half of the t's; values: lane = (c, h) and half of the groups (neighbouring lanes differ in c & 1 and
@@ -448,16 +458,17 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int k = 0; k < GP; ++k) vw[t][k] = 0;
-            const uint8_t* src = find(entry(0), 0);
+            look();
+            const uint8_t* src = find();
             load_par(src);
             load_keys(src);
             load_values(src);
-            int held = entry(1);
+            look();
             for (int i = 0; ok && i < n; ++i) {
                 const int at = done + i, buf = at & 1;
                 const long long token0 = (static_cast<long long>(i) * (KEYS / KV4_TILE) + part) * KV4_TILE;
-                const uint8_t* next = find(held, i + 1);
-                held = entry(i + 2);
+                const uint8_t* next = find();
+                look();
                 // ---- parameters (those of a missing page are 0: so are its keys and values)
 #pragma unroll
                 for (int k = 0; k < GP; ++k) {
@@ -493,7 +504,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                             for (int k = 0; k < 4; ++k) v[k] = as_word(__hfma2(c[k], s2, m2));
                             const int d = 32 * g + 8 * (2 * th + j);
                             *reinterpret_cast<uint4*>(kd + d / 64 * BLOCK + ((d % 64 / 8) ^ (row & 7)) * 16) =
-                                make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
+                                make_uint4(v[0], v[1], v[2], v[3]);  // (the queries' dims are in the same order)
                         }
                     }
                 }
@@ -541,7 +552,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
             const uint32_t q = smem_u32(s_q), k0 = smem_u32(s_k), v0 = smem_u32(s_v), p = smem_u32(s_p);
             auto scores = [&](int i) {
                 const int at = done + i, buf = at & 1;
-                if (!mbar_wait(bar(sh.k_full[buf]), (at >> 1) & 1, ctl, ST_TIMEOUT_FULL)) return false;
+                if (!wait_one(sh.k_full[buf], (at >> 1) & 1, ST_TIMEOUT_FULL)) return false;
                 fence_after();
                 for (int s = 0; s < N / 16; ++s)
                     product(tm_s + buf * KEYS, operand(q + s / 4 * BLOCK + s % 4 * 32), operand(k0 + buf * DB * BLOCK + s / 4 * BLOCK + s % 4 * 32), d_s, s > 0);
@@ -549,11 +560,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                 commit(bar(sh.k_empty[buf]));
                 return true;
             };
-            ok = mbar_wait(bar(sh.q_full), items & 1, ctl, ST_TIMEOUT_FULL) && scores(0);
+            ok = wait_one(sh.q_full, items & 1, ST_TIMEOUT_FULL) && scores(0);
             for (int i = 0; ok && i < n; ++i) {
                 const int at = done + i, buf = at & 1;
                 if (i + 1 < n && !(ok = scores(i + 1))) break;
-                if (!(ok = mbar_wait(bar(sh.v_full[buf]), (at >> 1) & 1, ctl, ST_TIMEOUT_FULL) && mbar_wait(bar(sh.p_full), at & 1, ctl, ST_TIMEOUT_FULL))) break;
+                if (!(ok = wait_one(sh.v_full[buf], (at >> 1) & 1, ST_TIMEOUT_FULL) && wait_one(sh.p_full, at & 1, ST_TIMEOUT_FULL))) break;
                 fence_after();
                 for (int s = 0; s < KEYS / 16; ++s)
                     product(tm_o, operand(p + s / 4 * BLOCK + s % 4 * 32), operand(v0 + (buf * 2 + s / 4) * VBLOCK + s % 4 * 32), d_o, i > 0 || s > 0);
