@@ -3,7 +3,21 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace cfb {
+
+// cudaFuncSetAttribute costs a microsecond of every call: once for each kernel and device is enough.  `done` is the kernel's own record.
+inline cudaError_t allow_shared_once(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    const cudaError_t s = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (s == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_release);
+    return s;
+}
 
 struct Kv4AttnArgs {
     const void* query;

@@ -8,6 +8,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 
 #include "../../include/clusterfusion_b200.h"
@@ -215,8 +216,18 @@ int check_launch(const char* what) {
     return CF_OK;
 }
 
-// From this many query rows a (request, cached head) on, 128 of them share each unpacked tile; below, each 8 or 16 read the cache for themselves
-bool prompt_sized(int64_t heads, int64_t kv_heads, int64_t max_q_len) { return max_q_len * (heads / kv_heads) > 48; }
+// Whether 128 query rows of a (request, cached head) shall share each unpacked tile (kv4_prompt.cu) or 16 at a time read the cache for
+// themselves (kv4_decode.cu).  The first takes 2.3 us for 128 tokens in each of 148 CTAs and does not divide the tokens among CTAs; the second
+// divides them evenly and takes 2 ns for 16 rows x 16 tokens, 8 us at least.  Measured (rows of a (request, head); the second against the
+// first): 32 pairs of 2048 tokens 48 rows 44 : 40 us, 24 rows 24 : 39; 256 pairs of 1000 tokens 24 rows 65 : 47; 8 pairs of 8192 tokens
+// 128 rows 44 : 136; 32 pairs of 4000 tokens 64 rows 68 : 72, 128 rows 89 : 74.
+bool prompt_sized(int64_t batch, int64_t heads, int64_t kv_heads, int64_t tokens, int64_t max_q_len) {
+    const int64_t rows = max_q_len * (heads / kv_heads);
+    if (rows <= 16) return false;
+    const double pairs = static_cast<double>(batch) * kv_heads;
+    const double turns = ceil(pairs * ((rows + 127) / 128) / 148);
+    return 8 + 0.002 * pairs * ((rows + 15) / 16) * ((tokens + 15) / 16) > 4 + 2.3 * turns * ((tokens + 127) / 128);
+}
 
 bool aligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
@@ -277,7 +288,7 @@ int cf_kv4_read(const void* cache, int64_t pages, int64_t page_size, int64_t kv_
 
 int64_t cf_kv4_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens, int64_t max_q_len) {
     if (batch < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || head_dim < 1 || head_dim > KV4_MAX_DIM || max_tokens < 1 || max_q_len < 1) return 0;
-    if (prompt_sized(heads, kv_heads, max_q_len)) return 0;
+    if (prompt_sized(batch, heads, kv_heads, max_tokens, max_q_len)) return 0;
     return kv4_few_uses_workspace(batch, heads, kv_heads, max_tokens, max_q_len) ? kv4_few_workspace(heads, kv_heads, static_cast<int>(head_dim), max_q_len) : 0;
 }
 
@@ -299,9 +310,10 @@ int cf_kv4_attention(const void* query, int dtype, int64_t rows, int64_t heads, 
     if (rows > 0x3fffffff / heads) return cf_host_fail(CF_ERR_INVALID, "%lld query rows of %lld heads in one call", (long long)rows, (long long)heads);
     if (batch * kv_heads > 0x7fffffff / 8) return cf_host_fail(CF_ERR_INVALID, "%lld requests of %lld cached heads in one call", (long long)batch, (long long)kv_heads);
     const int64_t needed = kv4_few_workspace(heads, kv_heads, static_cast<int>(head_dim), max_q_len);
-    if (workspace && !prompt_sized(heads, kv_heads, max_q_len) && (workspace_bytes < needed || !aligned(workspace, 16)))
+    const bool prompt = prompt_sized(batch, heads, kv_heads, table_width * page_size, max_q_len);
+    if (workspace && !prompt && (workspace_bytes < needed || !aligned(workspace, 16)))
         return cf_host_fail(CF_ERR_INVALID, "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)needed);
-    static int* status_word[64] = {};  // address of the device status word, by device
+    static std::atomic<int*> status_word[64];  // address of the device status word, by device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev < 0 || dev >= 64)) return cf_host_fail(CF_ERR_UNSUPPORTED, "device index %d", dev);
@@ -314,8 +326,8 @@ int cf_kv4_attention(const void* query, int dtype, int64_t rows, int64_t heads, 
     const Kv4AttnArgs a{query, static_cast<const uint8_t*>(cache), block_table, kv_lens, qo_indptr, out, query_token_stride, query_head_stride, table_stride, table_width, rows,
                         static_cast<int>(batch), static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(head_dim), static_cast<int>(page_size),
                         static_cast<int>(pages), scale * 1.4426950408889634f, status_word[dev], workspace};
-    e = prompt_sized(heads, kv_heads, max_q_len) ? kv4_attention_prompt(a, dtype == CF_DTYPE_BF16, max_q_len, static_cast<cudaStream_t>(stream))
-                                                 : kv4_attention_few(a, dtype == CF_DTYPE_BF16, max_q_len, static_cast<cudaStream_t>(stream));
+    e = prompt ? kv4_attention_prompt(a, dtype == CF_DTYPE_BF16, max_q_len, static_cast<cudaStream_t>(stream))
+               : kv4_attention_few(a, dtype == CF_DTYPE_BF16, max_q_len, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cf_host_fail(CF_ERR_CUDA, "4-bit attention launch failed: %s", cudaGetErrorString(e));
     return CF_OK;
 }

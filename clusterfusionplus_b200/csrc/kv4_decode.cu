@@ -775,10 +775,6 @@ constexpr int SMS = 148;
 constexpr int LEAST = 2 * W;  // tiles of a CTA's piece, at least: below that the join costs more than it saves
 template <int NT> constexpr int line_ctas() { return SMS * (NT == 1 ? 4 : 2); }
 
-template <class K> cudaError_t allow_smem(K kernel, int bytes) {
-    return bytes > 32 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : cudaSuccess;  // more than 48 KB with the static part
-}
-
 template <class T, int G, int NT> cudaError_t launch(const Kv4AttnArgs& a, long long max_q_len, cudaStream_t st) {
     constexpr int COLS = 8 * NT;
     constexpr int ring = W * STAGES * 2 * kv4_tile_bytes(G), merge = W * COLS * (32 * G + 4) * 4, smem = ring > merge ? ring : merge;
@@ -789,7 +785,8 @@ template <class T, int G, int NT> cudaError_t launch(const Kv4AttnArgs& a, long 
     cfg.attrs = at;
     if (a.workspace) {
         constexpr int ctas = line_ctas<NT>();
-        cudaError_t e = allow_smem(kv4_line_kernel<T, G, NT>, smem);
+        static std::atomic<unsigned long long> allowed{0};
+        cudaError_t e = allow_shared_once(reinterpret_cast<const void*>(kv4_line_kernel<T, G, NT>), smem, allowed);
         if (e != cudaSuccess) return e;
         cfg.gridDim = dim3(ctas);
         cfg.dynamicSmemBytes = smem;
@@ -809,7 +806,8 @@ template <class T, int G, int NT> cudaError_t launch(const Kv4AttnArgs& a, long 
     // as many CTAs to a (request, head) as fill the GPU (4 to an SM), but at least two tiles to a warp
     int cluster = 1;
     while (cluster < MAX_CLUSTER && items * q_tiles * cluster < 4 * SMS && tiles >= 4 * W * cluster) cluster *= 2;
-    const cudaError_t e = allow_smem(kv4_few_kernel<T, G, NT>, smem);
+    static std::atomic<unsigned long long> allowed{0};
+    const cudaError_t e = allow_shared_once(reinterpret_cast<const void*>(kv4_few_kernel<T, G, NT>), smem, allowed);
     if (e != cudaSuccess) return e;
     cfg.gridDim = dim3(static_cast<unsigned>(items * cluster), static_cast<unsigned>(q_tiles < 65535 ? q_tiles : 65535));
     cfg.dynamicSmemBytes = smem;

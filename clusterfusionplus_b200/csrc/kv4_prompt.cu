@@ -594,7 +594,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
 
 template <class T, int G> cudaError_t launch(const Kv4AttnArgs& a, long long max_q_len, cudaStream_t st) {
     constexpr int DB = (32 * G + 63) / 64, smem = 1024 + 3 * DB * BLOCK + 4 * 32 * G * 128 + 2 * BLOCK;
-    const cudaError_t e = cudaFuncSetAttribute(kv4_prompt_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<unsigned long long> allowed{0};
+    const cudaError_t e = allow_shared_once(reinterpret_cast<const void*>(kv4_prompt_kernel<T, G>), smem, allowed);
     if (e != cudaSuccess) return e;
     const long long q_tiles = (max_q_len * (a.heads / a.kv_heads) + ROWS - 1) / ROWS;
     const dim3 grid(static_cast<unsigned>(a.batch * a.kv_heads), static_cast<unsigned>(q_tiles < 65535 ? q_tiles : 65535));

@@ -172,7 +172,8 @@ def kv4_read(cache, slot_map, head_dim: int, dtype=torch.float16) -> Tuple[torch
         raise RuntimeError(f"dtype: expected torch.float16 or torch.bfloat16, got {dtype}")
     tokens, head_dim = slot_map.numel(), int(head_dim)
     cp, pages, heads, page = _cache(cache, dev, -1, head_dim)
-    key, value = (torch.empty((tokens, heads, head_dim), dtype=dtype, device=cache.device) for _ in range(2))
+    shape, where = (tokens, heads, head_dim), cache.device
+    key, value = torch.empty(shape, dtype=dtype, device=where), torch.empty(shape, dtype=dtype, device=where)
     check(lib.cf_kv4_read(cp, pages, page, heads, head_dim, sp, tokens, key.data_ptr(), value.data_ptr(), _HALVES[dtype], _raw_stream(dev)))
     return key, value
 

@@ -294,12 +294,17 @@ def attention_case(lens, counts, heads, kv_heads, D, page, dtype, seed, extra_co
     return qkv[:, :heads], cache, table, starts
 
 
-@pytest.fixture(params=["by_size", "line"])
+@pytest.fixture(params=["by_size", "line", "prompt"])
 def schedule(request, monkeypatch):
-    """Both ways of dealing out the work: the one that the sizes choose (little work: clusters), and the line of tiles with a workspace."""
+    """All three ways of doing the work: the one that the sizes choose (little work: clusters), the line of tiles with a workspace, and 128 rows at a
+    time on the tensor cores, which a large hint asks for."""
+    import clusterfusionplus_b200 as cf
+    from clusterfusionplus_b200 import serving
     if request.param == "line":
-        from clusterfusionplus_b200 import serving
         monkeypatch.setattr(serving, "_attention_workspace", lambda *a: 64 << 20)
+    if request.param == "prompt":
+        plain = cf.kv4_attention
+        monkeypatch.setattr(cf, "kv4_attention", lambda *a, **k: plain(*a, **(k | {"max_q_len": 4096})))
 
 
 def check_attention(lens, counts, heads, kv_heads, D, page, dtype, seed=1, scale=None, max_q=None):
@@ -360,6 +365,13 @@ def test_attention_of_uneven_requests(cuda_device, schedule):
     check_attention([1, 5000, 16, 0, 17, 300, 1600, 1], [1, 1, 1, 1, 1, 1, 1, 0], 8, 4, 128, 16, torch.float16, seed=2)
     check_attention([64] * 40, [1] * 40, 4, 4, 64, 32, torch.bfloat16, seed=3)
     check_attention([7000, 3, 900], [2, 3, 1], 16, 2, 96, 48, torch.float16, seed=4)
+
+
+def test_attention_of_long_prompts(cuda_device):
+    """The tensor cores' way chosen by the sizes: several tiles of rows, ends off the tiles' borders, a length that the last tile does not fill."""
+    check_attention([700, 333], [700, 200], 8, 2, 128, 16, torch.bfloat16, seed=7)
+    check_attention([1100], [513], 4, 4, 80, 48, torch.float16, seed=8)
+    check_attention([260, 5, 0, 129], [129, 5, 0, 129], 16, 2, 64, 32, torch.float16, seed=9)
 
 
 def test_attention_chooses_the_line_by_itself(cuda_device):
@@ -585,7 +597,7 @@ def serving_state(B, H, Hkv, D, page, prompt, seed=1):
 
 
 @pytest.mark.parametrize("dtype,H,Hkv,D", [(torch.float16, 4, 4, 128), (torch.bfloat16, 8, 2, 80)])
-def test_serving_steps(cuda_device, dtype, H, Hkv, D):
+def test_serving_steps(cuda_device, schedule, dtype, H, Hkv, D):
     """Prompts, then single tokens, then a request that ends and one that takes its place, all through plan, append and attention, with log
     probabilities of what a head makes of the result; compared with dense attention over what was written."""
     import clusterfusionplus_b200 as cf
