@@ -11,9 +11,10 @@
 //    multiply-add by the group's scale.  The minima contribute sum_g m_g (sum of q over group g): one more matrix instruction, the
 //    query sums as two fp16 numbers each (hi + lo, 22 bits).  Scores are exact to fp32's rounding.
 //  - values: O^T = V^T P^T, again codes as the 16-row operand (two tokens in one word's halves, so no re-pairing).  P is rounded to
-//    fp16, transposed, and multiplied by the groups' scales two tokens at a time (a second rounding).  One more instruction takes the
+//    fp16, transposed, and multiplied by the groups' scales two tokens at a time, q = p s (a second rounding).  One more instruction takes the
 //    minima and a row of ones times the same P: sum p m of every group and the softmax's denominator, fp32 sums of the P that the
-//    numerators use.
+//    numerators use.  The codes are not centred, so the rounding of q would weigh up to 15 of its steps where the values spread
+//    over +-8: 8 (p s - q), which is exact in fp16, goes to the group's sum as well, and what is left of the error is q's times c - 8.
 // Queries are scaled by a power of two to at most 2^10 before they become fp16: exact for fp16 and bf16 inputs of any size
 // down to 2^-20 of their row's largest, off by less than 2^-30 of it below.  Probabilities are kept within (0, 4] (the running maximum is
 // two binary steps low) so that their product with a scale of up to 8734 (the widest fp16 range / 15) fits fp16 and small
@@ -106,6 +107,13 @@ template <int N> __device__ __forceinline__ void pair_halves(uint32_t (&x)[N], u
 
 __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
     const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// a b - ab, ab being the rounded product: exact.  A NaN becomes a number: the caller's zeros take it out of rows that it does not belong to.
+__device__ __forceinline__ uint32_t rest_half2(uint32_t a, uint32_t b, uint32_t ab) {
+    const __half2 y = __hmax2(__hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), __hneg2(*reinterpret_cast<const __half2*>(&ab))),
+                              __floats2half2_rn(-65504.f, -65504.f));
     return *reinterpret_cast<const uint32_t*>(&y);
 }
 
@@ -412,6 +420,9 @@ __device__ __forceinline__ void Acc<G, NT>::step(const int (&tile)[K], int token
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const uint32_t h0 = v0[g] >> 8, h1 = v1[g] >> 8, q0 = mul_half2(p0, sa[g]), q1 = mul_half2(p1, sb[g]);
+                // what the rounding left, 8 times of it to the group's row: the products see q (c - 8) then, half as large as q c
+                const uint32_t eight = g8 == g ? 0x48004800u : 0u;
+                mma_16816(low[nt], eight, 0u, eight, 0u, rest_half2(p0, sa[g], q0), rest_half2(p1, sb[g], q1));
                 mma_16816(o[nt][2 * g], v0[g] & 0x000f000fu, h0 & 0x000f000fu, v1[g] & 0x000f000fu, h1 & 0x000f000fu, q0, q1);
                 mma_16816(o[nt][2 * g + 1], v0[g] & 0x00f000f0u, h0 & 0x00f000f0u, v1[g] & 0x00f000f0u, h1 & 0x00f000f0u, q0, q1);
             }
