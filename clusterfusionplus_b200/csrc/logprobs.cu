@@ -198,7 +198,8 @@ struct __align__(16) Shared {
     unsigned long long bound;
     float part[LW][3];
     float stat[3];
-    int kept;
+    int kept, found;
+    uint16_t who[LT];
 };
 
 // For each of n <= LT / PARTS values: how many of the n are greater; PARTS neighbouring threads work on a value and all get the count
@@ -215,7 +216,7 @@ template <int PARTS> __device__ __forceinline__ int count_greater(const unsigned
 // that does not has k elements above it in the exact order too.
 template <class T> __device__ void block_top(const Walk<T>& w, unsigned long long best, int k, Shared& sh) {
     constexpr int E = Walk<T>::E;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x;
     sh.best[tid] = best;
     unsigned long long mine = best;
 #pragma unroll
@@ -224,7 +225,7 @@ template <class T> __device__ void block_top(const Walk<T>& w, unsigned long lon
         mine = x > mine ? x : mine;
     }
     if (tid % (LT / GROUPS) == 0) sh.group[tid / (LT / GROUPS)] = mine;
-    if (tid == 0) sh.kept = 0, sh.bound = 0;
+    if (tid == 0) sh.kept = sh.found = 0, sh.bound = 0;
     if (tid < MAX_TOP) sh.top[tid] = 0;
     __syncthreads();
     {   // groups without elements have 0 and share a count: with fewer than k others the bound stays 0 and everything is kept
@@ -240,22 +241,21 @@ template <class T> __device__ void block_top(const Walk<T>& w, unsigned long lon
             if (at < KEEP) sh.keep[at] = ranked(x, idx);
         }
     };
-    // the threads that reach the bound: each one's elements are dealt out to a warp
-    int nth = 0;
-    for (int i = 0; i < LW; ++i) {
-        const unsigned long long theirs = sh.best[i * 32 + lane];
-        unsigned who = __ballot_sync(0xffffffffu, theirs >= bound && theirs != 0);
-        for (; who; who &= who - 1) {
-            if (nth++ % LW != warp) continue;
-            const int o = i * 32 + __ffs(who) - 1, s = w.single(o);
-            if (s >= 0 && lane == 0) keep(to_float(w.row[s]), s, s);
-            for (int v = o + lane * LT; v < w.vecs; v += 32 * LT) {
-                const int at = w.vec_at(v);
-                const uint4 raw = __ldg(reinterpret_cast<const uint4*>(w.row + at));
-                const T* e = reinterpret_cast<const T*>(&raw);
+    // the threads that reach the bound, and their vectors (and singles, last), dealt out one by one to all threads
+    if (best != 0 && best >= bound) sh.who[atomicAdd(&sh.found, 1)] = static_cast<uint16_t>(tid);
+    __syncthreads();
+    const int per = (w.vecs + LT - 1) / LT + 1, all = sh.found * per;
+    for (int p = tid; p < all; p += LT) {
+        const int nth = p / per, j = p - nth * per, o = sh.who[nth], v = o + j * LT;
+        if (j == per - 1) {
+            const int s = w.single(o);
+            if (s >= 0) keep(to_float(w.row[s]), s, s);
+        } else if (v < w.vecs) {
+            const int at = w.vec_at(v);
+            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(w.row + at));
+            const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-                for (int j = 0; j < E; ++j) keep(to_float(e[j]), at + j, at);
-            }
+            for (int i = 0; i < E; ++i) keep(to_float(e[i]), at + i, at);
         }
     }
     __syncthreads();
