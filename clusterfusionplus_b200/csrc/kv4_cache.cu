@@ -10,6 +10,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/clusterfusion_b200.h"
 #include "host_common.h"
@@ -73,26 +74,27 @@ template <class T> __device__ __forceinline__ unsigned quantise8(const uint32_t 
     if (real && sf > 0.f && !bad) {
         // rint((v - m) / s) by the reciprocal: off by a few 2^-24 of at most 22, which matters only next to a half; there it is divided
         constexpr float MAGIC = 12582912.f;
-        float q[8], off = 0.f;
+        const bool wide = sizeof(T) == 2 && Two<T>::INF == 0x00800080u && (lo <= -65504.f || hi >= 65504.f);  // bf16 beyond fp16
+        float t[8], off = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float2 v = Two<T>::floats(p[i]);
-            if (sizeof(T) == 2 && Two<T>::INF == 0x00800080u) v.x = fminf(fmaxf(v.x, -65504.f), 65504.f), v.y = fminf(fmaxf(v.y, -65504.f), 65504.f);
-            q[2 * i] = (v.x - mf) * r;
-            q[2 * i + 1] = (v.y - mf) * r;
+            if (wide) v.x = fminf(fmaxf(v.x, -65504.f), 65504.f), v.y = fminf(fmaxf(v.y, -65504.f), 65504.f);
+            const float x = (v.x - mf) * r, y = (v.y - mf) * r;
+            t[2 * i] = x + MAGIC, t[2 * i + 1] = y + MAGIC;
+            off = fmaxf(off, fmaxf(fabsf(x - (t[2 * i] - MAGIC)), fabsf(y - (t[2 * i + 1] - MAGIC))));
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) off = fmaxf(off, fabsf(q[i] - ((q[i] + MAGIC) - MAGIC)));
         if (off > 0.49999f) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float2 v = Two<T>::floats(p[i]);
-                q[2 * i] = (fminf(fmaxf(v.x, -65504.f), 65504.f) - mf) / sf;
-                q[2 * i + 1] = (fminf(fmaxf(v.y, -65504.f), 65504.f) - mf) / sf;
+                t[2 * i] = (fminf(fmaxf(v.x, -65504.f), 65504.f) - mf) / sf + MAGIC;
+                t[2 * i + 1] = (fminf(fmaxf(v.y, -65504.f), 65504.f) - mf) / sf + MAGIC;
             }
         }
+        // (no value is more than half a step below the minimum; a scale that was rounded down to one of fp16's last steps reaches beyond 15)
 #pragma unroll
-        for (int i = 7; i >= 0; --i) codes = codes * 16 + __float_as_uint(fminf(fmaxf(q[i], 0.f), 15.f) + MAGIC);
+        for (int i = 7; i >= 0; --i) codes = codes * 16 + __float_as_uint(fminf(t[i], MAGIC + 15.f));
         codes -= 0x4b400000u * 0x11111111u;
     }
     *scale = bad ? __ushort_as_half(0x7fff) : s;
@@ -106,11 +108,11 @@ __device__ __forceinline__ long long tile_of(int slot, int head, int heads, int 
     return (static_cast<long long>(page) * heads + head) * tiles_a_page + (tile - page * tiles_a_page);
 }
 
-template <class T>
+template <class T, int G>
 __global__ void __launch_bounds__(CT) kv4_append_kernel(const T* __restrict__ key, const T* __restrict__ value, const int* __restrict__ slot_map,
                                                         uint8_t* __restrict__ cache, unsigned items, int heads, int D, int tiles_a_page, long long slots,
                                                         long long k_ts, long long k_hs, long long v_ts, long long v_hs) {
-    const int G = kv4_groups(D), l = threadIdx.x & 15;
+    const int l = threadIdx.x & 15;
     const unsigned item = blockIdx.x * ITEMS + threadIdx.x / 16;
     const bool there = item < items;
     const unsigned tok = there ? item / heads : 0;
@@ -176,10 +178,10 @@ template <> __device__ __forceinline__ uint4 unpack8<__nv_bfloat16>(unsigned cod
     return *reinterpret_cast<const uint4*>(e);
 }
 
-template <class T>
+template <class T, int G>
 __global__ void __launch_bounds__(CT) kv4_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ slot_map, T* __restrict__ key,
                                                       T* __restrict__ value, unsigned items, int heads, int D, int tiles_a_page, long long slots) {
-    const int G = kv4_groups(D), l = threadIdx.x & 15, dim = 8 * l;
+    const int l = threadIdx.x & 15, dim = 8 * l;
     const unsigned item = blockIdx.x * ITEMS + threadIdx.x / 16;
     if (item >= items || dim >= D) return;
     const unsigned tok = item / heads;
@@ -208,6 +210,15 @@ int check_cache(int64_t pages, int64_t kv_heads, int64_t page, int64_t D) {
     if (pages < 1 || kv_heads < 1 || kv_heads > 1024 || pages > 0x7fffffff / page)
         return cf_host_fail(CF_ERR_INVALID, "cache of %lld pages of %lld rows, %lld heads (at most 2^31 - 1 rows)", (long long)pages, (long long)page, (long long)kv_heads);
     return CF_OK;
+}
+
+template <class F> void with_groups(int D, F f) {
+    switch (kv4_groups(D)) {
+        case 1: return f(std::integral_constant<int, 1>());
+        case 2: return f(std::integral_constant<int, 2>());
+        case 3: return f(std::integral_constant<int, 3>());
+        default: return f(std::integral_constant<int, 4>());
+    }
 }
 
 int check_launch(const char* what) {
@@ -261,8 +272,10 @@ int cf_kv4_append(const void* key, const void* value, int dtype, int64_t tokens,
             k, static_cast<decltype(k)>(value), slot_map, static_cast<uint8_t*>(cache), static_cast<unsigned>(items), static_cast<int>(kv_heads), static_cast<int>(head_dim),
             static_cast<int>(page_size / KV4_TILE), pages * page_size, key_token_stride, key_head_stride, value_token_stride, value_head_stride);
     };
-    if (dtype == CF_DTYPE_FP16) go(static_cast<const __half*>(key), kv4_append_kernel<__half>);
-    else go(static_cast<const __nv_bfloat16*>(key), kv4_append_kernel<__nv_bfloat16>);
+    with_groups(static_cast<int>(head_dim), [&](auto g) {
+        if (dtype == CF_DTYPE_FP16) go(static_cast<const __half*>(key), kv4_append_kernel<__half, g.value>);
+        else go(static_cast<const __nv_bfloat16*>(key), kv4_append_kernel<__nv_bfloat16, g.value>);
+    });
     return check_launch("4-bit append");
 }
 
@@ -281,8 +294,10 @@ int cf_kv4_read(const void* cache, int64_t pages, int64_t page_size, int64_t kv_
             static_cast<const uint8_t*>(cache), slot_map, k, static_cast<decltype(k)>(value), static_cast<unsigned>(items), static_cast<int>(kv_heads), static_cast<int>(head_dim),
             static_cast<int>(page_size / KV4_TILE), pages * page_size);
     };
-    if (dtype == CF_DTYPE_FP16) go(static_cast<__half*>(key), kv4_read_kernel<__half>);
-    else go(static_cast<__nv_bfloat16*>(key), kv4_read_kernel<__nv_bfloat16>);
+    with_groups(static_cast<int>(head_dim), [&](auto g) {
+        if (dtype == CF_DTYPE_FP16) go(static_cast<__half*>(key), kv4_read_kernel<__half, g.value>);
+        else go(static_cast<__nv_bfloat16*>(key), kv4_read_kernel<__nv_bfloat16, g.value>);
+    });
     return check_launch("4-bit read");
 }
 
