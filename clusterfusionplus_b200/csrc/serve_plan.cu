@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(PT) paged_kv_plan_kernel(const PlanArgs a) {
     int* s_tok = s_cached + a.batch;           // [batch + 1] first token of a request
     int* s_row = s_tok + a.batch + 1;          // [batch + 1] first row
     int* s_page = s_row + a.batch + 1;         // [batch + 1] first fresh page
+    int* s_have = s_page + a.batch + 1;        // [batch] pages held already
     __shared__ Sums buf[PT / 32];
     __shared__ int s_bits;
 
@@ -132,7 +133,8 @@ __global__ void __launch_bounds__(PT) paged_kv_plan_kernel(const PlanArgs a) {
             s_tok[b] = static_cast<int>(at.tokens);
             s_row[b] = static_cast<int>(at.rows);
             s_page[b] = static_cast<int>(at.pages);
-            at = at + Sums{n, static_cast<long long>(c) + n, pages_of(static_cast<long long>(c) + n, a.page) - pages_of(c, a.page)};
+            s_have[b] = pages_of(c, a.page);
+            at = at + Sums{n, static_cast<long long>(c) + n, pages_of(static_cast<long long>(c) + n, a.page) - s_have[b]};
         }
         if (tid == 0) {
             s_tok[a.batch] = static_cast<int>(all.tokens);
@@ -154,14 +156,15 @@ __global__ void __launch_bounds__(PT) paged_kv_plan_kernel(const PlanArgs a) {
         if (ok)
             for (int e = tid; e < s_page[a.batch]; e += PT) {
                 const int b = owner_of(s_page, a.batch, e);
-                a.table[b * a.table_stride + pages_of(s_cached[b], a.page) + (e - s_page[b])] = a.free_pages[avail - 1 - e];
+                a.table[b * a.table_stride + s_have[b] + (e - s_page[b])] = a.free_pages[avail - 1 - e];
             }
     }
-    // slot of position pos of request b: a held page from the table, a fresh one from where this step takes it
-    auto slot_of = [&](int b, int pos) -> int {
-        const int col = pos / a.page, have = pages_of(s_cached[b], a.page);
-        const long long held = col < have ? a.table[b * a.table_stride + col] : a.free_pages[avail - 1 - (s_page[b] + col - have)];
-        const long long slot = held * a.page + pos % a.page;
+    // page of column col of request b: held pages come from the table, fresh ones from where this step takes them
+    auto page_of = [&](int b, int col) -> long long {
+        return col < s_have[b] ? a.table[b * a.table_stride + col] : a.free_pages[avail - 1 - (s_page[b] + col - s_have[b])];
+    };
+    auto slot_at = [&](long long held, int in) -> int {
+        const long long slot = held * a.page + in;
         return held < 0 || slot > 0x7fffffffll ? -1 : static_cast<int>(slot);
     };
     const long long stride = static_cast<long long>(gridDim.x) * PT;
@@ -171,7 +174,8 @@ __global__ void __launch_bounds__(PT) paged_kv_plan_kernel(const PlanArgs a) {
         if (ok && j < all.tokens) {
             const int b = owner_of(s_tok, a.batch, static_cast<int>(j));
             pos = s_cached[b] + (j - s_tok[b]);
-            slot = slot_of(b, static_cast<int>(pos));
+            const int col = static_cast<int>(pos) / a.page;
+            slot = slot_at(page_of(b, col), static_cast<int>(pos) - col * a.page);
         }
         a.positions[j] = pos;
         a.slot_map[j] = slot;
@@ -180,15 +184,26 @@ __global__ void __launch_bounds__(PT) paged_kv_plan_kernel(const PlanArgs a) {
     for (long long g = static_cast<long long>(blockIdx.x) * PT + tid; g < groups; g += stride) {
         const long long j0 = g * ROWS_PER_THREAD;
         int slot[ROWS_PER_THREAD];
-        int b = -1;
+        int b = -1, left = 0, in = 0, col = 0;  // request; its rows from here on; place in the page; column
+        long long held = 0;
 #pragma unroll
         for (int i = 0; i < ROWS_PER_THREAD; ++i) {
             slot[i] = -1;
             if (ok && j0 + i < all.rows) {
                 const int j = static_cast<int>(j0) + i;
-                if (b < 0) b = owner_of(s_row, a.batch, j);
-                while (j >= s_row[b + 1]) ++b;
-                slot[i] = slot_of(b, j - s_row[b]);
+                if (left == 0) {  // the first row, or the first of the next request that has any
+                    if (b < 0) b = owner_of(s_row, a.batch, j);
+                    while (j >= s_row[b + 1]) ++b;
+                    left = s_row[b + 1] - j;
+                    const int pos = j - s_row[b];
+                    col = pos / a.page, in = pos - col * a.page;
+                    held = page_of(b, col);
+                } else if (in == a.page) {
+                    in = 0;
+                    held = page_of(b, ++col);
+                }
+                slot[i] = slot_at(held, in++);
+                --left;
             }
         }
         if (j0 + ROWS_PER_THREAD <= a.max_rows) {
@@ -298,7 +313,7 @@ int cf_paged_kv_plan(const int* cached_lens, const int* new_lens, int64_t batch,
     // a CTA for 256 tokens or 1024 rows, at most four for each SM: more would only repeat the scan
     const int64_t want = max_tokens / PT + max_rows / (PT * ROWS_PER_THREAD) + 1;
     const unsigned grid = static_cast<unsigned>(want < 4 * 148 ? want : 4 * 148);
-    const size_t smem = (4 * batch + 3) * sizeof(int);
+    const size_t smem = (5 * batch + 3) * sizeof(int);
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(paged_kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (e != cudaSuccess) return cf_host_fail(CF_ERR_CUDA, "paged plan: %s", cudaGetErrorString(e));
