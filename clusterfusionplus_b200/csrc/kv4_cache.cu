@@ -8,6 +8,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -328,6 +330,11 @@ int cf_kv4_attention(const void* query, int dtype, int64_t rows, int64_t heads, 
     const bool prompt = prompt_sized(batch, heads, kv_heads, table_width * page_size, max_q_len);
     if (workspace && !prompt && (workspace_bytes < needed || !aligned(workspace, 16)))
         return cf_host_fail(CF_ERR_INVALID, "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)needed);
+    // rows of one request, and its heads, are written while others are still read
+    const int64_t to_row = (rows - 1) * query_token_stride, to_head = (heads - 1) * query_head_stride;
+    const char *q_from = static_cast<const char*>(query) + 2 * (std::min<int64_t>(to_row, 0) + std::min<int64_t>(to_head, 0));
+    const char *q_to = static_cast<const char*>(query) + 2 * (std::max<int64_t>(to_row, 0) + std::max<int64_t>(to_head, 0) + head_dim), *o_from = static_cast<const char*>(out);
+    if (o_from < q_to && q_from < o_from + 2 * rows * heads * head_dim) return cf_host_fail(CF_ERR_INVALID, "out overlaps the queries");
     static std::atomic<int*> status_word[64];  // address of the device status word, by device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);

@@ -460,8 +460,8 @@ int cf_kv4_read(const void* cache, int64_t pages, int64_t page_size, int64_t kv_
                 int64_t tokens, void* key, void* value, int dtype, void* stream);
 
 /* Causal attention over that cache.  query [rows][heads][head_dim] (fp16 or bf16; strides in elements, multiples of 8, last
- * axis contiguous), out [rows][heads][head_dim] contiguous, heads a multiple of kv_heads (query head h reads cached head
- * h / (heads / kv_heads)).  Request b owns query rows qo_indptr[b] .. qo_indptr[b + 1) (int32 [batch + 1], ascending; NULL: row
+ * axis contiguous), out [rows][heads][head_dim] contiguous and apart from the queries, heads a multiple of kv_heads
+ * (query head h reads cached head h / (heads / kv_heads)).  Request b owns query rows qo_indptr[b] .. qo_indptr[b + 1) (int32 [batch + 1], ascending; NULL: row
  * b); they are its last tokens: of n queries and kv_lens[b] cached tokens, query i sees the first kv_lens[b] - n + i + 1
  * tokens, which lie in the pages block_table[b][0 ..].  A query that sees no token gives zeros.  Rows of out that no
  * request owns stay as they are.  A page number outside the cache is skipped as if its tokens were not there, and recorded
