@@ -139,6 +139,24 @@ def _load():
 lib = _load()
 
 
+def serving_binding():
+    """The extension module of the serving calls (csrc/serving_binding.cpp), bound to the library loaded above."""
+    import importlib.util
+
+    import torch
+    path = os.path.join(_HERE, "lib", "_serving.so")
+    if not os.path.exists(path):
+        raise ImportError(f"{path} is missing: build it with `python clusterfusionplus_b200/build.py`. There is no fallback implementation.")
+    spec = importlib.util.spec_from_file_location("_serving", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    if mod.torch_version != torch.__version__.split("+")[0]:
+        raise ImportError(f"{path} was built for torch {mod.torch_version}, this is {torch.__version__}: run `python clusterfusionplus_b200/build.py --force`")
+    mod.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
+        "cf_last_error", "cf_paged_kv_plan", "cf_paged_kv_release", "cf_kv4_append", "cf_kv4_read", "cf_kv4_attention", "cf_kv4_attention_workspace", "cf_token_logprobs")))
+    return mod
+
+
 def last_error() -> str:
     msg = lib.cf_last_error()
     return msg.decode() if msg else ""

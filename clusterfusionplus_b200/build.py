@@ -7,7 +7,8 @@ shared library: the decode kernel with the C ABI, the batched Llama decode block
 tcgen05 skinny GEMMs + paged attention), the elementwise kernels of the prompt pass, the plan of a step over a
 paged cache, the cache held in 4 bits, the log probabilities of tokens, and the tensor-core prefill GEMM, which is built from the CUTLASS / CuTe headers found in the Python environment (the `flashinfer` wheel
 vendors them; set CUTLASS_INCLUDE to use another copy).  The library has no torch dependency;
-it links the CUDA runtime statically and finds the driver's tensor-map encoder at run time.
+it links the CUDA runtime statically and finds the driver's tensor-map encoder at run time.  Beside it, lib/_serving.so binds
+the serving calls to Python (g++, torch's C++ headers).
 """
 from __future__ import annotations
 
@@ -16,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -36,6 +38,8 @@ UNITS = {
     "kv4_prompt.cu": (["f32x2.cuh", "kv4_layout.cuh", "kv4_attention.h", "mma.cuh", "pipeline.cuh"], False),
     "logprobs.cu": (["f32x2.cuh", "host_common.h", HEADER], False),
 }
+BINDING = os.path.join(CSRC, "serving_binding.cpp")
+BINDING_OUT = os.path.join(HERE, "lib", "_serving.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -93,8 +97,22 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _bind(verbose: bool) -> None:
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc_path())))
+    dirs = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    # the compiler that nvcc takes too: one that links libstdc++ statically would put a second copy next to torch's
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", *(x for d in dirs for x in ("-isystem", d)), "-o", BINDING_OUT, BINDING,
+           "-L" + os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed on serving_binding.cpp")
+
+
 def up_to_date() -> bool:
-    return not _stale(OUT, [d for s in UNITS for d in _deps(s)])
+    return not _stale(OUT, [d for s in UNITS for d in _deps(s)]) and not _stale(BINDING_OUT, [BINDING, HEADER])
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -102,8 +120,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return OUT
     os.makedirs(OBJ, exist_ok=True)
     todo = [s for s in UNITS if force or _stale(os.path.join(OBJ, s.replace(".cu", ".o")), _deps(s))]
-    with ThreadPoolExecutor(max_workers=len(UNITS)) as ex:
+    with ThreadPoolExecutor(max_workers=len(UNITS) + 1) as ex:
+        binding = ex.submit(_bind, verbose) if force or _stale(BINDING_OUT, [BINDING, HEADER]) else None
         list(ex.map(lambda s: _compile(s, verbose), todo))
+        if binding:
+            binding.result()
     objs = [os.path.join(OBJ, s.replace(".cu", ".o")) for s in UNITS]
     r = subprocess.run([nvcc_path(), *ARCH, "-shared", "-o", OUT, *objs], capture_output=True, text=True)
     if r.returncode != 0:

@@ -67,6 +67,15 @@ def test_attention_refusals(kw, match):
     refused("cf_kv4_attention", list((a | kw).values()), match)
 
 
+@pytest.mark.parametrize("at", [0, 256 * 7, 2 * 1024 * 2 + 2 * 1024 - 16])
+@pytest.mark.parametrize("first", ["query", "out"])
+def test_attention_refuses_an_output_over_the_queries(at, first):
+    """3 rows of 8 heads of 128: 6144 bytes each; the other tensor starts inside the first."""
+    base, shifted = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + at)
+    q, o = (base, shifted) if first == "query" else (shifted, base)
+    refused("cf_kv4_attention", [q, 0, 3, 8, 128, 1024, 128, ONE, 4, 16, 4, ONE, 8, 8, ONE, ONE, 4, 1, 0.1, None, 0, o, None], "overlaps")
+
+
 @pytest.mark.parametrize("kw,match", [
     (dict(dtype=3), "dtype"), (dict(rows=-1), "rows"), (dict(vocab=0), "vocabulary"), (dict(top=33), "top_k"), (dict(top=-1), "top_k"), (dict(vocab=4), "top_k"), (dict(bytes=2), "tokens"),
     (dict(logits=None), "null"), (dict(tops=None), "null"), (dict(logits=ctypes.c_void_p(4097)), "aligned")])
@@ -98,6 +107,18 @@ def test_cpu_tensors_are_rejected():
     with pytest.raises(RuntimeError, match="multiple of"):
         cf.kv4_cache(2, 2, 24, 128, device="cpu")
     assert cf.kv4_cache(2, 3, 32, 80, device="cpu").shape == (2, 3, 32, 120)
+
+
+def test_binding_reports_what_is_wrong():
+    """The compiled checks: messages with numbers and shapes in them arrive as Python exceptions."""
+    from clusterfusionplus_b200 import serving
+    x, i = torch.zeros(2, 2, 64, dtype=torch.float16), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="kv4_attention: 9 arguments, got 2"):
+        serving._call.attention(x, i)
+    with pytest.raises(RuntimeError, match="key: expected a torch.Tensor"):
+        serving.kv4_append(None, x, i, x)
+    with pytest.raises(RuntimeError, match="logits: expected a CUDA tensor, got cpu"):
+        serving.token_logprobs(x[0], i)
 
 
 # ------------------------------------------------------------------------------------------------------------- oracle

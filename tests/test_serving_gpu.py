@@ -14,6 +14,7 @@ Tolerances.  u = finfo(dtype).eps / 2 is the relative error of a rounding.
  - log probabilities: x - m and its product with log2(e) round three times in fp32, ex2 is good to 2^-22, a sum over n terms adds in runs of at most
    n / 512 terms and trees: (n / 512 + 24) 2^-24 + 2^-22 relative on z and w; so 2 (n / 512 + 24 + 4) 2^-24 times max(1, |log p|, entropy's terms <= 12)."""
 import math
+import os
 import random
 
 import numpy as np
@@ -301,7 +302,7 @@ def schedule(request, monkeypatch):
     import clusterfusionplus_b200 as cf
     from clusterfusionplus_b200 import serving
     if request.param == "line":
-        monkeypatch.setattr(serving, "_attention_workspace", lambda *a: 64 << 20)
+        monkeypatch.setattr(serving, "_workspace", 64 << 20)
     if request.param == "prompt":
         plain = cf.kv4_attention
         monkeypatch.setattr(cf, "kv4_attention", lambda *a, **k: plain(*a, **(k | {"max_q_len": 4096})))
@@ -375,8 +376,8 @@ def test_attention_of_long_prompts(cuda_device):
 
 
 def test_attention_chooses_the_line_by_itself(cuda_device):
-    from clusterfusionplus_b200 import serving
-    assert serving._attention_workspace(2, 8, 8, 128, 16384, 1) > 0 and serving._attention_workspace(1, 8, 8, 128, 1024, 1) == 0
+    from clusterfusionplus_b200._lib import lib
+    assert lib.cf_kv4_attention_workspace(2, 8, 8, 128, 16384, 1) > 0 and lib.cf_kv4_attention_workspace(1, 8, 8, 128, 1024, 1) == 0
     check_attention([16000, 9000], [1, 1], 8, 8, 128, 64, torch.float16, seed=6)
 
 
@@ -701,6 +702,98 @@ def test_serving_step_captured_and_replayed(cuda_device):
         want = run_eager(seed, steps)
         got = (p.kv_lens, p.slot_map, p.kv_indices, out, lp.logprobs, lp.entropy, lp.top_tokens, s["table"], s["cache"])
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_calls_on_two_streams_do_not_disturb_each_other(cuda_device, schedule):
+    import clusterfusionplus_b200 as cf
+    cases = []
+    for seed, lens in ((1, [5000, 40, 700]), (2, [90, 6000, 1])):
+        q, cache, table, starts = attention_case(lens, [1, 3, 1], 8, 2, 128, 16, torch.float16, seed)
+        cases.append((q, cache, ints(table), ints(lens), ints(starts)))
+    want = [cf.kv4_attention(*c, max_q_len=3) for c in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(50):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(cf.kv4_attention(*cases[i], max_q_len=3))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in (0, 1) for x in got[i])
+
+
+def test_first_calls_of_a_process_inside_a_capture(cuda_device):
+    """Nothing that a first call sets up (kernel attributes, addresses) is forbidden while a stream is captured."""
+    import subprocess
+    import sys
+    code = """
+import torch
+import clusterfusionplus_b200 as cf
+dev = torch.device("cuda:0")
+i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)
+cached, new, free, count, table = i32(200, 3), i32(1, 1), torch.arange(40, dtype=torch.int32, device=dev), i32(10), torch.zeros(2, 16, dtype=torch.int32, device=dev)
+table[0] = torch.arange(40, 56, device=dev)
+table[1] = torch.arange(56, 72, device=dev)
+cache, x = cf.kv4_cache(72, 2, 16, 64), torch.ones(2, 12, 64, dtype=torch.float16, device=dev)
+many, starts, logits = torch.ones(140, 8, 64, dtype=torch.float16, device=dev), i32(0, 139, 140), torch.zeros(2, 50304, device=dev)
+big, wide = cf.kv4_cache(72, 8, 1024, 64), torch.ones(2, 8, 64, dtype=torch.float16, device=dev)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    p = cf.paged_kv_plan(cached, new, table, free, count, 16, 2, 300)
+    cf.kv4_append(x[:, 8:10], x[:, 10:], p.slot_map, cache)
+    k, v = cf.kv4_read(cache, p.slot_map, 64)
+    a = cf.kv4_attention(x[:, :8], cache, table, p.kv_lens)
+    b = cf.kv4_attention(many, cache, table, p.kv_lens, starts, max_q_len=139)
+    c = cf.kv4_attention(wide, big, table, p.kv_lens)
+    s = cf.token_logprobs(logits, new, 3)
+    left, status = cf.paged_kv_release(new, p.kv_lens, table, free, p.free_count, 16)
+g.replay()  # once: its last call gives the pages back
+torch.cuda.synchronize()
+assert bool((k == 1).all()) and bool((v == 1).all()) and int(status) == 0, (k, v, status)
+assert abs(float(s.entropy[0]) - 10.82584) < 1e-4, s.entropy
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
+def test_attention_of_shared_pages(cuda_device, schedule):
+    """Requests with a common prefix name the same pages."""
+    import clusterfusionplus_b200 as cf
+    q, cache, table, starts = attention_case([300, 300], [1, 1], 8, 2, 64, 16, torch.float16, 12)
+    shared = [table[0], table[0][:10] + table[1][10:]]
+    K, V = S.unpack(cache.cpu().numpy(), 64)
+    out = cf.kv4_attention(q, cache, ints(shared), ints([300, 290]), ints(starts))
+    close(out, S.attention(q, K, V, shared, [300, 290], starts, 64 ** -0.5), q, K, V, 64 ** -0.5)
+
+
+def test_offsets_beyond_32_bits(cuda_device):
+    """Rows of queries, keys and logits that lie more than 2^31 elements apart."""
+    import clusterfusionplus_b200 as cf
+    apart = 1 << 30
+    room = torch.empty(2 * apart + 60000, dtype=torch.float16, device=DEV)
+    q, cache, table, starts = attention_case([300, 20, 77], [1, 1, 1], 8, 2, 64, 16, torch.float16, 13)
+    far = room.as_strided((3, 8, 64), (apart, 64, 1))
+    far.copy_(q)
+    n = ints([300, 20, 77])
+    assert torch.equal(cf.kv4_attention(far, cache, ints(table), n), cf.kv4_attention(q, cache, ints(table), n))
+    one, two = cache.clone(), cache.clone()
+    cf.kv4_append(far[:, :2], far[:, 2:4], ints([5, 6, 7]), one)
+    cf.kv4_append(q[:, :2], q[:, 2:4], ints([5, 6, 7]), two)
+    assert torch.equal(one, two)
+    x = logits(3, 50301, torch.float16, 5)
+    far = room.as_strided((3, 50301), (apart, 1))
+    far.copy_(x)
+    check_logprobs(far, [1, 2, 50300], 5)  # to 64-bit numbers: where a row starts within 16 bytes decides the order of its sums
+
+
+def test_results_carry_no_gradient(cuda_device):
+    import clusterfusionplus_b200 as cf
+    x = logits(2, 100, torch.float32, 3).requires_grad_()
+    assert not any(t.requires_grad for t in cf.token_logprobs(x, ints([1, 2]), 2))
+    with torch.inference_mode():
+        assert torch.equal(cf.token_logprobs(x, ints([1, 2]), 2).logprobs, cf.token_logprobs(x.detach(), ints([1, 2]), 2).logprobs)
 
 
 def test_results_are_the_same_every_time(cuda_device):
