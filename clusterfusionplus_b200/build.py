@@ -33,7 +33,7 @@ UNITS = {
     "prefill_gemm.cu": (["prefill_gemm.h"], True),
     "prefill_ops.cu": (["host_common.h", HEADER], False),
     "serve_plan.cu": (["host_common.h", HEADER], False),
-    "kv4_cache.cu": (["kv4_layout.cuh", "kv4_attention.h", "host_common.h", HEADER], False),
+    "kv4_cache.cu": (["f32x2.cuh", "kv4_layout.cuh", "kv4_attention.h", "host_common.h", HEADER], False),
     "kv4_decode.cu": (["kv4_layout.cuh", "kv4_attention.h", "mma.cuh"], False),
     "kv4_prompt.cu": (["f32x2.cuh", "kv4_layout.cuh", "kv4_attention.h", "mma.cuh", "pipeline.cuh"], False),
     "logprobs.cu": (["f32x2.cuh", "host_common.h", HEADER], False),

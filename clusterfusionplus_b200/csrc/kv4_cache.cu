@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "../../include/clusterfusion_b200.h"
+#include "f32x2.cuh"
 #include "host_common.h"
 #include "kv4_attention.h"
 #include "kv4_layout.cuh"
@@ -38,37 +39,58 @@ constexpr int ITEMS = CT / 16;   // (token, head) pairs of a CTA
 template <class T> struct Two;
 template <> struct Two<__half> {
     using P = __half2;
+    static constexpr bool BEYOND = false;         // whether finite numbers reach beyond fp16
     static constexpr uint32_t INF = 0x04000400u;  // what carries an exponent of all ones into bit 15
+    static constexpr uint32_t LEAST = 0xfbfffbffu;
     static __device__ __forceinline__ float2 floats(P v) { return __half22float2(v); }
 };
 template <> struct Two<__nv_bfloat16> {
     using P = __nv_bfloat162;
-    static constexpr uint32_t INF = 0x00800080u;
+    static constexpr bool BEYOND = true;
+    static constexpr uint32_t INF = 0x00800080u, LEAST = 0xff7fff7fu;
     static __device__ __forceinline__ float2 floats(P v) { return __bfloat1622float2(v); }
 };
+template <class P> __device__ __forceinline__ uint32_t bits_of(P v) { return *reinterpret_cast<const uint32_t*>(&v); }
+template <class P> __device__ __forceinline__ P pair_of(uint32_t w) { return *reinterpret_cast<const P*>(&w); }
 
-// Codes of this lane's eight values (raw words, nibble i: value i), scale and minimum of its group of four lanes.  Extremes and the test
-// for NaN and infinities work on the 16-bit pairs; codes are rounded by adding 1.5 * 2^23, which leaves them in the low mantissa
-// bits (conversions run at a quarter of the rate), and put together by multiply-adds.
+// n / d for n < 2^31 by a multiplication: with 2^(l - 1) < d <= 2^l, (n (floor(2^(31 + l) / d) + 1)) >> (31 + l) is exact
+struct Divisor {
+    unsigned times, shift;
+    explicit Divisor(unsigned d) {
+        unsigned l = 0;
+        while ((1ull << l) < d) ++l;
+        times = static_cast<unsigned>((1ull << (31 + l)) / d + 1);
+        shift = 31 + l;
+    }
+    __device__ __forceinline__ unsigned operator()(unsigned n) const { return static_cast<unsigned>((static_cast<unsigned long long>(n) * times) >> shift); }
+};
+
+// Codes of this lane's eight values (raw words, nibble i: value i), scale and minimum of its group of four lanes.  Extremes stay in the 16-bit
+// type, the greatest value and the greatest negated one as a pair, and carry a NaN or an infinity along.  A code is rounded by adding
+// 1.5 * 2^23 and taking it off (conversions run at a quarter of the rate); four codes are put together as one fp32 number below 2^16.
 template <class T> __device__ __forceinline__ unsigned quantise8(const uint32_t (&raw)[4], bool real, __half* scale, __half* low) {
     using P = typename Two<T>::P;
-    const P* p = reinterpret_cast<const P*>(raw);
-    const float2 hi2 = Two<T>::floats(__hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]))), lo2 = Two<T>::floats(__hmin2(__hmin2(p[0], p[1]), __hmin2(p[2], p[3])));
-    float hi = real ? fminf(fmaxf(hi2.x, hi2.y), 65504.f) : -65504.f, lo = real ? fmaxf(fminf(lo2.x, lo2.y), -65504.f) : 65504.f;
-    uint32_t over = 0;
+    auto p = [&](int i) { return pair_of<P>(raw[i]); };
+    const uint32_t hi2 = bits_of(__hmax2_nan(__hmax2_nan(p(0), p(1)), __hmax2_nan(p(2), p(3))));
+    const uint32_t lo2 = bits_of(__hmin2_nan(__hmin2_nan(p(0), p(1)), __hmin2_nan(p(2), p(3)))) ^ 0x80008000u;
+    uint32_t ends = bits_of(__hmax2_nan(pair_of<P>(__byte_perm(hi2, lo2, 0x5410)), pair_of<P>(__byte_perm(hi2, lo2, 0x7632))));
+    if (!real) ends = Two<T>::LEAST;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) over |= (raw[i] & 0x7fff7fffu) + Two<T>::INF;
-    unsigned bad = real && (over & 0x80008000u);
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+    for (int o = 1; o < 4; o <<= 1) ends = bits_of(__hmax2_nan(pair_of<P>(ends), pair_of<P>(__shfl_xor_sync(0xffffffffu, ends, o))));
+    const bool bad = ((ends & 0x7fff7fffu) + Two<T>::INF) & 0x80008000u;
+    float2 end = Two<T>::floats(pair_of<P>(ends));
+    end.y = -end.y;
+    bool wide = false;
+    if constexpr (Two<T>::BEYOND) {
+        wide = end.y < -65504.f || end.x > 65504.f;
+        end.x = fminf(fmaxf(end.x, -65504.f), 65504.f), end.y = fminf(fmaxf(end.y, -65504.f), 65504.f);
     }
-    lo = fminf(lo, 65504.f), hi = fmaxf(hi, -65504.f);  // bf16 beyond fp16 on one side only
-    const __half m = __float2half_rn(lo);
+    const __half m = __float2half_rn(end.y);
     const float mf = __half2float(m);
-    const __half s = __float2half_rn((hi - mf) / 15.f);
+    // x / 15 correctly rounded: the product with the rounded 1 / 15, corrected by its residual, which is exact in a fused multiply-add (where
+    // that would fall below fp32's range the quotient is far below fp16's)
+    const float x15 = end.x - mf, near = x15 * (1.f / 15.f);
+    const __half s = __float2half_rn(fmaf(fmaf(-15.f, near, x15), 1.f / 15.f, near));
     const float sf = __half2float(s);
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(sf));
@@ -76,28 +98,37 @@ template <class T> __device__ __forceinline__ unsigned quantise8(const uint32_t 
     if (real && sf > 0.f && !bad) {
         // rint((v - m) / s) by the reciprocal: off by a few 2^-24 of at most 22, which matters only next to a half; there it is divided
         constexpr float MAGIC = 12582912.f;
-        const bool wide = sizeof(T) == 2 && Two<T>::INF == 0x00800080u && (lo <= -65504.f || hi >= 65504.f);  // bf16 beyond fp16
-        float t[8], off = 0.f;
+        const Pair magic(MAGIC, MAGIC), less(-MAGIC, -MAGIC), lowest(-mf, -mf), times(r, r), minus(-1.f, -1.f);
+        Pair c[4];
+        float off = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float2 v = Two<T>::floats(p[i]);
-            if (wide) v.x = fminf(fmaxf(v.x, -65504.f), 65504.f), v.y = fminf(fmaxf(v.y, -65504.f), 65504.f);
-            const float x = (v.x - mf) * r, y = (v.y - mf) * r;
-            t[2 * i] = x + MAGIC, t[2 * i + 1] = y + MAGIC;
-            off = fmaxf(off, fmaxf(fabsf(x - (t[2 * i] - MAGIC)), fabsf(y - (t[2 * i + 1] - MAGIC))));
+            float2 v = Two<T>::floats(p(i));
+            if (Two<T>::BEYOND && wide) v.x = fminf(fmaxf(v.x, -65504.f), 65504.f), v.y = fminf(fmaxf(v.y, -65504.f), 65504.f);
+            const Pair x = (Pair(v.x, v.y) + lowest) * times;
+            c[i] = (x + magic) + less;
+            const float2 e = fma2(c[i], minus, x).both();
+            off = fmaxf(off, fmaxf(fabsf(e.x), fabsf(e.y)));
         }
         if (off > 0.49999f) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float2 v = Two<T>::floats(p[i]);
-                t[2 * i] = (fminf(fmaxf(v.x, -65504.f), 65504.f) - mf) / sf + MAGIC;
-                t[2 * i + 1] = (fminf(fmaxf(v.y, -65504.f), 65504.f) - mf) / sf + MAGIC;
+                const float2 v = Two<T>::floats(p(i));
+                c[i] = Pair(rintf((fminf(fmaxf(v.x, -65504.f), 65504.f) - mf) / sf), rintf((fminf(fmaxf(v.y, -65504.f), 65504.f) - mf) / sf));
             }
         }
-        // (no value is more than half a step below the minimum; a scale that was rounded down to one of fp16's last steps reaches beyond 15)
+        // No value is more than half a step below the minimum.  Above, a normal scale is at most 2^-11 too small (15.008 steps); one rounded to
+        // fp16's last steps reaches beyond 15.
+        if (sf < 6.103515625e-5f) {
 #pragma unroll
-        for (int i = 7; i >= 0; --i) codes = codes * 16 + __float_as_uint(fminf(t[i], MAGIC + 15.f));
-        codes -= 0x4b400000u * 0x11111111u;
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = c[i].both();
+                c[i] = Pair(fminf(f.x, 15.f), fminf(f.y, 15.f));
+            }
+        }
+        const Pair step(256.f, 256.f);
+        const float2 a = fma2(c[1], step, c[0]).both(), b = fma2(c[3], step, c[2]).both();
+        codes = __byte_perm(__float_as_uint(fmaf(a.y, 16.f, a.x + 8388608.f)), __float_as_uint(fmaf(b.y, 16.f, b.x + 8388608.f)), 0x5410);
     }
     *scale = bad ? __ushort_as_half(0x7fff) : s;
     *low = m;
@@ -105,19 +136,19 @@ template <class T> __device__ __forceinline__ unsigned quantise8(const uint32_t 
 }
 
 // the tile that holds a row, and the row in it
-__device__ __forceinline__ long long tile_of(int slot, int head, int heads, int tiles_a_page) {
-    const unsigned tile = static_cast<unsigned>(slot) / KV4_TILE, page = tile / tiles_a_page;
+__device__ __forceinline__ long long tile_of(int slot, int head, int heads, int tiles_a_page, Divisor by_page) {
+    const unsigned tile = static_cast<unsigned>(slot) / KV4_TILE, page = by_page(tile);
     return (static_cast<long long>(page) * heads + head) * tiles_a_page + (tile - page * tiles_a_page);
 }
 
 template <class T, int G>
 __global__ void __launch_bounds__(CT) kv4_append_kernel(const T* __restrict__ key, const T* __restrict__ value, const int* __restrict__ slot_map,
-                                                        uint8_t* __restrict__ cache, unsigned items, int heads, int D, int tiles_a_page, long long slots,
+                                                        uint8_t* __restrict__ cache, unsigned items, int heads, int D, int tiles_a_page, Divisor by_heads, Divisor by_page, long long slots,
                                                         long long k_ts, long long k_hs, long long v_ts, long long v_hs) {
     const int l = threadIdx.x & 15;
     const unsigned item = blockIdx.x * ITEMS + threadIdx.x / 16;
     const bool there = item < items;
-    const unsigned tok = there ? item / heads : 0;
+    const unsigned tok = there ? by_heads(item) : 0;
     const int head = there ? static_cast<int>(item - tok * heads) : 0;
     const int slot = there ? slot_map[tok] : -1;
     if (slot >= slots && l == 0) report_bad_slot();
@@ -135,7 +166,7 @@ __global__ void __launch_bounds__(CT) kv4_append_kernel(const T* __restrict__ ke
     const unsigned kc = quantise8<T>(xk, real, &ks, &km), vc = quantise8<T>(xv, real, &vs, &vm);
     if (!kept || dim >= 32 * G) return;
     const int row = slot % KV4_TILE, which = l & 3;
-    uint8_t* tile = cache + tile_of(slot, head, heads, tiles_a_page) * kv4_tile_bytes(G);
+    uint8_t* tile = cache + tile_of(slot, head, heads, tiles_a_page, by_page) * kv4_tile_bytes(G);
     *reinterpret_cast<uint32_t*>(tile + kv4_key_half(G, row, dim)) = kc;
     *reinterpret_cast<uint16_t*>(tile + kv4_value_half(G, row, dim)) = static_cast<uint16_t>(vc);
     *reinterpret_cast<uint16_t*>(tile + kv4_value_half(G, row, dim + 4)) = static_cast<uint16_t>(vc >> 16);
@@ -182,16 +213,16 @@ template <> __device__ __forceinline__ uint4 unpack8<__nv_bfloat16>(unsigned cod
 
 template <class T, int G>
 __global__ void __launch_bounds__(CT) kv4_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ slot_map, T* __restrict__ key,
-                                                      T* __restrict__ value, unsigned items, int heads, int D, int tiles_a_page, long long slots) {
+                                                      T* __restrict__ value, unsigned items, int heads, int D, int tiles_a_page, Divisor by_heads, Divisor by_page, long long slots) {
     const int l = threadIdx.x & 15, dim = 8 * l;
     const unsigned item = blockIdx.x * ITEMS + threadIdx.x / 16;
     if (item >= items || dim >= D) return;
-    const unsigned tok = item / heads;
+    const unsigned tok = by_heads(item);
     const int head = static_cast<int>(item - tok * heads), slot = slot_map[tok];
     uint4 k = make_uint4(0, 0, 0, 0), v = k;
     if (slot >= 0 && slot < slots) {
         const int row = slot % KV4_TILE, g = l >> 2;
-        const uint8_t* tile = cache + tile_of(slot, head, heads, tiles_a_page) * kv4_tile_bytes(G);
+        const uint8_t* tile = cache + tile_of(slot, head, heads, tiles_a_page, by_page) * kv4_tile_bytes(G);
         auto par = [&](int which) { return *reinterpret_cast<const __half*>(tile + kv4_param(G, row, which, g)); };
         const unsigned kc = *reinterpret_cast<const uint32_t*>(tile + kv4_key_half(G, row, dim));
         const unsigned vc = *reinterpret_cast<const uint16_t*>(tile + kv4_value_half(G, row, dim)) |
@@ -272,7 +303,7 @@ int cf_kv4_append(const void* key, const void* value, int dtype, int64_t tokens,
     auto go = [&](auto* k, auto kernel) {
         kernel<<<static_cast<unsigned>(grid), CT, 0, static_cast<cudaStream_t>(stream)>>>(
             k, static_cast<decltype(k)>(value), slot_map, static_cast<uint8_t*>(cache), static_cast<unsigned>(items), static_cast<int>(kv_heads), static_cast<int>(head_dim),
-            static_cast<int>(page_size / KV4_TILE), pages * page_size, key_token_stride, key_head_stride, value_token_stride, value_head_stride);
+            static_cast<int>(page_size / KV4_TILE), Divisor(static_cast<unsigned>(kv_heads)), Divisor(static_cast<unsigned>(page_size / KV4_TILE)), pages * page_size, key_token_stride, key_head_stride, value_token_stride, value_head_stride);
     };
     with_groups(static_cast<int>(head_dim), [&](auto g) {
         if (dtype == CF_DTYPE_FP16) go(static_cast<const __half*>(key), kv4_append_kernel<__half, g.value>);
@@ -294,7 +325,7 @@ int cf_kv4_read(const void* cache, int64_t pages, int64_t page_size, int64_t kv_
     auto go = [&](auto* k, auto kernel) {
         kernel<<<static_cast<unsigned>(grid), CT, 0, static_cast<cudaStream_t>(stream)>>>(
             static_cast<const uint8_t*>(cache), slot_map, k, static_cast<decltype(k)>(value), static_cast<unsigned>(items), static_cast<int>(kv_heads), static_cast<int>(head_dim),
-            static_cast<int>(page_size / KV4_TILE), pages * page_size);
+            static_cast<int>(page_size / KV4_TILE), Divisor(static_cast<unsigned>(kv_heads)), Divisor(static_cast<unsigned>(page_size / KV4_TILE)), pages * page_size);
     };
     with_groups(static_cast<int>(head_dim), [&](auto g) {
         if (dtype == CF_DTYPE_FP16) go(static_cast<__half*>(key), kv4_read_kernel<__half, g.value>);
