@@ -814,9 +814,10 @@ template <class T, int G, int NT> cudaError_t launch(const Kv4AttnArgs& a, long 
     const long long items = static_cast<long long>(a.batch) * a.kv_heads;
     const long long q_tiles = (max_q_len * (a.heads / a.kv_heads) + COLS - 1) / COLS;
     const long long tiles = (a.table_width * a.page + KV4_TILE - 1) / KV4_TILE;
-    // as many CTAs to a (request, head) as fill the GPU (4 to an SM), but at least two tiles to a warp
+    // As many CTAs to a (request, head) as find room on the GPU at once (4 to an SM; a CTA costs 4 us besides its tiles, a tile 0.5 us of a
+    // warp: 256 pairs of up to 2048 tokens 19.4 us with 2, 23.8 with 4), but at least two tiles to a warp
     int cluster = 1;
-    while (cluster < MAX_CLUSTER && items * q_tiles * cluster < 4 * SMS && tiles >= 4 * W * cluster) cluster *= 2;
+    while (cluster < MAX_CLUSTER && items * q_tiles * cluster * 2 <= 4 * SMS && tiles >= 4 * W * cluster) cluster *= 2;
     static std::atomic<unsigned long long> allowed{0};
     const cudaError_t e = allow_shared_once(reinterpret_cast<const void*>(kv4_few_kernel<T, G, NT>), smem, allowed);
     if (e != cudaSuccess) return e;
@@ -850,13 +851,14 @@ long long kv4_few_workspace(long long heads, long long kv_heads, int D, long lon
 }
 
 // The line pays where requests of any length have to keep the GPU busy for long (from about 100 000 tiles of 16 tokens: 250 MB at
-// head_dim 128; below, its second launch and its look at all lengths cost what the even spread gives: 32 heads x 4096 tokens 15 us
-// against 9 us), and where there are too few (request, head) pairs for clusters of 8 CTAs to reach half the GPU and each is long
-// (8 heads x 32768 tokens: 21 us against 33 us).
+// head_dim 128; below, its second launch and its look at all lengths cost what the even spread gives.  Requests of mixed lengths, the line
+// against clusters: 512 (request, head) pairs of up to 8192 tokens 85 : 115 us, 256 pairs 49 : 59, 128 pairs 33 : 34, 160 pairs of up to 1000
+// tokens 16 : 12), and where there are too few pairs for clusters of 8 CTAs to reach half the GPU and each is long (8 heads x 32768
+// tokens 21 : 34, x 16384 16 : 19, x 8192 13 : 12).
 bool kv4_few_uses_workspace(long long batch, long long heads, long long kv_heads, long long tokens, long long max_q_len) {
     const long long rows = max_q_len * (heads / kv_heads), cols = rows <= 8 ? 8 : 16;
     const long long items = batch * kv_heads * ((rows + cols - 1) / cols), tiles = (tokens + KV4_TILE - 1) / KV4_TILE;
-    return items * tiles >= 100000 || (items * MAX_CLUSTER < 2 * SMS && tiles >= 512);
+    return items * tiles >= 100000 || (items * MAX_CLUSTER < 2 * SMS && tiles >= 640);
 }
 
 cudaError_t kv4_attention_few(const Kv4AttnArgs& a, bool bf16, long long max_q_len, cudaStream_t st) {
