@@ -5,8 +5,9 @@
 Nine translation units, compiled separately (objects cached under lib/obj/) and linked into one
 shared library: the decode kernel with the C ABI, the batched Llama decode blocks (hand-written
 tcgen05 skinny GEMMs + paged attention), the elementwise kernels of the prompt pass, the plan of a step over a
-paged cache, the cache held in 4 bits, the log probabilities of tokens, and the tensor-core prefill GEMM, which is built from the CUTLASS / CuTe headers found in the Python environment (the `flashinfer` wheel
-vendors them; set CUTLASS_INCLUDE to use another copy).  The library has no torch dependency;
+paged cache, the cache held in 4 bits (append and read; attention of few query rows; of many), the log probabilities of
+tokens, and the tensor-core prefill GEMM, which is built from the CUTLASS / CuTe headers found in the Python
+environment (the `flashinfer` wheel vendors them; set CUTLASS_INCLUDE to use another copy).  The library has no torch dependency;
 it links the CUDA runtime statically and finds the driver's tensor-map encoder at run time.  Beside it, lib/_serving.so binds
 the serving calls to Python (g++, torch's C++ headers).
 """

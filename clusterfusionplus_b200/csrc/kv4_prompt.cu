@@ -13,6 +13,10 @@
 //    memory is rescaled and the pass repeated.
 //  - 1 thread issues the products: S of the next tile before P V of this one, so that they run under the softmax.
 // Every wait is bounded; one that runs out ends the kernel with a device status.
+// Measured: chunks of 267, 723 and 985 queries over 267, 3514 and 3954 tokens, 32 heads over 8 of 128: 213 us, 440 TFLOP/s of products
+// (a quarter of the measured rate of large products).  The softmax warps are the chain: 3500 clocks a tile, 2400 of them arithmetic, 450 for
+// the agreement of a row's two threads, the rest waits that find their event already there; the unpacking warps need as many.  One
+// thread a row took 234 us, 256 rows a CTA (each unpacked tile used twice, at half the warps a row) 246 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -128,7 +132,7 @@ __device__ __forceinline__ uint32_t within_range(uint32_t s, uint32_t m) {
 }
 __device__ __forceinline__ bool finite_half(uint32_t x) { return (x & 0x7c00u) != 0x7c00u; }
 
-// N consecutive words / 16-bit numbers of global memory; two and four words are aligned to all of them
+// N consecutive words of global memory; two and four are aligned to all of them
 template <int N> __device__ __forceinline__ void global_words(uint32_t (&x)[N], const uint8_t* p) {
     if constexpr (N == 4) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
@@ -140,10 +144,6 @@ template <int N> __device__ __forceinline__ void global_words(uint32_t (&x)[N], 
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
     }
-}
-template <int N> __device__ __forceinline__ void global_halves(uint32_t (&x)[N], const uint8_t* p) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = __ldg(reinterpret_cast<const unsigned short*>(p) + i);
 }
 
 struct Shared {
