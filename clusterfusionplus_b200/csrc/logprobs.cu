@@ -8,7 +8,7 @@
 // 50304: 32 us of reading, 23 us of MUFU).  One CTA takes a row, or a cluster of CTAs a row when there are few rows: the partial
 // results meet in distributed shared memory, so there is no workspace and no second launch.  Measured on the GPU: 2047 rows of 50304 in
 // fp16 with the top 20 56 us (3.65 TB/s, 57 % of the copy bandwidth; issue slots 73 %, exponentials 51 %, memory 48 %: 7 instructions an
-// element, of which the top k takes one); one row of 50304 in fp32 with the top 5 7.5 us.
+// element, of which the top k takes one); one row of 50304 in fp32 with the top 5 7.1 us.
 //
 // The top k (at most 32) cost little more: every thread remembers its greatest element.  Of 64 groups of threads, the k-th
 // greatest group maximum bounds the k-th greatest element from below (k groups hold one each), and only a thread whose own greatest
@@ -463,9 +463,10 @@ extern "C" int cf_token_logprobs(const void* logits, int dtype, int64_t rows, in
     const int size = dtype == CF_DTYPE_FP32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(logits) % size != 0) return cf_host_fail(CF_ERR_INVALID, "logits are not aligned to their elements");
     LogprobArgs a{logits, tokens, logprobs, entropy, top_logprobs, reinterpret_cast<long long*>(top_tokens), row_stride, static_cast<int>(vocab), static_cast<int>(top_k), token_bytes == 8};
-    // few rows: up to 8 CTAs share one, each with at least 4096 elements (16 16-byte loads a thread; the exchange takes about 1 us)
+    // Few rows: up to 8 CTAs share one, each with at least 16 KB, below which the exchange costs what it saves (fp16, top 5: a row of 8192 alone
+    // 5.5 us, by two 6.5; 16 rows of 50304 by one CTA 9.6, by 4 7.8, by 8 8.4; fp32: a row of 50304 by one 11.2, by 4 7.4, by 8 7.1)
     int cluster = 1;
-    while (cluster < MAX_CLUSTER && rows * cluster < 148 && vocab / (2 * cluster) >= 4096) cluster *= 2;
+    while (cluster < MAX_CLUSTER && rows * cluster < 148 && vocab * size / (2 * cluster) >= 16384) cluster *= 2;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const cudaError_t e = dtype == CF_DTYPE_FP16   ? launch<__half>(a, rows, cluster, st)
                           : dtype == CF_DTYPE_BF16 ? launch<__nv_bfloat16>(a, rows, cluster, st)
