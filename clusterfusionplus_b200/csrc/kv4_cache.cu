@@ -264,16 +264,16 @@ int check_launch(const char* what) {
 }
 
 // Whether 128 query rows of a (request, cached head) shall share each unpacked tile (kv4_prompt.cu) or 16 at a time read the cache for
-// themselves (kv4_decode.cu).  The first takes 2.3 us for 128 tokens in each of 148 CTAs and does not divide the tokens among CTAs; the second
-// divides them evenly and takes 2 ns for 16 rows x 16 tokens, 8 us at least.  Measured (rows of a (request, head); the second against the
-// first): 32 pairs of 2048 tokens 48 rows 44 : 40 us, 24 rows 24 : 39; 256 pairs of 1000 tokens 24 rows 65 : 47; 8 pairs of 8192 tokens
-// 128 rows 44 : 136; 32 pairs of 4000 tokens 64 rows 68 : 72, 128 rows 89 : 74.
+// themselves (kv4_decode.cu).  The first takes 2.1 us for 128 tokens in each of 148 CTAs and does not divide the tokens among CTAs; the second
+// divides them evenly and takes 1.1 ns for 16 rows x 16 tokens and 14 us besides.  Measured (rows of a (request, head); the second against the
+// first): 32 pairs of 2048 tokens 64 rows 36 : 40 us, 24 rows 25 : 39; 256 pairs of 1000 tokens 32 rows 46 : 47; 8 pairs of 8192 tokens
+// 128 rows 48 : 134; 32 pairs of 4000 tokens 64 rows 50 : 71, 96 rows 72 : 72, 128 rows 82 : 72.
 bool prompt_sized(int64_t batch, int64_t heads, int64_t kv_heads, int64_t tokens, int64_t max_q_len) {
     const int64_t rows = max_q_len * (heads / kv_heads);
     if (rows <= 16) return false;
     const double pairs = static_cast<double>(batch) * kv_heads;
     const double turns = ceil(pairs * ((rows + 127) / 128) / 148);
-    return 8 + 0.002 * pairs * ((rows + 15) / 16) * ((tokens + 15) / 16) > 4 + 2.3 * turns * ((tokens + 127) / 128);
+    return 14 + 0.0011 * pairs * ((rows + 15) / 16) * ((tokens + 15) / 16) > 5 + 2.1 * turns * ((tokens + 127) / 128);
 }
 
 bool aligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }

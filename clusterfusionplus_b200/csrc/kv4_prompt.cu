@@ -13,9 +13,10 @@
 //    memory is rescaled and the pass repeated.
 //  - 1 thread issues the products: S of the next tile before P V of this one, so that they run under the softmax.
 // Every wait is bounded; one that runs out ends the kernel with a device status.
-// Measured: chunks of 267, 723 and 985 queries over 267, 3514 and 3954 tokens, 32 heads over 8 of 128: 213 us, 440 TFLOP/s of products
-// (a quarter of the measured rate of large products).  The softmax warps are the chain: 3500 clocks a tile, 2400 of them arithmetic, 450 for
-// the agreement of a row's two threads, the rest waits that find their event already there; the unpacking warps need as many.  One
+// Measured: chunks of 267, 723 and 985 queries over 267, 3514 and 3954 tokens, 32 heads over 8 of 128: 202 us, 465 TFLOP/s of products
+// (28 % of the measured rate of large products).  The softmax warps are the chain: 3500 clocks a tile, 2400 of them arithmetic, 450 for
+// the agreement of a row's two threads, the rest waits that find their event already there; the unpacking warps need as many, and what makes
+// one of them faster (a hardware barrier for the agreement, half the commits, no bank conflicts, look-ups moved) slows the others: 202 to 210.  One
 // thread a row took 234 us, 256 rows a CTA (each unpacked tile used twice, at half the warps a row) 246 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -233,12 +234,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
             const int last = real ? static_cast<int>(max(min(before + qi, cap - 1), -1ll)) : -1;
             const int all_see = static_cast<int>(max(min(before + r0 / per, cap - 1), -1ll));  // every real row sees these
             if (n > 0) {
-                float top = 0.f;
-                for (int d = 0; d < a.D; d += 8) {
-                    const uint4 v = real ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                // all loads of the row at once: in turn they would take longer than a tile.  The row's two threads write half of it each.
+                uint4 own[DP / 16], rest[DP / 16];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                for (int j = 0; j < DP / 16; ++j) {
+                    const int d = 16 * j + 8 * half, e = 16 * j + 8 * (half ^ 1);
+                    own[j] = real && d < a.D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+                    rest[j] = real && e < a.D ? *reinterpret_cast<const uint4*>(src + e) : make_uint4(0, 0, 0, 0);
+                }
+                float top = 0.f;
+#pragma unroll
+                for (int j = 0; j < DP / 16; ++j) {
+                    const uint32_t w[8] = {own[j].x, own[j].y, own[j].z, own[j].w, rest[j].x, rest[j].y, rest[j].z, rest[j].w};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
                         const float2 f = to_float2<T>(w[i]);
                         top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
                     }
@@ -246,9 +255,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                 // a power of two takes the row to at most 2^10 (exact; bf16 reaches beyond fp16), the scale's sign goes along
                 const int e = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100);
                 const float up = copysignf(power_of_two(min(9 - e, 127)), a.scale_log2);
-                for (int d = 8 * half; d < N; d += 16) {
-                    const uint4 v = real && d < a.D ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < DP / 16; ++j) {
+                    const int d = 16 * j + 8 * half;
+                    const uint32_t w[4] = {own[j].x, own[j].y, own[j].z, own[j].w};
                     float v8[8];
                     uint32_t o[4];
 #pragma unroll
