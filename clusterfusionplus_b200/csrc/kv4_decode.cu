@@ -562,8 +562,10 @@ __global__ void __launch_bounds__(32 * W, NT == 1 ? 4 : 2) kv4_few_kernel(const 
     const int item = static_cast<int>(blockIdx.x / cluster), b = item / a.kv_heads, kvh = item - b * a.kv_heads;
     const Request own(a, b);
     const int units = cluster * W, unit = rank * W + warp;
+    if (cluster > 1) cluster_arrive();  // waited for before the first store to a peer, which must have begun by then
 
-    for (int r0 = blockIdx.y * COLS; r0 < own.rows; r0 += gridDim.y * COLS) {
+    const int first_row = blockIdx.y * COLS;
+    for (int r0 = first_row; r0 < own.rows; r0 += gridDim.y * COLS) {
         const long long end = min(own.before + (min(r0 + COLS, own.rows) - 1) / own.per, own.cap - 1);  // the last token that these rows see
         const int tiles = end < 0 ? 0 : static_cast<int>(end / KV4_TILE) + 1;
         Feed<G> feed(a, warp);
@@ -578,6 +580,7 @@ __global__ void __launch_bounds__(32 * W, NT == 1 ? 4 : 2) kv4_few_kernel(const 
         float* lines = reinterpret_cast<float*>(smem);
         acc.store(lines + warp * COLS * LINE);
         __syncthreads();
+        if (cluster > 1 && r0 == first_row) cluster_wait();
         const int cols = min(COLS, own.rows - r0);
         const int owned = (PIECES + cluster - 1) / cluster;  // pieces of one CTA, at most
         for (int e = threadIdx.x; e < cols * DP; e += 32 * W) {
@@ -614,6 +617,7 @@ __global__ void __launch_bounds__(32 * W, NT == 1 ? 4 : 2) kv4_few_kernel(const 
             __syncthreads();
         }
     }
+    if (cluster > 1 && first_row >= own.rows) cluster_wait();  // no rows
 }
 
 // ---------------------------------------------------------------------------------------------------- much work

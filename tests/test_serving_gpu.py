@@ -704,6 +704,19 @@ def test_serving_step_captured_and_replayed(cuda_device):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_attention_with_ctas_that_have_nothing_to_read(cuda_device):
+    """A wide block table asks for clusters of 8 CTAs; requests of 0, 1 and 17 tokens, and without queries, leave most of them nothing to do but
+    send their empty results to the others."""
+    import clusterfusionplus_b200 as cf
+    lens, counts = [1, 0, 17, 1, 300, 2, 1, 1], [1, 1, 1, 0, 1, 1, 0, 1]
+    q, cache, table, starts = attention_case(lens, counts, 4, 2, 64, 16, torch.float16, 21)
+    wide = [row + [-1] * (4096 - len(row)) for row in table]
+    K, V = S.unpack(cache, 64)
+    ref = S.attention(q, K, V, table, lens, starts, 64 ** -0.5)
+    for _ in range(20):
+        close(cf.kv4_attention(q, cache, ints(wide), ints(lens), ints(starts)), ref, q, K, V, 64 ** -0.5)
+
+
 def test_calls_on_two_streams_do_not_disturb_each_other(cuda_device, schedule):
     import clusterfusionplus_b200 as cf
     cases = []
