@@ -82,6 +82,12 @@ def test_plan(cuda_device, B, page, most_len, most_new, rows):
     check_plan(lens, new, table, free, len(free), page, sum(new) + rng.choice([0, 1, 5, 300]), (total + rng.choice([0, 1, 2, 3, 1030]) or 1) if rows else 0, strided=B % 2 == 1)
 
 
+@pytest.mark.parametrize("B", [2390, 2448, 2457, 2458])
+def test_plan_batches_around_the_default_shared_memory(cuda_device, B):
+    lens, new, table, free = plan_case(random.Random(B), B, 16, 4, 30, 3)
+    check_plan(lens, new, table, free, len(free), 16, sum(new), sum(lens) + sum(new))
+
+
 def test_plan_long_prompts_fill_many_pages(cuda_device):
     rng = random.Random(2)
     lens, new = [5, 0, 1000], [20000, 1, 9000]
