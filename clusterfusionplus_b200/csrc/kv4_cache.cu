@@ -338,7 +338,9 @@ int cf_kv4_read(const void* cache, int64_t pages, int64_t page_size, int64_t kv_
 }
 
 int64_t cf_kv4_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_tokens, int64_t max_q_len) {
-    if (batch < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || head_dim < 1 || head_dim > KV4_MAX_DIM || max_tokens < 1 || max_q_len < 1) return 0;
+    if (batch < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || head_dim < 1 || head_dim > KV4_MAX_DIM || max_tokens < 1 || max_q_len < 1 || max_q_len > 0x7fffffff ||
+        batch > 0x7fffffff || heads > 0x7fffffff || max_tokens > 0x7fffffffll * 65536)
+        return 0;
     if (prompt_sized(batch, heads, kv_heads, max_tokens, max_q_len)) return 0;
     return kv4_few_uses_workspace(batch, heads, kv_heads, max_tokens, max_q_len) ? kv4_few_workspace(heads, kv_heads, static_cast<int>(head_dim), max_q_len) : 0;
 }
@@ -350,7 +352,7 @@ int cf_kv4_attention(const void* query, int dtype, int64_t rows, int64_t heads, 
     if (int rc = check_cache(pages, kv_heads, page_size, head_dim)) return rc;
     if (dtype != CF_DTYPE_FP16 && dtype != CF_DTYPE_BF16) return cf_host_fail(CF_ERR_INVALID, "dtype %d is neither fp16 nor bf16", dtype);
     if (heads < kv_heads || heads % kv_heads != 0) return cf_host_fail(CF_ERR_INVALID, "%lld query heads over %lld cached heads", (long long)heads, (long long)kv_heads);
-    if (rows < 0 || rows > 0x7fffffff || batch < 1 || batch > 0x7fffffff || max_q_len < 1)
+    if (rows < 0 || rows > 0x7fffffff || batch < 1 || batch > 0x7fffffff || max_q_len < 1 || max_q_len > 0x7fffffff)
         return cf_host_fail(CF_ERR_INVALID, "rows %lld, batch %lld, max_q_len %lld", (long long)rows, (long long)batch, (long long)max_q_len);
     if (!qo_indptr && rows < batch) return cf_host_fail(CF_ERR_INVALID, "%lld query rows for %lld requests", (long long)rows, (long long)batch);
     if (table_width < 1 || table_stride < table_width || table_width > 0x7fffffff) return cf_host_fail(CF_ERR_INVALID, "block table of %lld columns, %lld entries apart", (long long)table_width, (long long)table_stride);

@@ -54,7 +54,8 @@ def paged_kv_plan(cached_lens, new_lens, block_table, free_pages, free_count, pa
 
 def paged_kv_release(finished, kv_lens, block_table, free_pages, free_count, page_size: int):
     """Gives the pages of the requests with finished[b] != 0 (int32 [batch]) back: the first ceil(kv_lens[b] / page_size) entries of their
-    table rows go on top of free_pages and become -1.  Returns (free_count, status), int32 [1] each; all or nothing like paged_kv_plan."""
+    table rows go on top of free_pages and become -1.  Returns (free_count, status), int32 [1] each; all or nothing like paged_kv_plan.
+    Pages are not counted: one that several requests name goes onto the list with each of them."""
     return _call.release(finished, kv_lens, block_table, free_pages, free_count, page_size)
 
 

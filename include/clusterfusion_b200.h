@@ -436,7 +436,8 @@ int cf_paged_kv_plan(const int* cached_lens, const int* new_lens, int64_t batch,
 
 /* Gives the pages of the requests with finished[b] != 0 (int32 [batch]) back: the first ceil(kv_lens[b] / page_size) entries
  * of their table rows go on top of the free list (capacity n_free_pages) in request and column order and become -1.
- * *free_count_out as above.  All or nothing, *status as above. */
+ * *free_count_out as above.  All or nothing, *status as above.  Pages are not counted: one that several requests name
+ * goes onto the list with each of them that is released. */
 int cf_paged_kv_release(const int* finished, const int* kv_lens, int64_t batch, int* block_table, int64_t table_width,
                         int64_t table_stride, int* free_pages, int64_t n_free_pages, const int* free_count, int* free_count_out,
                         int64_t page_size, int* status, void* stream);

@@ -67,6 +67,14 @@ def test_attention_refusals(kw, match):
     refused("cf_kv4_attention", list((a | kw).values()), match)
 
 
+def test_attention_refuses_a_hint_beyond_any_call():
+    from clusterfusionplus_b200._lib import lib
+    a = [ONE, 0, 3, 8, 128, 1024, 128, ONE, 4, 16, 4, ONE, 8, 8, ONE, ONE, 4, 1 << 62, 0.1, None, 0, ctypes.c_void_p(1 << 20), None]
+    refused("cf_kv4_attention", a, "max_q_len")
+    assert lib.cf_kv4_attention_workspace(4, 8, 4, 128, 1 << 14, 1 << 62) == 0
+    assert lib.cf_kv4_attention_workspace(4, 1 << 62, 1 << 61, 128, 1 << 14, 4) == 0
+
+
 @pytest.mark.parametrize("at", [0, 256 * 7, 2 * 1024 * 2 + 2 * 1024 - 16])
 @pytest.mark.parametrize("first", ["query", "out"])
 def test_attention_refuses_an_output_over_the_queries(at, first):
