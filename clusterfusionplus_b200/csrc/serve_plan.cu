@@ -10,7 +10,7 @@
 // free list, and expands its share of the token and row lists; CTA 0 writes what exists once.  A CTA reads only table
 // entries below have_b and CTA 0 writes only entries from have_b on, so nothing is read that another CTA writes.
 // Measured on the GPU: 16 requests of up to 2048 tokens 4.6 us, 256 requests of up to 8192 with 1.0 M listed rows (4.8 MB, 0.7 us of
-// writing) 8.0 us: a launch, three scans of the batch and the issue of ~8 instructions a row (65 % of the issue slots).
+// writing) 8.0 us: a launch, three scans of the batch and the issue of ~5 instructions a row (63 % of the issue slots).
 #include <cuda_runtime.h>
 
 #include <cstdint>
