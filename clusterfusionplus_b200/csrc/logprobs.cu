@@ -7,10 +7,10 @@
 // fp32's relative precision.  The floor is reading the logits once; one exponential an element comes second (2047 rows of
 // 50304: 32 us of reading, 23 us of MUFU).  One CTA takes a row, or a cluster of CTAs a row when there are few rows: the partial
 // results meet in distributed shared memory, so there is no workspace and no second launch.  Measured on the GPU: 2047 rows of 50304 in
-// fp16 with the top 20 56 us (3.65 TB/s, 57 % of the copy bandwidth; issue slots 73 %, exponentials 51 %, memory 48 %: 7 instructions an
-// element, of which the top k takes one); one row of 50304 in fp32 with the top 5 7.1 us.
+// fp16 with the top 20 56 us (3.65 TB/s, 57 % of the copy bandwidth; issue slots 73 %, exponentials 51 %, memory 48 %: 14 instructions an
+// element; without the top k 43 us); one row of 50304 in fp32 with the top 5 7.1 us.
 //
-// The top k (at most 32) cost little more: every thread remembers its greatest element.  Of 64 groups of threads, the k-th
+// The top k (at most 32) cost a quarter more: every thread remembers its greatest element.  Of 32 or 64 groups of threads, the k-th
 // greatest group maximum bounds the k-th greatest element from below (k groups hold one each), and only a thread whose own greatest
 // reaches the bound can hold any of the top k.  There are a few more than k of them: their elements are looked through
 // once more, what reaches the bound is kept, ranked by counting and written.  Order: greater first, equal values by the lower
@@ -33,7 +33,6 @@ using cfb::Pair;
 
 constexpr int LT = 256;        // threads of a CTA
 constexpr int LW = LT / 32;
-constexpr int GROUPS = 64;     // of LT / GROUPS threads, for the bound of the top k
 constexpr int MAX_TOP = 32;
 constexpr int MAX_CLUSTER = 8;
 constexpr int KEEP = 1024;     // candidates that are kept; more (adversarial orders only) take the slow way
@@ -193,7 +192,7 @@ __device__ __forceinline__ unsigned long long peer_u64(uint32_t a) {
 
 struct __align__(16) Shared {
     unsigned long long best[LT];
-    unsigned long long group[GROUPS];
+    unsigned long long group[64];
     unsigned long long keep[KEEP];
     unsigned long long top[MAX_TOP];
     unsigned long long all[MAX_CLUSTER * MAX_TOP];
@@ -216,7 +215,7 @@ template <int PARTS> __device__ __forceinline__ int count_greater(const unsigned
 // The k greatest of [w.begin, w.end) as ranked() words in sh.top, greatest first, 0 where there are fewer.  `best`: this thread's greatest (0
 // for none), its index rounded down to the start of its vector.  In this coarser order k elements reach the bound, and one
 // that does not has k elements above it in the exact order too.
-template <class T> __device__ void block_top(const Walk<T>& w, unsigned long long best, int k, Shared& sh) {
+template <int GROUPS, class T> __device__ void block_top(const Walk<T>& w, unsigned long long best, int k, Shared& sh) {
     constexpr int E = Walk<T>::E;
     const int tid = threadIdx.x;
     sh.best[tid] = best;
@@ -382,7 +381,11 @@ __global__ void __launch_bounds__(LT, 8) token_logprobs_kernel(const LogprobArgs
                     }
             }
         }
-        block_top(w, best, a.top, sh);
+        // Ranking g groups costs g squared; of g the k-th greatest has about g ln(g / (g - k)) elements above it (k = 5: 5.4 with 32, 5.2 with
+        // 64; k = 20: 31 and 24).  One row of 50304 with the top 5 6.7 us by 32 groups, 7.0 by 64; 2047 rows with the top 20 57.0 and 56.4.
+        // Groups without elements bound nothing, so every thread has to have some for the large groups.
+        if (a.top <= 10 && w.vecs >= LT) block_top<32>(w, best, a.top, sh);
+        else block_top<64>(w, best, a.top, sh);
     }
 
     auto join_lanes = [&](int width) {

@@ -573,6 +573,13 @@ def test_logprobs_large_logits_keep_their_precision(cuda_device):
     check_logprobs(x, [1, 2, 3, 4], 8)
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.float16, v) for v in (2040, 2047, 2048, 2049, 2063)] + [(torch.float32, v) for v in (1020, 1024, 1027)])
+@pytest.mark.parametrize("k", [1, 10, 11])
+def test_logprobs_where_every_thread_just_has_elements(cuda_device, dtype, vocab, k):
+    """256 threads of one 16-byte vector each, give or take one: the bound of the top k comes from more or fewer groups of them."""
+    check_logprobs(logits(3, vocab, dtype, vocab + k, pad=3), [0, vocab - 1, vocab // 2], k)
+
+
 def test_logprobs_of_one_vector_and_of_none(cuda_device):
     import clusterfusionplus_b200 as cf
     x = logits(1, 1000, torch.float32, 2)
