@@ -748,6 +748,35 @@ def test_calls_on_two_streams_do_not_disturb_each_other(cuda_device, schedule):
     assert all(torch.equal(x, want[i]) for i in (0, 1) for x in got[i])
 
 
+def test_calls_of_two_threads(cuda_device):
+    """Each on a stream of its own; one thread's refusals do not reach the other."""
+    import threading
+
+    import clusterfusionplus_b200 as cf
+    want, got, errors = [], [[], []], []
+    cases = [attention_case(lens, [1, 1], 8, 2, 64, 16, torch.float16, seed) for seed, lens in ((1, [700, 30]), (2, [9, 1200]))]
+    args = [(q, cache, ints(table), ints(lens)) for (q, cache, table, _), lens in zip(cases, ([700, 30], [9, 1200]))]
+    want = [cf.kv4_attention(*a) for a in args]
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(200):
+                    got[i].append(cf.kv4_attention(*args[i]))
+                    with pytest.raises(RuntimeError, match="page size" if i else "max_q_len"):
+                        cf.paged_kv_plan(args[i][3], args[i][3], args[i][2], args[i][3], args[i][3][:1], 0, 4) if i else cf.kv4_attention(*args[i], max_q_len=0)
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # noqa: BLE001 (handed to the test's own thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors, errors
+    assert all(len(got[i]) == 200 and torch.equal(x, want[i]) for i in (0, 1) for x in got[i])
+
+
 def test_first_calls_of_a_process_inside_a_capture(cuda_device):
     """Nothing that a first call sets up (kernel attributes, addresses) is forbidden while a stream is captured."""
     import subprocess
