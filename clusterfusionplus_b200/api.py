@@ -226,7 +226,8 @@ def llama_decoder_layer_batch_decode_sglang(output, residual_output, input, resi
     """The Llama-2-7B attention block for a batch of decode sequences over a paged KV pool; writes into
     `output` and `residual_output` ([batch, 4096] fp16 each) and returns None, like the reference.
     input / residual [batch, 4096] fp16; paged_kv_indptr [batch + 1] and paged_kv_indices int32 (one pool row per
-    token; a sequence's last entry is the slot the new key / value go to); k_cache_ptrs / v_cache_ptrs: int64 /
+    token; a sequence's last entry is the slot the new key / value go to; an entry below 0 is left out and reported by
+    device_status(), an empty list writes nothing); k_cache_ptrs / v_cache_ptrs: int64 /
     uint64 device tensors with one pool pointer per layer ([pool_rows, 4096] fp16 pools); positions [batch] int64;
     cos_sin [max_position, 128] fp32 (64 cosines, 64 sines per row).
     Reference: llama_decoder_layer_batch_sglang_sm120, include/pybind.cpp:90-106,282."""

@@ -876,7 +876,7 @@ int cf_get_status(int* status) {
     if (worst != 0)
         return fail(CF_ERR_DEVICE,
                     "device status %d (1-2 TMA ring, 3 grid barrier / flag wait, 4 cluster exchange, 5 bad seq_len, "
-                    "6 drain, 7 tensor-parallel peer never answered, 8 page or slot outside the 4-bit cache)",
+                    "6 drain, 7 tensor-parallel peer never answered, 8 page, slot or row outside its paged cache)",
                     worst);
     return CF_OK;
 }

@@ -36,6 +36,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "pipeline.cuh"
 
 namespace cfb {
@@ -54,6 +56,7 @@ constexpr int KV_ROWS = 128;          // cache rows per attention item
 constexpr int REC = D + 4;            // partial record: D numerators, max, denominator, pad
 constexpr int TMEM_COLS = 512;
 
+constexpr int ST_NO_ROW = 8;          // device status: an entry of a page list names no row
 enum : int { MODE_ATTN = 0, MODE_MLP = 1 };
 
 // One weight matrix [rows, K] as a 3-D tensor {64 K elements, rows, K / 64 blocks}: a box {64, R, kb} brings R
@@ -219,7 +222,7 @@ struct Ring {
 // ---------------------------------------------------------------- the kernel
 __global__ void __launch_bounds__(THREADS, 1) llama_batch_kernel(const __grid_constant__ Params p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    // [ring NSTAGE x STAGE_BYTES][q 128 f][merge 16 x 128 f + 32 f][red 32 f][prefix 17 i][barriers][tmem ptr][abort]
+    // [ring NSTAGE x STAGE_BYTES][q 128 f][merge 16 x 128 f + 32 f][red 32 f][prefix 17 i, lengths 16 i][barriers][tmem ptr][abort][holes]
     uint8_t* ring = smem_raw;
     float* q_s = reinterpret_cast<float*>(ring + NSTAGE * STAGE_BYTES);
     float* mbuf = q_s + D;             // [16][D]
@@ -237,6 +240,7 @@ __global__ void __launch_bounds__(THREADS, 1) llama_batch_kernel(const __grid_co
     uint64_t* acc_bar = bars + 4 * NSTAGE;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * NSTAGE + 1);
     int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+    volatile int* holes = abort_flag + 1;  // an entry of a history that this CTA reads is below 0
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = gridDim.x, cta = blockIdx.x;
@@ -245,6 +249,7 @@ __global__ void __launch_bounds__(THREADS, 1) llama_batch_kernel(const __grid_co
 
     if (tid == 0) {
         *abort_flag = 0;
+        *holes = 0;
         for (int s = 0; s < NSTAGE; ++s) {
             mbar_init(smem_u32(full + s), 1);
             mbar_init(smem_u32(empty + s), 1);
@@ -539,22 +544,46 @@ __global__ void __launch_bounds__(THREADS, 1) llama_batch_kernel(const __grid_co
                 }
             });
         }
+        // ---- meanwhile, by warps that the projection leaves idle: the items of the attention, (sequence, head, 128-row chunk), and
+        // whether each entry of the page lists that this CTA's share of them reads names a row
+        if (warp >= 1 && warp < NCW) {
+            const int s = lane < B ? max(0, __ldg(p.indptr + lane + 1) - 1 - __ldg(p.indptr + lane)) : 0;
+            const int mine = NH * ((s + KV_ROWS - 1) / KV_ROWS);
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += up;
+            }
+            if (warp == 1) {
+                if (lane <= MAXB) pre[lane] = upto - mine;
+                if (lane < B) pre[MAXB + 1 + lane] = s;
+            }
+            const int total = __shfl_sync(0xffffffffu, upto, 31), from = pbegin(cta, total, G), to = pbegin(cta + 1, total, G);
+            bool hole = false;
+            for (int b = 0; b < B; ++b) {
+                const int first = __shfl_sync(0xffffffffu, upto - mine, b), rows = __shfl_sync(0xffffffffu, s, b), nch = (rows + KV_ROWS - 1) / KV_ROWS;
+                const int lo = max(from - first, 0), n = min(to - first, NH * nch) - lo;
+                if (n <= 0) continue;
+                const int* list = p.indices + __ldg(p.indptr + b);
+                auto scan = [&](int c0, int c1) {
+#pragma unroll 4
+                    for (int i = c0 * KV_ROWS + tid - 32; i < min(c1 * KV_ROWS, rows); i += NCT - 32) hole |= __ldg(list + i) < 0;
+                };
+                const int c0 = n < nch ? lo % nch : 0;  // chunks c0 .. and, past the last, those of the next head from 0
+                scan(c0, min(c0 + n, nch));
+                if (n < nch && c0 + n > nch) scan(0, c0 + n - nch);
+            }
+            if (hole) {
+                *holes = 1;
+                atomicCAS(p.status, 0, ST_NO_ROW);
+            }
+        }
         mark();
         grid_barrier();
         mark();
 
-        // ---- attention over the cached rows: items (sequence, head, 128-row chunk), evenly split
-        if (tid == 0) {
-            int acc = 0;
-            for (int b = 0; b < B; ++b) {
-                const int s = max(0, __ldg(p.indptr + b + 1) - 1 - __ldg(p.indptr + b));
-                pre[b] = acc;
-                pre[MAXB + 1 + b] = s;
-                acc += NH * ((s + KV_ROWS - 1) / KV_ROWS);
-            }
-            for (int b = B; b <= MAXB; ++b) pre[b] = acc;
-        }
-        __syncthreads();
+        // ---- attention over the cached rows, its items evenly split
         const int T = pre[B];
         const int ta = pbegin(cta, T, G), tb = pbegin(cta + 1, T, G);
         const __half* kpool = reinterpret_cast<const __half*>(__ldg(p.k_ptrs + p.layer_id));
@@ -569,6 +598,9 @@ __global__ void __launch_bounds__(THREADS, 1) llama_batch_kernel(const __grid_co
             ch = rem - h * nch;
         };
         const float qscale = 1.4426950408889634f * rsqrtf(static_cast<float>(D));
+        // HOLES: some entry is below 0.  Nothing is copied for it, its score is -inf and its value zero.
+        auto attend = [&](auto with_holes) {
+        constexpr bool HOLES = decltype(with_holes)::value;
         if (warp >= NCW) {
             // ---- gather producers: NGW warps, each copies a quarter of a tile's rows with 16-byte asynchronous
             // copies (one bulk copy per row measured 8 us per item: the copy engine takes one operation at a
@@ -602,7 +634,7 @@ __global__ void __launch_bounds__(THREADS, 1) llama_batch_kernel(const __grid_co
                         const int rl = 2 * i + hi;                 // row within this warp's quarter
                         const int page = __shfl_sync(0xffffffffu, pg, rl);
                         const int r = gw * 32 + rl;
-                        if (r < nvalid) {
+                        if (r < nvalid && (!HOLES || page >= 0)) {
                             const __half* src = pool + static_cast<size_t>(page) * H + piece * 8;
                             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sb + r * D * 2 + piece * 16), "l"(src) : "memory");
                         }
@@ -703,6 +735,15 @@ __global__ void __launch_bounds__(THREADS, 1) llama_batch_kernel(const __grid_co
 #pragma unroll
                     for (int j = 0; j < 8; ++j) sc8[j] += __shfl_xor_sync(0xffffffffu, sc8[j], o);
                 }
+                unsigned gone = 0;  // bit j: row j is an entry below 0
+                if (HOLES) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (grow + j < s && __ldg(p.indices + __ldg(p.indptr + b) + grow + j) < 0) {
+                            gone |= 1u << j;
+                            sc8[j] = -INFINITY;
+                        }
+                }
                 float mx = m_run;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -724,7 +765,7 @@ __global__ void __launch_bounds__(THREADS, 1) llama_batch_kernel(const __grid_co
                     for (int k = 0; k < 8; ++k) acc[k] *= scl;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        if (grow + j < s) {
+                        if (grow + j < s && !(HOLES && (gone >> j & 1u))) {
                             const float pj = sc8[j];
                             l_run += pj;
                             const uint4 raw = *reinterpret_cast<const uint4*>(vt + (r0 + j) * D + l16 * 8);
@@ -744,6 +785,9 @@ __global__ void __launch_bounds__(THREADS, 1) llama_batch_kernel(const __grid_co
             }
             if (cur_pair >= 0) flush(cur_pair);
         }
+        };
+        if (*holes) attend(std::true_type());
+        else attend(std::false_type());
         mark();
         grid_barrier();
         mark();
@@ -767,11 +811,19 @@ __global__ void __launch_bounds__(THREADS, 1) llama_batch_kernel(const __grid_co
                     const __half v16 = __float2half_rn(__ldcg(base + 2 * H + d));
                     kd = __half2float(k16);
                     vd = __half2float(v16);
-                    // the slot of the new token: last entry of the sequence's page list
-                    const int slot = __ldg(p.indices + __ldg(p.indptr + b + 1) - 1);
-                    const size_t off = static_cast<size_t>(slot) * H + h * D + d;
-                    const_cast<__half*>(reinterpret_cast<const __half*>(__ldg(p.k_ptrs + p.layer_id)))[off] = k16;
-                    const_cast<__half*>(reinterpret_cast<const __half*>(__ldg(p.v_ptrs + p.layer_id)))[off] = v16;
+                    // the slot of the new token: last entry of the sequence's page list.  An empty list (a request without tokens, or
+                    // the lists of a plan that did not fit) has none, and an entry below 0 is no row: nothing is stored then.
+                    const int end = __ldg(p.indptr + b + 1);
+                    if (end > __ldg(p.indptr + b)) {
+                        const int slot = __ldg(p.indices + end - 1);
+                        if (slot >= 0) {
+                            const size_t off = static_cast<size_t>(slot) * H + h * D + d;
+                            const_cast<__half*>(reinterpret_cast<const __half*>(__ldg(p.k_ptrs + p.layer_id)))[off] = k16;
+                            const_cast<__half*>(reinterpret_cast<const __half*>(__ldg(p.v_ptrs + p.layer_id)))[off] = v16;
+                        } else if (d == 0) {
+                            atomicCAS(p.status, 0, ST_NO_ROW);
+                        }
+                    }
                 }
                 const float s_new = csum(qd * kd, red, tid);
                 if (tid < D) {

@@ -86,8 +86,8 @@ int cf_launch_info(int model, int* sm_count, int* grid, int* cluster, int* stage
  * (synchronises the device) -- clears what was set and re-arms the barrier words.
  * *status = 0 when every launch so far finished normally; otherwise the call returns
  * CF_ERR_DEVICE and *status is 1-2 TMA ring, 3 grid barrier / flag wait, 4 cluster exchange,
- * 5 bad seq_len, 6 drain, 7 tensor-parallel peer never answered, 8 a page or slot outside the
- * 4-bit cache (its rows were skipped). */
+ * 5 bad seq_len, 6 drain, 7 tensor-parallel peer never answered, 8 a page, slot or row outside its
+ * paged cache (it was skipped). */
 int cf_get_status(int* status);
 
 /* Fused decoder layer, one token at batch 1.  The first call with a given set of tensors
@@ -180,7 +180,8 @@ int cf_batch_abort(void);
  * paged_kv_indices[paged_kv_indptr[b] .. paged_kv_indptr[b+1]) -- one row = one token, [4096] fp16 --
  * of the pools k_cache_ptrs[layer_id] / v_cache_ptrs[layer_id] (device arrays of device pointers): the LAST
  * entry is the slot the new key / value are written to, the entries before it are the history that is
- * attended to (plus the new token); every sequence needs at least that one entry.
+ * attended to (plus the new token).  An entry below 0 is not there: it is not attended to, nothing is written to it, and it is
+ * recorded (cf_get_status 8).  A sequence whose list is empty writes nothing and attends to its new token alone.
  * output[b] = weight_o attention(b).  All tensors [batch, 4096] fp16 unless said otherwise; indptr /
  * indices int32, positions int64.  The weights are streamed once for the whole batch: the projections run
  * as skinny GEMMs on the tensor cores (tcgen05), the rest as in the batch-1 block.  The first call on a

@@ -1,0 +1,115 @@
+"""Calls of the serving operators, and of the paged Llama block behind a step plan, that their documentation allows and that lie at the edges:
+lists of a plan that did not fit, idle requests, pages that were never given, values next to a type's largest."""
+import math
+import random
+
+import pytest
+import torch
+
+from oracle import llama_oracle as LO
+from oracle import pythia_oracle as O
+from oracle import serving_oracle as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+H = 4096
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+@pytest.fixture(autouse=True)
+def clean_status(cuda_device):
+    import clusterfusionplus_b200 as cf
+    yield
+    torch.cuda.synchronize()
+    assert cf.device_status() == 0
+
+
+# ------------------------------------------------------------------------------------------- the paged Llama block's lists
+@pytest.fixture(scope="module")
+def llama(cuda_device):
+    inv = 1.0 / (10000.0 ** (torch.arange(0, 128, 2, dtype=torch.float32) / 128))
+    ang = torch.outer(torch.arange(512, dtype=torch.float32), inv)
+    return dict(wqkv=O.seeded_normal((3 * H, H), 5, std=0.02, device=DEV), wo=O.seeded_normal((H, H), 6, std=0.02, device=DEV),
+                g=O.seeded_normal((H,), 7, mean=1.0, std=0.02, device=DEV), cs=torch.cat([ang.cos(), ang.sin()], dim=1).contiguous().to(DEV))
+
+
+class Pools:
+    """Key and value rows with two more ahead of them and behind them, which nothing may touch."""
+
+    def __init__(self, rows):
+        self.room = [O.seeded_normal((rows + 4, H), seed, device=DEV) for seed in (1, 2)]
+        self.before = [r.clone() for r in self.room]
+        self.pools = [r[2:-2] for r in self.room]
+        self.start = [p.clone() for p in self.pools]
+
+    def only(self, rows):
+        """Only these rows have changed."""
+        keep = torch.ones(self.room[0].shape[0], dtype=torch.bool, device=DEV)
+        if rows:
+            keep[torch.tensor(rows, device=DEV) + 2] = False
+        return all(torch.equal(r[keep], b[keep]) for r, b in zip(self.room, self.before))
+
+
+def run_block(w, pools, indptr, indices, positions):
+    import clusterfusionplus_b200 as cf
+    B = indptr.numel() - 1
+    x, res = O.seeded_normal((B, H), 3, device=DEV), O.seeded_normal((B, H), 4, device=DEV)
+    out, res_out = torch.empty_like(x), torch.empty_like(x)
+    ptr = [torch.tensor([p.data_ptr()], dtype=torch.int64, device=DEV) for p in pools.pools]
+    cf.llama_decoder_layer_batch_decode_sglang(out, res_out, x, res, w["wqkv"], w["wo"], indptr, indices, *ptr, 0, w["g"], 1e-5, positions, w["cs"])
+    return x, res, out
+
+
+def close_to_lists(w, pools, x, res, out, lists, positions):
+    """`lists`: for every sequence the history rows that are there; a row of the pool stands in for the new token's (its content is not read)."""
+    indptr, indices = [0], []
+    for rows in lists:
+        indices += rows + [0]
+        indptr.append(len(indices))
+    ref = LO.llama_attn_block_batch_fp32(x, res, w["wqkv"], w["wo"], *pools.start, ints(indptr), ints(indices), positions, w["cs"], w["g"], 1e-5)[0]
+    mx, rl = O.compare(out, ref)
+    assert mx <= 2e-2 and rl <= 1e-3, (mx, rl)
+
+
+def test_paged_block_with_an_empty_list(cuda_device, llama):
+    """A request without tokens owns no row: nothing is stored for it, least of all over the last row of the request before it."""
+    pools = Pools(300)
+    rows = list(range(10, 51)), list(range(100, 230))
+    positions = torch.tensor([40, 0, 129], device=DEV)
+    x, res, out = run_block(llama, pools, ints([0, 41, 41, 171]), ints(rows[0] + rows[1]), positions)
+    assert pools.only([50, 229])
+    close_to_lists(llama, pools, x, res, out, [rows[0][:-1], [], rows[1][:-1]], positions)
+
+
+@pytest.mark.parametrize("batch", [1, 5, 16])
+def test_paged_block_with_the_lists_of_a_plan_that_did_not_fit(cuda_device, llama, batch):
+    import clusterfusionplus_b200 as cf
+    pools = Pools(64)
+    p = cf.paged_kv_plan(ints([16] * batch), ints([1] * batch), torch.zeros(batch, 4, dtype=torch.int32, device=DEV), ints([1]), ints([0]), 16, batch, 32 * batch)
+    assert int(p.status) != 0
+    x, res, out = run_block(llama, pools, p.kv_indptr.clone(), p.kv_indices.clone(), p.positions)
+    assert pools.only([])
+    close_to_lists(llama, pools, x, res, out, [[]] * batch, p.positions)
+
+
+def test_paged_block_leaves_out_entries_below_zero(cuda_device, llama):
+    """Pages that were never given: their rows are not read and not written, and the call says so."""
+    import clusterfusionplus_b200 as cf
+    pools = Pools(400)
+    lists = [list(range(0, 200)), list(range(200, 209)), list(range(300, 340)), list(range(360, 380))]
+    lists[0][3], lists[0][128:140], lists[0][199] = -1, [-1] * 12, 395          # inside a tile, across its border
+    lists[1][-1] = -1                                                           # the new token's own row
+    lists[2][:-1] = [-1] * 39                                                   # the whole history
+    lists[3][0] = -2147483648
+    positions = torch.tensor([len(x) - 1 for x in lists], device=DEV)
+    starts = [0]
+    for rows in lists:
+        starts.append(starts[-1] + len(rows))
+    x, res, out = run_block(llama, pools, ints(starts), ints(sum(lists, [])), positions)
+    with pytest.raises(RuntimeError, match="status 8"):
+        cf.device_status()
+    assert pools.only([395, 339, 379])
+    close_to_lists(llama, pools, x, res, out, [[r for r in rows[:-1] if r >= 0] for rows in lists], positions)
