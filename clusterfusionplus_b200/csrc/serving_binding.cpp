@@ -173,8 +173,9 @@ PyObject* py_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
         at::Tensor r[8];
         {
             Aside aside;
-            // one allocation: rows (16-byte aligned), slots, lengths, both indptr arrays, count, status
-            const int64_t slots = (max_rows + 3) / 4 * 4, lens = slots + max_tokens, qo = lens + batch, kv = qo + batch + 1, left = kv + batch + 1, status = left + 1;
+            // one allocation, each piece 16-byte aligned (as the calls that read them ask): rows, slots, lengths, both indptr arrays, count, status
+            auto after = [](int64_t at, int64_t n) { return at + (n + 3) / 4 * 4; };
+            const int64_t slots = after(0, max_rows), lens = after(slots, max_tokens), qo = after(lens, batch), kv = after(qo, batch + 1), left = after(kv, batch + 1), status = after(left, 1);
             const at::Tensor buf = empty({status + 1}, cached, at::kInt), positions = empty({max_tokens}, cached, at::kLong);
             int* p = buf.data_ptr<int>();
             check(cf.plan(cached.data_ptr<int>(), fresh.data_ptr<int>(), batch, table.data_ptr<int>(), width, apart, free_pages.data_ptr<int>(), free_pages.numel(), count.data_ptr<int>(), p + left,

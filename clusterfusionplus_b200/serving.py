@@ -9,8 +9,11 @@ One step of a server, all of it on the GPU and capturable (nothing is read back 
     ...
     scored = cf.token_logprobs(logits, tokens, top_k=5)
 
-The lists of a plan made with max_rows are what llama_decoder_layer_batch_decode_sglang takes as paged_kv_indptr,
-paged_kv_indices and positions.  The reference's batched entry point (include/pybind.cpp:90-106) leaves all of this to its
+A plan made with max_rows and max_tokens = batch, in which every request gets one token, is what llama_decoder_layer_batch_decode_sglang
+takes: kv_indptr, kv_indices and positions as they are.  That block always writes one token a request, to the last row of its list, so a request
+that gets no token in a step must hold none (cached 0: its list is empty and nothing is written) or be left out of the plan.  With
+such idle requests positions, which has one entry a token, is not one a request: pass (plan.kv_lens - 1).clamp(min=0).long().  Of a plan that
+did not fit the block writes nothing either.  The reference's batched entry point (include/pybind.cpp:90-106) leaves all of this to its
 caller.  Like the rest of the package these functions validate, allocate their results and launch on torch's current stream.
 """
 from __future__ import annotations
@@ -48,7 +51,8 @@ def paged_kv_plan(cached_lens, new_lens, block_table, free_pages, free_count, pa
     rows of all requests are listed too (kv_indices), the form that llama_decoder_layer_batch_decode_sglang reads.
 
     All or nothing: if the pages, the table's columns, max_tokens or max_rows do not suffice, or a length is negative, nothing
-    changes, the lists come back empty and status[0] holds CF_PLAN_* bits.  Read it where the host waits anyway."""
+    changes, the lists come back empty and status[0] holds CF_PLAN_* bits.  Read it where the host waits anyway.  The results share one
+    allocation: keeping one of them keeps all."""
     return PagedKvPlan._make(_call.plan(cached_lens, new_lens, block_table, free_pages, free_count, page_size, max_tokens, max_rows))
 
 

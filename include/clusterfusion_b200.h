@@ -425,7 +425,8 @@ int cf_prefill_rope_split(const void* qkv, const float* cos, const float* sin, v
  *   positions    int64 [max_tokens], slot_map int32 [max_tokens]: position in its request and row in the cache of every
  *                new token (row = page * page_size + position % page_size); behind the last token 0 and -1
  *   kv_indptr    int32 [batch + 1], kv_indices int32 [max_rows]: the cache rows of every request, all cached + new of them,
- *                as cf_llama_decoder_layer_batch_sglang reads them; behind the last row -1.  max_rows = 0: only kv_indptr.
+ *                as cf_llama_decoder_layer_batch_sglang reads them (that block writes one token a request, to the last row of its
+ *                list: give every request one, or let it hold none); behind the last row -1.  max_rows = 0: only kv_indptr.
  *                kv_indices must be 16-byte aligned.
  *   *status      0, or CF_PLAN_* bits.  All or nothing: with a bit set the table and the count stay as they are, kv_lens =
  *                cached_lens, the indptr arrays are 0 and the lists empty (0 / -1).

@@ -113,3 +113,34 @@ def test_paged_block_leaves_out_entries_below_zero(cuda_device, llama):
         cf.device_status()
     assert pools.only([395, 339, 379])
     close_to_lists(llama, pools, x, res, out, [[r for r in rows[:-1] if r >= 0] for rows in lists], positions)
+
+
+@pytest.mark.parametrize("batch", list(range(1, 17)))
+def test_plan_goes_into_the_paged_block_as_it_is(cuda_device, llama, batch):
+    """kv_indptr, kv_indices and positions of a plan, not copied, for every batch of the block; the same as from tensors of their own."""
+    import clusterfusionplus_b200 as cf
+    rng = random.Random(batch)
+    lens = [rng.choice([0, 15, 16, rng.randint(1, 60)]) for _ in range(batch)]
+    ids = list(range(5 * batch))
+    rng.shuffle(ids)
+    table = [[ids.pop() if i * 16 < n else -1 for i in range(4)] for n in lens]
+    p = cf.paged_kv_plan(ints(lens), ints([1] * batch), ints(table), ints(ids), ints([len(ids)]), 16, batch, sum(lens) + batch + 3)
+    assert int(p.status) == 0
+    pools = [Pools(80 * batch) for _ in range(2)]
+    *_, one = run_block(llama, pools[0], p.kv_indptr, p.kv_indices, p.positions)
+    *_, two = run_block(llama, pools[1], p.kv_indptr.clone(), p.kv_indices.clone(), ints(lens).long())
+    assert torch.equal(one, two) and all(torch.equal(a, b) for a, b in zip(pools[0].room, pools[1].room))
+    assert pools[0].only(p.slot_map.tolist())
+
+
+def test_plan_with_idle_requests_goes_into_the_paged_block(cuda_device, llama):
+    """Places of a batch that hold no request: no page, no row, no position of their own in `positions`."""
+    import clusterfusionplus_b200 as cf
+    lens, new = [0, 31, 0, 16], [0, 1, 0, 1]
+    p = cf.paged_kv_plan(ints(lens), ints(new), ints([[-1] * 3, [5, 2, -1], [-1] * 3, [0, -1, -1]]), ints([9, 7]), ints([2]), 16, 4, 64)
+    assert int(p.status) == 0 and p.slot_map.tolist() == [47, 7 * 16, -1, -1]
+    pools, positions = Pools(192), (p.kv_lens - 1).clamp(min=0).long()
+    x, res, out = run_block(llama, pools, p.kv_indptr, p.kv_indices, positions)
+    assert pools.only([47, 112])
+    rows = p.kv_indices.tolist()
+    close_to_lists(llama, pools, x, res, out, [[], rows[:31], [], rows[32:48]], positions)
