@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(PT) paged_kv_plan_kernel(const PlanArgs a) {
     const int tid = threadIdx.x, per = (a.batch + PT - 1) / PT;
     const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
     if (tid == 0) s_bits = 0;
-    const long long avail = min(static_cast<long long>(max(*a.free_count, 0)), a.n_free);
+    const long long avail = *a.free_count;
     Sums mine = {0, 0, 0};
     int bits = 0;
     for (int b = b0; b < b1; ++b) {
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(PT) paged_kv_plan_kernel(const PlanArgs a) {
     Sums all;
     const Sums before = block_exclusive(mine, &all, buf);  // its barrier also orders s_bits
     bits = s_bits;
-    if (all.pages > avail) bits |= CF_PLAN_NO_PAGES;
+    if (avail < 0 || avail > a.n_free || all.pages > avail) bits |= CF_PLAN_NO_PAGES;  // a count that the list cannot have says nothing about which entries are free
     if (all.tokens > a.max_tokens) bits |= CF_PLAN_MAX_TOKENS;
     if (a.max_rows > 0 ? all.rows > a.max_rows : all.rows > 0x7fffffffll) bits |= CF_PLAN_MAX_ROWS;
     const bool ok = bits == 0;  // all or nothing: a step that does not fit changes no table and deals out nothing
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(PT) paged_kv_plan_kernel(const PlanArgs a) {
             if (b < a.batch) a.kv_lens[b] = a.cached[b] + (ok ? a.fresh[b] : 0);
         }
         if (tid == 0) {
-            *a.free_count_out = *a.free_count - (ok ? static_cast<int>(all.pages) : 0);
+            *a.free_count_out = static_cast<int>(avail - (ok ? all.pages : 0));
             *a.status = bits;
         }
         if (ok)

@@ -50,8 +50,8 @@ def paged_kv_plan(cached_lens, new_lens, block_table, free_pages, free_count, pa
     pass it, and the result's kv_lens as cached_lens, to the next step.  max_tokens bounds the new tokens of the step; with max_rows > 0 the cache
     rows of all requests are listed too (kv_indices), the form that llama_decoder_layer_batch_decode_sglang reads.
 
-    All or nothing: if the pages, the table's columns, max_tokens or max_rows do not suffice, or a length is negative, nothing
-    changes, the lists come back empty and status[0] holds CF_PLAN_* bits.  Read it where the host waits anyway.  The results share one
+    All or nothing: if the pages, the table's columns, max_tokens or max_rows do not suffice, a length is negative, or free_count is not one
+    that free_pages can have, nothing changes, the lists come back empty and status[0] holds CF_PLAN_* bits.  Read it where the host waits anyway.  The results share one
     allocation: keeping one of them keeps all."""
     return PagedKvPlan._make(_call.plan(cached_lens, new_lens, block_table, free_pages, free_count, page_size, max_tokens, max_rows))
 

@@ -408,7 +408,7 @@ int cf_prefill_rope_split(const void* qkv, const float* cos, const float* sin, v
 #define CF_DTYPE_FP32 2
 
 /* Bits of the status word of a plan or a release. */
-#define CF_PLAN_NO_PAGES 1     /* plan: the free list holds too few pages; release: it has no room */
+#define CF_PLAN_NO_PAGES 1     /* plan: the free list holds too few pages; release: it has no room; both: *free_count is not 0 .. n_free_pages */
 #define CF_PLAN_TABLE_WIDTH 2  /* a request needs more pages than the block table has columns */
 #define CF_PLAN_MAX_TOKENS 4   /* more new tokens than max_tokens */
 #define CF_PLAN_MAX_ROWS 8     /* more cached rows than max_rows (max_rows = 0: than 2^31 - 1) */

@@ -24,8 +24,8 @@ def plan(cached, new, table, free, count, page, max_tokens, max_rows):
     have = [pages(c) if g else 0 for c, g in zip(cached, good)]
     if any(n > width for n in need):
         status |= 2
-    avail = min(max(count, 0), len(free))
-    if sum(need) - sum(have) > avail:
+    avail = count
+    if not 0 <= count <= len(free) or sum(need) - sum(have) > avail:
         status |= 1
     if sum(n for n, g in zip(new, good) if g) > max_tokens:
         status |= 4

@@ -196,6 +196,12 @@ def test_plan_of_the_oracle():
     assert full["status"] == 1 + 4 + 8 and full["table"][0] == [7, -1] and full["kv_lens"] == [16, 0, 5] and full["free_count"] == 1
 
 
+@pytest.mark.parametrize("count", [4, 90, -1])
+def test_plan_of_the_oracle_refuses_a_count_beyond_the_list(count):
+    got = S.plan([0], [0], [[-1]], [9, 8, 7], count, 16, 4, 0)
+    assert got["status"] == 1 and got["free_count"] == count and got["table"] == [[-1]]
+
+
 def test_logprobs_of_the_oracle():
     x = torch.tensor([[0.0, math.log(3.0), -math.inf, math.log(3.0)]])
     lp, h, tl, ti = S.logprobs(x, [1], 3)

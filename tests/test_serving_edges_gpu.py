@@ -144,3 +144,28 @@ def test_plan_with_idle_requests_goes_into_the_paged_block(cuda_device, llama):
     assert pools.only([47, 112])
     rows = p.kv_indices.tolist()
     close_to_lists(llama, pools, x, res, out, [[], rows[:31], [], rows[32:48]], positions)
+
+
+# ------------------------------------------------------------------------------------------------------------ the free list
+@pytest.mark.parametrize("count", [10, 4, 2147483647, -1])
+def test_plan_refuses_a_count_that_the_list_cannot_have(cuda_device, count):
+    """Two steps from a count beyond the list would deal the same pages out twice; release refuses such a count too."""
+    import clusterfusionplus_b200 as cf
+    table, free, n, lens = ints([[-1] * 2, [-1] * 2]), ints([9, 8, 7]), ints([count]), ints([0, 0])
+    for new in ([16, 0], [0, 16], [0, 0]):
+        p = cf.paged_kv_plan(lens, ints(new), table, free, n, 16, 16)
+        assert int(p.status) == 1 and int(p.free_count) == count and (table == -1).all() and (p.slot_map == -1).all() and p.kv_lens.tolist() == [0, 0]
+    _, status = cf.paged_kv_release(ints([0, 0]), lens, table, free, n, 16)
+    assert int(status) == 1
+
+
+def test_plans_of_several_steps_deal_no_page_out_twice(cuda_device):
+    import clusterfusionplus_b200 as cf
+    table, free, n, lens = torch.full((4, 8), -1, dtype=torch.int32, device=DEV), torch.randperm(32, device=DEV).int(), ints([32]), ints([0] * 4)
+    for _ in range(8):
+        p = cf.paged_kv_plan(lens, ints([16] * 4), table, free, n, 16, 64)
+        assert int(p.status) == 0
+        lens, n = p.kv_lens, p.free_count
+    assert sorted(table.flatten().tolist()) == list(range(32)) and int(n) == 0
+    p = cf.paged_kv_plan(lens, ints([0, 0, 0, 1]), table, free, n, 16, 64)
+    assert int(p.status) == 1 + 2
