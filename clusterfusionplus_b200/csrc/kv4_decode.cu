@@ -14,11 +14,13 @@
 //    fp16, transposed, and multiplied by the groups' scales two tokens at a time, q = p s (a second rounding).  One more instruction takes the
 //    minima and a row of ones times the same P: sum p m of every group and the softmax's denominator, fp32 sums of the P that the
 //    numerators use.  The codes are not centred, so the rounding of q would weigh up to 15 of its steps where the values spread
-//    over +-8: 8 (p s - q), which is exact in fp16, goes to the group's sum as well, and what is left of the error is q's times c - 8.
+//    over +-8: 8 (p s - q), which fp16 holds to 2^-25, goes to the group's sum as well, and what is left of the error is q's times c - 8.
 // Queries are scaled by a power of two to at most 2^10 before they become fp16: exact for fp16 and bf16 inputs of any size
-// down to 2^-20 of their row's largest, off by less than 2^-30 of it below.  Probabilities are kept within (0, 4] (the running maximum is
-// two binary steps low) so that their product with a scale of up to 8734 (the widest fp16 range / 15) fits fp16 and small
-// scales keep their bits.
+// down to 2^-20 of their row's largest, off by less than 2^-30 of it below.  Both p and q = p s have to stay among fp16's normal numbers: a
+// token far below the maximum may still carry the result where the maximum's value is next to nothing, and scales of 2^-8 are usual.  So p
+// is kept as large as the scales allow, up to 2^13 with scales up to 4, and lower only once a warp meets larger ones (up to 8734, the widest
+// fp16 range / 15): p s <= 2^15 always.  With p <= 4 whatever the scales, values of std 0.005 beside a token 10 nats above
+// them were off by 7e-3, where the rounding of bf16 results is 1.7e-3.  It costs 1 % of the line's time.
 //
 // Two ways to deal out the work, both without a wait between CTAs and with the same bits every time:
 //  - little work: a cluster of up to 8 CTAs takes a (request, cached head), its tiles go round the warps, the partial results meet in
@@ -256,7 +258,9 @@ template <int G, int NT> struct Acc {
     static constexpr int DP = 32 * G, LINE = DP + 4;
     float o[NT][2 * G][4];  // numerators in units of 2^-24 and 2^-20
     float low[NT][4];       // row g: group g's sum of p times the minimum; row G: the sum of p
-    float m[NT][2];         // reference of a column: p = 2^(score - m), at most 4
+    float m[NT][2];         // reference of a column: p = 2^(score - m), at most 2^room
+    float room;
+    uint32_t wide;          // 2^(15 - room) twice, fp16: no scale of a token that some row sees is larger
     bool first_tile;
 
     __device__ __forceinline__ void reset() {
@@ -271,10 +275,29 @@ template <int G, int NT> struct Acc {
             m[nt][0] = m[nt][1] = 0.f;
         }
         first_tile = true;
+        room = 13.f, wide = 0x44004400u;
     }
+    template <int K> __device__ __forceinline__ void make_room(const uint32_t (&scales)[K]);
     template <int K> __device__ __forceinline__ void step(const int (&tile)[K], int token, const Rows<G, NT>& r, int lane);
     __device__ __forceinline__ void store(float* lines) const;
 };
+
+// scales beyond `wide` among the warp's: room for the greatest of them (one that is not finite makes its group NaN anyway)
+template <int G, int NT>
+template <int K>
+__device__ __forceinline__ void Acc<G, NT>::make_room(const uint32_t (&scales)[K]) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int u = 0; u < K; ++u) {
+        const uint32_t x = scales[u] & finite_halves(scales[u]) & 0x7fff7fffu;
+        most = max(most, max(x & 0xffffu, x >> 16));
+    }
+    const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 10) - 14;  // the greatest is below 2^e
+    if (e > 15 - static_cast<int>(room)) {
+        room = static_cast<float>(15 - e);
+        wide = static_cast<uint32_t>(e + 15) * 0x04000400u;  // (2^16 is infinity: nothing lies beyond)
+    }
+}
 
 // K tiles of 16 tokens in a row, the first token of all `token`, the tiles at these offsets of shared memory
 template <int G, int NT>
@@ -329,10 +352,23 @@ __device__ __forceinline__ void Acc<G, NT>::step(const int (&tile)[K], int token
             }
         }
     }
-    // ---- softmax: x becomes the binary logarithm of p.  The reference is set so that the greatest p is 2 and moves when one exceeds 4: seldom
-    // after the first tiles.  (Lower would move less often, but p times a small scale would leave the range of normal fp16 numbers sooner.)
+    // ---- softmax: x becomes the binary logarithm of p.  The reference is set so that the greatest p is a quarter of the most and moves when one
+    // exceeds that: seldom after the first tiles.  Each lane looks at one token's scales (two groups of four), whose greatest decides how much
+    // p may be; tokens that no row sees do not count.
     const bool whole = token + K * KV4_TILE - 1 <= r.all_see;
     bool rise = first_tile;
+    uint32_t scales[K];
+#pragma unroll
+    for (int u = 0; u < K; ++u) {
+        const int row = G == 4 ? lane >> 1 : lane & 15;
+        const uint32_t at = tile[u] + 512 * G + row * 8 * G + 4 * G;
+        if constexpr (G == 4) scales[u] = load_word(at + (lane & 1) * 4);
+        else if constexpr (G == 1) scales[u] = load_half(at);
+        else if constexpr (G == 2) scales[u] = load_word(at);
+        else scales[u] = lane < 16 ? load_word(at) : load_half(at + 4);
+        if (!whole && token + u * KV4_TILE + row > r.most) scales[u] = 0;
+        rise |= !__hble2(__habs2(*reinterpret_cast<const __half2*>(&scales[u])), *reinterpret_cast<const __half2*>(&wide));
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -352,9 +388,10 @@ __device__ __forceinline__ void Acc<G, NT>::step(const int (&tile)[K], int token
     for (int nt = 0; nt < NT; ++nt) {
         float top = fmaxf(fmaxf(x[0][nt][0], x[0][nt][2]), fmaxf(x[0][nt][1], x[0][nt][3]));
         if constexpr (K == 2) top = fmaxf(top, fmaxf(fmaxf(x[K - 1][nt][0], x[K - 1][nt][2]), fmaxf(x[K - 1][nt][1], x[K - 1][nt][3])));
-        rise |= top > 2.f;
+        rise |= top > room;
     }
     if (__any_sync(0xffffffffu, rise)) {
+        make_room(scales);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -364,7 +401,7 @@ __device__ __forceinline__ void Acc<G, NT>::step(const int (&tile)[K], int token
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
                 // a column's first tiles set its reference; one that sees nothing of them sees nothing of later ones
-                const float up = (first_tile || top > 2.f) && top != -INFINITY ? top - 1.f : 0.f;
+                const float up = (first_tile || top > room) && top != -INFINITY ? top - (room - 2.f) : 0.f;
                 m[nt][c] += up;
 #pragma unroll
                 for (int u = 0; u < K; ++u) x[u][nt][c] -= up, x[u][nt][c + 2] -= up;

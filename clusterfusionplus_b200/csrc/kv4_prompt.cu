@@ -9,7 +9,7 @@
 //    value: the operands' type; scores and sums stay fp32).  Keys as rows of dims, values as rows of tokens, which is how the cache's
 //    words hold them: two neighbouring tokens in the halves of a word are two neighbouring elements of a row of V^T.
 //  - 8 warps do the softmax, two threads a query row, in one pass over a tile's scores.  The reference of a row moves only when a score
-//    lies more than 8 binary steps above it, which after a row's first tile hardly ever happens: then the accumulator in tensor
+//    lies more than 8 binary steps above the greatest before it, which after a row's first tile hardly ever happens: then the accumulator in tensor
 //    memory is rescaled and the pass repeated.
 //  - 1 thread issues the products: S of the next tile before P V of this one, so that they run under the softmax.
 // Every wait is bounded; one that runs out ends the kernel with a device status.
@@ -38,7 +38,9 @@ constexpr int KEYS = 128;            // tokens of a tile
 constexpr int SOFT = 8, UNPACK = 8;  // warps; one more issues the products
 constexpr int THREADS = 32 * (SOFT + UNPACK + 1);
 constexpr int BLOCK = 128 * 128;     // bytes of a K-major operand block of 128 rows x 64 elements
-constexpr float SLACK = 8.f;         // binary steps that a score may lie above its row's reference
+// A row's reference is set so that its greatest p is 2^HIGH, and moves when one exceeds 2^SLACK: p is an fp16 operand, and what lies far below the
+// maximum keeps its bits (normal numbers down to 2^-14) the longer the higher the maximum stands
+constexpr float HIGH = 7.f, SLACK = 15.f;
 
 // ------------------------------------------------------------------------------------------------ tensor cores
 __device__ __forceinline__ uint64_t operand(uint32_t saddr) {  // K-major, 128-byte swizzle: rows of 128 bytes, groups of 8 rows 1024 bytes apart
@@ -350,7 +352,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                             l += both.x + both.y;
                             break;
                         }
-                        const float by = move ? high : 0.f, keep = set ? ex2(-by) : 1.f;
+                        const float by = move ? high - HIGH : 0.f, keep = set ? ex2(-by) : 1.f;
                         m += by;
                         l *= keep;
                         set |= move;

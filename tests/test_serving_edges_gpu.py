@@ -169,3 +169,74 @@ def test_plans_of_several_steps_deal_no_page_out_twice(cuda_device):
     assert sorted(table.flatten().tolist()) == list(range(32)) and int(n) == 0
     p = cf.paged_kv_plan(lens, ints([0, 0, 0, 1]), table, free, n, 16, 64)
     assert int(p.status) == 1 + 2
+
+
+# ----------------------------------------------------------------------------------------------------------- attention's range
+@pytest.fixture(params=["by_size", "line", "prompt"])
+def schedule(request, monkeypatch):
+    """Clusters or what the sizes choose, the line of tiles with a workspace, 128 rows at a time on the tensor cores (a large hint asks for it)."""
+    import clusterfusionplus_b200 as cf
+    from clusterfusionplus_b200 import serving
+    if request.param == "line":
+        monkeypatch.setattr(serving, "_workspace", 64 << 20)
+    if request.param == "prompt":
+        plain = cf.kv4_attention
+        monkeypatch.setattr(cf, "kv4_attention", lambda *a, **k: plain(*a, **(k | {"max_q_len": 4096})))
+
+
+def near(got, ref):
+    """rel-L2 of the roundings that the kernels are allowed (probabilities, operands and results once each): 1e-3 for fp16 results, 2.5e-3 for bf16;
+    fp16 results below its normal range are off by half a step of 2^-24 besides."""
+    err = (got.double().cpu() - ref).norm()
+    tol = (1e-3 if got.dtype == torch.float16 else 2.5e-3) * ref.norm() + (2.0 ** -25 * math.sqrt(ref.numel()) if got.dtype == torch.float16 else 0.0)
+    assert err <= tol, (err / ref.norm()).item()
+
+
+def sink_case(count, T, D, dtype, gap, std, at, seed=1):
+    """Rows whose token `at` stands `gap` nats above the middle of the others and has next to no value."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    base = torch.randn(2, D, device=DEV, generator=g)                                   # a direction for each cached head
+    q = base.repeat_interleave(2, 0)[None] + 0.05 * torch.randn(count, 4, D, device=DEV, generator=g)
+    key = torch.randn(T, 2, D, device=DEV, generator=g)
+    value = torch.randn(T, 2, D, device=DEV, generator=g) * std
+    key[at] = base * (gap * D ** 0.5) / (base * base).sum(-1, keepdim=True)
+    value[at] *= 0.02 if gap < 12 else 0.0
+    return q.to(dtype), key.to(dtype), value.to(dtype)
+
+
+@pytest.mark.parametrize("dtype,std", [(torch.bfloat16, 0.005), (torch.bfloat16, 0.02), (torch.float16, 0.02), (torch.float16, 0.1)])
+@pytest.mark.parametrize("gap", [0.0, 7.0, 10.0, 14.0])
+@pytest.mark.parametrize("count,at", [(1, 0), (1, 1234), (6, 0), (40, 3)])
+def test_attention_with_one_dominant_token_of_little_value(cuda_device, schedule, dtype, std, gap, count, at):
+    """What the other tokens give has to keep its precision: small probabilities times small scales."""
+    import clusterfusionplus_b200 as cf
+    T, D = 2000, 128
+    q, key, value = sink_case(count, T, D, dtype, gap, std, at)
+    cache = cf.kv4_cache(125, 2, 16, D)
+    cf.kv4_append(key, value, ints(list(range(T))), cache)
+    K, V = S.unpack(cache, D)
+    table = [list(range(125))]
+    got = cf.kv4_attention(q, cache, ints(table), ints([T]), ints([0, count]), max_q_len=count)
+    near(got, S.attention(q, K, V, table, [T], [0, count], D ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("count", [1, 3, 40])
+def test_attention_of_values_of_all_sizes_in_one_request(cuda_device, schedule, dtype, D, count):
+    """Tokens and groups whose scales differ by many binary orders, small ones first: fp16's largest among them, behind the last token too."""
+    import clusterfusionplus_b200 as cf
+    T = 700
+    g = torch.Generator(device=DEV).manual_seed(D + count)
+    q, key = (torch.randn(n, h, D, device=DEV, generator=g).to(dtype) for n, h in ((count, 4), (T + 20, 2)))
+    size = torch.exp2(torch.randint(-6, 14, (T + 20, 1, 1), device=DEV, generator=g).float())
+    size[:300] = 2.0 ** -6
+    size[T:] = 2.0 ** 13
+    value = (torch.randn(T + 20, 2, D, device=DEV, generator=g) * size).clamp(-30000, 30000).to(dtype)
+    cache = cf.kv4_cache(45, 2, 16, D)
+    cf.kv4_append(key, value, ints(list(range(T + 20))), cache)
+    K, V = S.unpack(cache, D)
+    table = [list(range(45))]
+    for n in (T, 290):
+        got = cf.kv4_attention(q, cache, ints(table), ints([n]), ints([0, count]), max_q_len=count)
+        near(got, S.attention(q, K, V, table, [n], [0, count], D ** -0.5))
