@@ -1,7 +1,8 @@
 // The paged cache held in 4 bits (layout: kv4_layout.cuh): rows written at their slots and read back, and the C entry
 // points.  Asymmetric 4-bit codes over groups of 32 values of one token and head:
 //   m = fp16(min x), s = fp16((max x - m) / 15), code = clamp(rint((x - m) / s), 0, 15), value = code * s + m
-// x in fp32 (clamped to fp16's range, which bf16 exceeds); the codes are computed against the rounded s and m, so the rounding of
+// A scale that was rounded up so far that m + 15 s would lie beyond fp16's largest number is stored one step lower: whatever reads
+// the row, in fp16 or not, gets the same finite values.  x in fp32 (clamped to fp16's range, which bf16 exceeds); the codes are computed against the rounded s and m, so the rounding of
 // the parameters costs no accuracy but the last step's.  A group that is constant has s = 0 and code 0; one that holds a
 // NaN or whose extremes are not finite in the input stores NaN as its scale: it comes back as NaN instead of as numbers.
 #include <cuda_bf16.h>
@@ -93,7 +94,8 @@ template <class T> __device__ __forceinline__ unsigned quantise8(const uint32_t 
     // x / 15 correctly rounded: the product with the rounded 1 / 15, corrected by its residual, which is exact in a fused multiply-add (where
     // that would fall below fp32's range the quotient is far below fp16's)
     const float x15 = end.x - mf, near = x15 * (1.f / 15.f);
-    const __half s = __float2half_rn(fmaf(fmaf(-15.f, near, x15), 1.f / 15.f, near));
+    __half s = __float2half_rn(fmaf(fmaf(-15.f, near, x15), 1.f / 15.f, near));
+    if (fmaf(15.f, __half2float(s), mf) > 65504.f) s = __ushort_as_half(static_cast<unsigned short>(__half_as_ushort(s) - 1));
     const float sf = __half2float(s);
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(sf));
@@ -120,7 +122,7 @@ template <class T> __device__ __forceinline__ unsigned quantise8(const uint32_t 
                 c[i] = Pair(rintf((fminf(fmaxf(v.x, -65504.f), 65504.f) - mf) / sf), rintf((fminf(fmaxf(v.y, -65504.f), 65504.f) - mf) / sf));
             }
         }
-        // No value is more than half a step below the minimum.  Above, a normal scale is at most 2^-11 too small (15.008 steps); one rounded to
+        // No value is more than half a step below the minimum.  Above, a normal scale is at most 2^-10 too small (15.015 steps); one rounded to
         // fp16's last steps reaches beyond 15.
         if (sf < 6.103515625e-5f) {
 #pragma unroll

@@ -55,7 +55,8 @@ template <class T> __device__ __forceinline__ float2 to_float2(uint32_t v);
 template <> __device__ __forceinline__ float2 to_float2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 template <> __device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
 template <class T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+// (a result is a mean of values within fp16's range: what the sums' rounding puts beyond it is not infinity; NaN stays)
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v > 65504.f ? 65504.f : v < -65504.f ? -65504.f : v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // e in -126 .. 127

@@ -105,7 +105,11 @@ template <class T> __device__ __forceinline__ float2 to_float2(uint32_t v);
 template <> __device__ __forceinline__ float2 to_float2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 template <> __device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
 template <class T> __device__ __forceinline__ uint32_t pack(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) { return pack_half2(a, b); }
+// (a result is a mean of values within fp16's range: what the sums' rounding puts beyond it is not infinity; NaN stays)
+template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
+    auto held = [](float x) { return x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x; };
+    return pack_half2(held(a), held(b));
+}
 template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
@@ -128,10 +132,6 @@ __device__ __forceinline__ void code_pairs(uint32_t w, __half2 (&c)[4]) {
     c[1] = __hsub2(as_half2(select_or(w, 0x00f000f0u, 0x54005400u)), k64);
     c[2] = __hsub2(as_half2(select_or(h, 0x000f000fu, 0x64006400u)), k1024);
     c[3] = __hsub2(as_half2(select_or(h, 0x00f000f0u, 0x54005400u)), k64);
-}
-// A scale whose largest value minimum + 15 scale would round beyond fp16 (the scale was rounded up at the end of the range): one step lower
-__device__ __forceinline__ uint32_t within_range(uint32_t s, uint32_t m) {
-    return fmaf(15.f, __half2float(__ushort_as_half(static_cast<unsigned short>(s))), __half2float(__ushort_as_half(static_cast<unsigned short>(m)))) > 65504.f ? s - 1 : s;
 }
 __device__ __forceinline__ bool finite_half(uint32_t x) { return (x & 0x7c00u) != 0x7c00u; }
 
@@ -489,9 +489,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                     if (g0 + k < G) {
                         const bool seen = token0 + row <= end, fine = finite_half(par[2][k]) && finite_half(par[3][k]);
                         if (seen && !fine) sh.not_finite = 1;
-                        sh.kpar[part][row][g0 + k] = static_cast<uint16_t>(within_range(par[0][k], par[1][k]));
+                        sh.kpar[part][row][g0 + k] = static_cast<uint16_t>(par[0][k]);
                         sh.kpar[part][row][4 + g0 + k] = static_cast<uint16_t>(par[1][k]);
-                        sh.vpar[part][0][g0 + k][row] = static_cast<uint16_t>(seen && fine ? within_range(par[2][k], par[3][k]) : 0u);
+                        sh.vpar[part][0][g0 + k][row] = static_cast<uint16_t>(seen && fine ? par[2][k] : 0u);
                         sh.vpar[part][1][g0 + k][row] = static_cast<uint16_t>(seen && fine ? par[3][k] : 0u);
                     }
                 }

@@ -447,7 +447,8 @@ int cf_paged_kv_release(const int* finished, const int* kv_lens, int64_t batch, 
 /* The paged cache held in 4 bits: uint8 [pages][kv_heads][page_size][40 * G], G = ceil(head_dim / 32), page_size a multiple
  * of 16, head_dim a multiple of 8 in 16..128, at most 2^31 - 1 rows, 16-byte aligned.  Every 32 values of one token and head
  * (the last group of a head may be shorter) share an fp16 minimum m and an fp16 scale s = (max - m) / 15; a value is
- * code * s + m with code = rint((x - m) / s) in 0..15 (x clamped to fp16's range; a group holding a NaN or an infinity reads
+ * code * s + m with code = rint((x - m) / s) in 0..15 (x clamped to fp16's range, s one step lower where m + 15 s would lie
+ * beyond it; a group holding a NaN or an infinity reads
  * back as NaN).  The order of the codes inside a page is described in csrc/kv4_layout.cuh.  Row r of the cache is token
  * r % page_size of page r / page_size.
  *

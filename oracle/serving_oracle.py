@@ -75,6 +75,8 @@ def quantise(x):
             part = np.fmin(np.fmax(part, np.float32(-65504)), np.float32(65504))
             m = part.min(-1).astype(np.float16)
             s = ((part.max(-1) - m.astype(np.float32)) / np.float32(15)).astype(np.float16)
+            beyond = m.astype(np.float64) + 15 * s.astype(np.float64) > 65504   # the largest value would not be an fp16 number: one step lower
+            s = np.where(beyond, np.nextafter(s, np.float16(0)), s)
             c = np.rint((part - m.astype(np.float32)[..., None]) / s.astype(np.float32)[..., None])
         c = np.where((s[..., None] > 0) & ~bad[..., None], np.clip(np.nan_to_num(c), 0, 15), 0)
         codes[..., 32 * g:32 * g + 32] = c.astype(np.uint8)

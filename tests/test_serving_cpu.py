@@ -226,3 +226,14 @@ def test_random_plans_keep_every_page_once():
         got = S.plan(lens, new, table, ids, len(ids), page, 200, 0)
         used = [e for r in got["table"] for e in r if e >= 0]
         assert got["status"] == 0 and sorted(used + ids[:got["free_count"]]) == list(range(400))
+
+
+@pytest.mark.parametrize("lo,hi", [(0.0, 65504.0), (-65504.0, 65504.0), (-1.0, 65504.0), (-1e38, 1e38), (-30000.0, 65504.0), (60000.0, 65504.0)])
+def test_quantised_values_stay_within_fp16(lo, hi):
+    """m + 15 s is an fp16 number where s would round it beyond (0 .. 65504: s = 4368, 15 x 4368 = 65520), and no further off than half a step."""
+    x = np.linspace(lo, hi, 32).astype(np.float32)
+    c, s, m = S.quantise(x[None])
+    back = c[0] * s[0].astype(np.float64) + m[0].astype(np.float64)
+    assert np.abs(back).max() <= 65504 and c[0, 0] == 0 and c[0, -1] == 15
+    held = np.clip(x.astype(np.float64), -65504, 65504)
+    assert (np.abs(back - held) <= s.astype(np.float64)[0] * (0.5 + 15 * 2.0 ** -10)).all()

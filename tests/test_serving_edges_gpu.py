@@ -240,3 +240,60 @@ def test_attention_of_values_of_all_sizes_in_one_request(cuda_device, schedule, 
     for n in (T, 290):
         got = cf.kv4_attention(q, cache, ints(table), ints([n]), ints([0, count]), max_q_len=count)
         near(got, S.attention(q, K, V, table, [n], [0, count], D ** -0.5))
+
+
+# -------------------------------------------------------------------------------------------------------- the type's largest values
+def largest_rows(dtype, D):
+    """Groups from 0, from the middle and from the lowest number to fp16's largest; bf16 beyond it too."""
+    g = torch.Generator(device=DEV).manual_seed(D)
+    top = torch.finfo(torch.float16).max
+    x = torch.rand(32, 2, D, device=DEV, generator=g)
+    x[:8] = x[:8] * top
+    x[8:16] = (x[8:16] * 2 - 1) * top
+    x[16:24] = x[16:24] * 35000 + 30000
+    x[:24, :, 0::32], x[:24, :, 1::32] = top, -top
+    x[:8, :, 1::32] = 0
+    x[16:24, :, 1::32] = 30000
+    if dtype == torch.bfloat16:
+        x[24:28] = (x[24:28] * 2 - 1) * 1e38
+    x[28:] = top
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [32, 80, 128])
+def test_rows_of_the_largest_values_come_back_finite(cuda_device, dtype, D):
+    import numpy as np
+
+    import clusterfusionplus_b200 as cf
+    x = largest_rows(dtype, D)
+    cache, slots = cf.kv4_cache(2, 2, 16, D), list(range(32))
+    want = cache.cpu().numpy().copy()
+    for t in slots:
+        S.store(want, t, x[t].float().cpu().numpy(), x[t].float().cpu().numpy())
+    cf.kv4_append(x, x, ints(slots), cache)
+    assert np.array_equal(cache.cpu().numpy(), want)
+    ref = S.unpack(want, D)[0].transpose(1, 2).reshape(32, 2, D)
+    for out in (torch.float16, torch.bfloat16):
+        for got in cf.kv4_read(cache, ints(slots), D, out):
+            assert got.isfinite().all() and ((got.double().cpu() - ref).abs() <= (torch.finfo(out).eps / 2 + 2.0 ** -24) * ref.abs() + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [32, 80, 128])
+@pytest.mark.parametrize("count", [1, 5, 30])
+def test_attention_over_the_largest_values(cuda_device, schedule, dtype, D, count):
+    """The same finite values whatever the schedule; where all that a query sees is the largest number the result is it."""
+    import clusterfusionplus_b200 as cf
+    value = largest_rows(dtype, D)
+    g = torch.Generator(device=DEV).manual_seed(count)
+    q, key = torch.randn(count, 4, D, device=DEV, generator=g).to(dtype), torch.randn(32, 2, D, device=DEV, generator=g).to(dtype)
+    for rows, n in ((slice(0, 32), 32), (slice(28, 32), 4)):
+        cache = cf.kv4_cache(2, 2, 16, D)
+        cf.kv4_append(key[rows].contiguous(), value[rows].contiguous(), ints(list(range(n))), cache)
+        K, V = S.unpack(cache, D)
+        m = min(count, n)
+        got = cf.kv4_attention(q[:m], cache, ints([[0, 1]]), ints([n]), ints([0, m]), max_q_len=m)
+        ref = S.attention(q[:m], K, V, [[0, 1]], [n], [0, m], D ** -0.5)
+        assert got.isfinite().all()
+        near(got, ref)
