@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(LT, 8) token_logprobs_kernel(const LogprobArgs
         float hi, lo;
         extremes(raw, hi, lo, T());
         meet(hi, at);
-        if (lo < -1e37f) {  // masked by -inf or the lowest number
+        if (lo - st.m < -1e38f) {  // masked by -inf or the lowest number, or so far below the greatest that the difference may overflow
 #pragma unroll
             for (int i = 0; i < E; i += 2) st.template add<true>(to_float(e[i]), to_float(e[i + 1]));
         } else {

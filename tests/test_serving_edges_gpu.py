@@ -297,3 +297,24 @@ def test_attention_over_the_largest_values(cuda_device, schedule, dtype, D, coun
         ref = S.attention(q[:m], K, V, [[0, 1]], [n], [0, m], D ** -0.5)
         assert got.isfinite().all()
         near(got, ref)
+
+
+# -------------------------------------------------------------------------------------------------------------- log probabilities
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [50, 9000, 50304])
+@pytest.mark.parametrize("far", [-1e31, -9e36, -9.99e36, -1e37, -3e38])
+def test_logprobs_beside_the_type_s_largest(cuda_device, dtype, vocab, far):
+    """Finite logits whose distance from the greatest is no fp32 number: probability 0, and nothing of the entropy."""
+    import clusterfusionplus_b200 as cf
+    top = torch.finfo(dtype).max
+    x = torch.full((4, vocab), far, dtype=dtype, device=DEV)
+    x[0, 7] = top
+    x[1, 3], x[1, 40] = top, top
+    x[2, ::2], x[2, 1::2] = 0.0, far
+    x[3, 5:], x[3, 20] = -math.inf, top
+    got = cf.token_logprobs(x, ints([7, 40, 0, 20]), 2)
+    zeros = (vocab + 1) // 2
+    want = torch.tensor([0.0, math.log(2), math.log(zeros), 0.0], device=DEV)
+    tol = 2 * (vocab / 512 + 28) * 2.0 ** -24 * max(1.0, math.log(zeros))         # sums of equal numbers, as derived for all rows
+    assert ((got.entropy - want).abs() <= tol).all() and ((got.logprobs + want).abs() <= tol).all(), (got.entropy, got.logprobs)
+    assert got.top_tokens.tolist() == [[7, 0], [3, 40], [0, 2], [20, 0]]
