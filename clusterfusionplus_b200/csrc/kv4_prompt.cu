@@ -156,7 +156,9 @@ struct Shared {
     unsigned there[4];          // [tile % 4] bit t: the 16 tokens t of the tile exist.  Four: keys are unpacked two tiles ahead of the softmax
     unsigned long long agreed[4], summed[4];  // of the two warps that share rows
     float high[2][2][ROWS], sums[2][ROWS];    // [tile & 1][half][row]: greatest score; [half][row]: denominator
-    int not_finite;                           // a token that some row sees has value parameters that are not finite
+    // [item % 8][group]: the first token that some row sees and whose value parameters are not finite.  The unpacking warps may be three tiles, so as
+    // many items, ahead of the softmax; a thread of the softmax clears an item's place four items before it, when that of four items ago was read.
+    int first_broken[8][4];
     __align__(16) uint16_t kpar[8][16][8];     // [unpacking warp][token][scales, minima of the keys]
     __align__(16) uint16_t vpar[8][2][4][16];  // [unpacking warp][scale, minimum of the values][group][token]
 };
@@ -191,7 +193,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
             mbar_init(bar(sh.agreed[i]), 64);
             mbar_init(bar(sh.summed[i]), 64);
         }
-        sh.abort = sh.not_finite = 0;
+        sh.abort = 0;
+        for (int i = 0; i < 8 * 4; ++i) sh.first_broken[i / 4][i % 4] = 0x7fffffff;
         for (int i = 0; i < 4; ++i) sh.there[i] = 0;
     }
     if (warp == SOFT + UNPACK) {  // scores twice 128 columns, numerators 128: 512 is the next size there is
@@ -236,6 +239,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
             const int last = real ? static_cast<int>(max(min(before + qi, cap - 1), -1ll)) : -1;
             const int all_see = static_cast<int>(max(min(before + r0 / per, cap - 1), -1ll));  // every real row sees these
             if (n > 0) {
+                if (tid < 4) sh.first_broken[(items + 4) & 7][tid] = 0x7fffffff;
                 // all loads of the row at once: in turn they would take longer than a tile.  The row's two threads write half of it each.
                 uint4 own[DP / 16], rest[DP / 16];
 #pragma unroll
@@ -378,21 +382,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                 if (ok) {
                     fence_after();
                     l += sh.sums[half ^ 1][line];
-                    unsigned broken = 0;  // groups in which the row sees a value that is not finite: looked up only if there was one at all
-                    if (sh.not_finite) {
-                        const int tiles_a_page = a.page / KV4_TILE;
-                        for (int t = 0; t * KV4_TILE <= last; ++t) {
-                            const int held = table[t / tiles_a_page];
-                            if (held < 0 || held >= a.pages) continue;
-                            const uint8_t* tile = a.cache + ((static_cast<long long>(held) * a.kv_heads + kvh) * tiles_a_page + t % tiles_a_page) * TB;
-                            for (int k = 0; k < KV4_TILE && t * KV4_TILE + k <= last; ++k)
-                                for (int g = 0; g < G; ++g)
-                                    if (!finite_half(*reinterpret_cast<const unsigned short*>(tile + kv4_param(G, k, 2, g))) ||
-                                        !finite_half(*reinterpret_cast<const unsigned short*>(tile + kv4_param(G, k, 3, g))))
-                                        broken |= 1u << g;
-                        }
-                        __syncwarp();
-                    }
+                    unsigned broken = 0;  // groups in which the row sees a value that is not finite
+#pragma unroll
+                    for (int g = 0; g < G; ++g) broken |= (sh.first_broken[items & 7][g] <= last ? 1u : 0u) << g;
                     const float by = l == 0.f ? 0.f : 1.f / l;  // no token seen: zeros; NaN stays
                     for (int c = 16 * half; c < N; c += 32) {
                         float o[16];
@@ -488,7 +480,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                     // rows that see it become NaN in this group at the end.  Behind the last token, where anything may lie, nothing is taken.
                     if (g0 + k < G) {
                         const bool seen = token0 + row <= end, fine = finite_half(par[2][k]) && finite_half(par[3][k]);
-                        if (seen && !fine) sh.not_finite = 1;
+                        if (seen && !fine) atomicMin(&sh.first_broken[items & 7][g0 + k], static_cast<int>(token0) + row);
                         sh.kpar[part][row][g0 + k] = static_cast<uint16_t>(par[0][k]);
                         sh.kpar[part][row][4 + g0 + k] = static_cast<uint16_t>(par[1][k]);
                         sh.vpar[part][0][g0 + k][row] = static_cast<uint16_t>(seen && fine ? par[2][k] : 0u);

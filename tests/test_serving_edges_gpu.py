@@ -318,3 +318,50 @@ def test_logprobs_beside_the_type_s_largest(cuda_device, dtype, vocab, far):
     tol = 2 * (vocab / 512 + 28) * 2.0 ** -24 * max(1.0, math.log(zeros))         # sums of equal numbers, as derived for all rows
     assert ((got.entropy - want).abs() <= tol).all() and ((got.logprobs + want).abs() <= tol).all(), (got.entropy, got.logprobs)
     assert got.top_tokens.tolist() == [[7, 0], [3, 40], [0, 2], [20, 0]]
+
+
+# ------------------------------------------------------------------------------------------------ values that are not finite
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("T,count,where", [(60, 30, [(40, 0)]), (700, 200, [(0, 3), (520, 33), (690, 70), (699, 0)]), (700, 1, [(300, 90)]), (700, 200, [(t, 5) for t in range(0, 700, 7)]),
+                                           (300, 150, [(t, d) for t in range(200, 216) for d in range(0, 128, 32)])])
+@pytest.mark.parametrize("D", [32, 96, 128])
+def test_attention_marks_the_groups_of_values_that_are_not_finite(cuda_device, schedule, bad, T, count, where, D):
+    """NaN in the group's dims for the queries that see such a token, and nothing of it for the others, wherever in tiles and pages it lies."""
+    import clusterfusionplus_b200 as cf
+    g = torch.Generator(device=DEV).manual_seed(T + D)
+    q, key, value = (torch.randn(n, h, D, device=DEV, generator=g).half() for n, h in ((count, 4), (T, 2), (T, 2)))
+    for t, d in where:
+        value[t, 1, d % D] = bad
+    cache = cf.kv4_cache(-(-T // 32) + 1, 2, 32, D)
+    order = torch.randperm(-(-T // 32), device=DEV).int()
+    at = torch.arange(T, device=DEV)
+    cf.kv4_append(key, value, (order[at // 32] * 32 + at % 32).int(), cache)
+    K, V = S.unpack(cache, D)
+    table = [order.tolist()]
+    got = cf.kv4_attention(q, cache, ints(table), ints([T]), ints([0, count]), max_q_len=count)
+    ref = S.attention(q, K, V, table, [T], [0, count], D ** -0.5)
+    assert torch.equal(got.isnan().cpu(), ref.isnan())
+    fine = ~ref.isnan()
+    near(got[fine.to(DEV)], ref[fine])
+
+
+@pytest.mark.parametrize("T", [100, 700])
+def test_attention_marks_them_where_a_cta_takes_several_tiles_of_rows(cuda_device, T):
+    """More rows than the hint says: the same CTAs go through 128 rows after 128 rows, the marks of one are not those of the next."""
+    import clusterfusionplus_b200 as cf
+    D, count, B = 64, T, 2
+    g = torch.Generator(device=DEV).manual_seed(T)
+    q, key, value = (torch.randn(B * n, h, D, device=DEV, generator=g).half() for n, h in ((count, 16), (T, 8), (T, 8)))
+    for t, h, d in ((T - 1, 0, 0), (T // 2, 1, 40), (0, 2, 5), (T + T // 3, 1, 1), (2 * T - 2, 7, 63)):
+        value[t, h, d] = math.nan
+    pages = -(-T // 16)
+    cache = cf.kv4_cache(B * pages, 8, 16, D)
+    at = torch.arange(B * T, device=DEV, dtype=torch.int32)
+    cf.kv4_append(key, value, at // T * (pages * 16) + at % T, cache)
+    K, V = S.unpack(cache, D)
+    table = [list(range(pages)), list(range(pages, 2 * pages))]
+    got = cf.kv4_attention(q, cache, ints(table), ints([T] * B), ints([0, count, 2 * count]), max_q_len=128)
+    ref = S.attention(q, K, V, table, [T] * B, [0, count, 2 * count], D ** -0.5)
+    assert torch.equal(got.isnan().cpu(), ref.isnan())
+    fine = ~ref.isnan()
+    near(got[fine.to(DEV)], ref[fine])
