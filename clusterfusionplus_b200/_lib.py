@@ -140,18 +140,23 @@ lib = _load()
 
 
 def serving_binding():
-    """The extension module of the serving calls (csrc/serving_binding.cpp), bound to the library loaded above."""
+    """The extension module of the serving calls (csrc/serving_binding.cpp), bound to the library loaded above.  It uses torch's C++ interface, which
+    holds for one version of torch only; the rest of the package does not."""
     import importlib.util
 
     import torch
     path = os.path.join(_HERE, "lib", "_serving.so")
     if not os.path.exists(path):
         raise ImportError(f"{path} is missing: build it with `python clusterfusionplus_b200/build.py`. There is no fallback implementation.")
+    built_for = None
+    if os.path.exists(path[:-3] + ".torch"):
+        with open(path[:-3] + ".torch") as f:
+            built_for = f.read()
+    if built_for != str(torch.__version__):
+        raise ImportError(f"{path} was built for torch {built_for}, this is {torch.__version__}: run `python clusterfusionplus_b200/build.py`")
     spec = importlib.util.spec_from_file_location("_serving", path)
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
-    if mod.torch_version != torch.__version__.split("+")[0]:
-        raise ImportError(f"{path} was built for torch {mod.torch_version}, this is {torch.__version__}: run `python clusterfusionplus_b200/build.py --force`")
     mod.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
         "cf_last_error", "cf_paged_kv_plan", "cf_paged_kv_release", "cf_kv4_append", "cf_kv4_read", "cf_kv4_attention", "cf_kv4_attention_workspace", "cf_token_logprobs")))
     return mod

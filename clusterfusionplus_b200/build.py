@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -41,6 +42,7 @@ UNITS = {
 }
 BINDING = os.path.join(CSRC, "serving_binding.cpp")
 BINDING_OUT = os.path.join(HERE, "lib", "_serving.so")
+BINDING_TORCH = os.path.join(HERE, "lib", "_serving.torch")  # the torch version that it was built for
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -98,6 +100,20 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def torch_version() -> str:
+    """torch.__version__, without the import."""
+    path = os.path.join(os.path.dirname(importlib.util.find_spec("torch").origin), "version.py")
+    with open(path) as f:
+        return re.search(r"^__version__\s*=\s*['\"]([^'\"]+)['\"]", f.read(), re.M).group(1)
+
+
+def _binding_stale() -> bool:
+    if _stale(BINDING_OUT, [BINDING, HEADER]) or not os.path.exists(BINDING_TORCH):
+        return True
+    with open(BINDING_TORCH) as f:
+        return f.read() != torch_version()
+
+
 def _bind(verbose: bool) -> None:
     torch = os.path.dirname(importlib.util.find_spec("torch").origin)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc_path())))
@@ -110,10 +126,12 @@ def _bind(verbose: bool) -> None:
         sys.stderr.write(r.stdout + r.stderr)
     if r.returncode != 0:
         raise RuntimeError("g++ failed on serving_binding.cpp")
+    with open(BINDING_TORCH, "w") as f:
+        f.write(torch_version())
 
 
 def up_to_date() -> bool:
-    return not _stale(OUT, [d for s in UNITS for d in _deps(s)]) and not _stale(BINDING_OUT, [BINDING, HEADER])
+    return not _stale(OUT, [d for s in UNITS for d in _deps(s)]) and not _binding_stale()
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -122,7 +140,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     todo = [s for s in UNITS if force or _stale(os.path.join(OBJ, s.replace(".cu", ".o")), _deps(s))]
     with ThreadPoolExecutor(max_workers=len(UNITS) + 1) as ex:
-        binding = ex.submit(_bind, verbose) if force or _stale(BINDING_OUT, [BINDING, HEADER]) else None
+        binding = ex.submit(_bind, verbose) if force or _binding_stale() else None
         list(ex.map(lambda s: _compile(s, verbose), todo))
         if binding:
             binding.result()

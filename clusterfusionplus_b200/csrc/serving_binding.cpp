@@ -13,7 +13,6 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
-#include <torch/version.h>
 
 #include <cmath>
 #include <cstring>
@@ -355,7 +354,5 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serving", nullptr, -1, methods, n
 }  // namespace
 
 PyMODINIT_FUNC PyInit__serving(void) {
-    PyObject* m = PyModule_Create(&module);
-    if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) < 0) Py_CLEAR(m);
-    return m;
+    return PyModule_Create(&module);
 }

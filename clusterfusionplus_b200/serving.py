@@ -26,7 +26,18 @@ from ._lib import serving_binding
 
 # The steps that these calls make are short (a few microseconds on the GPU): the tensors are checked, and the results allocated, in
 # csrc/serving_binding.cpp.
-_call = serving_binding()
+class _Calls:
+    """The calls of that module, which the first of them loads."""
+
+    def __getattr__(self, name):
+        if name not in ("plan", "release", "append", "read", "attention", "logprobs"):
+            raise AttributeError(name)
+        module = serving_binding()
+        self.__dict__.update({n: getattr(module, n) for n in ("plan", "release", "append", "read", "attention", "logprobs")})
+        return self.__dict__[name]
+
+
+_call = _Calls()
 _workspace = None  # bytes of kv4_attention's workspace; None: what cf_kv4_attention_workspace says
 
 

@@ -2,7 +2,10 @@
 with (the plan, the order of the 4-bit codes, the quantisation) against properties that define it."""
 import ctypes
 import math
+import os
 import random
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -237,3 +240,29 @@ def test_quantised_values_stay_within_fp16(lo, hi):
     assert np.abs(back).max() <= 65504 and c[0, 0] == 0 and c[0, -1] == 15
     held = np.clip(x.astype(np.float64), -65504, 65504)
     assert (np.abs(back - held) <= s.astype(np.float64)[0] * (0.5 + 15 * 2.0 ** -10)).all()
+
+
+def test_another_torch_does_not_keep_the_package_from_loading():
+    """Only the serving calls need the module that is built for one torch: they say so, everything else works."""
+    code = """
+import torch
+torch.__version__ = "99.0.0a0+other"
+import clusterfusionplus_b200 as cf
+assert cf.kv4_cache(1, 1, 16, 64, device="cpu").shape == (1, 1, 16, 80)
+from clusterfusionplus_b200.api import model_dims
+try:
+    cf.kv4_append(None, None, None, None)
+except ImportError as e:
+    assert "was built for torch" in str(e) and "99.0.0a0+other" in str(e), e
+    print("said so")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and "said so" in r.stdout, r.stdout + r.stderr
+
+
+def test_a_build_for_another_torch_is_out_of_date(monkeypatch):
+    from clusterfusionplus_b200 import build
+    assert build.torch_version() == str(torch.__version__)
+    assert not build._binding_stale()
+    monkeypatch.setattr(build, "torch_version", lambda: "99.0.0")
+    assert build._binding_stale() and not build.up_to_date()
