@@ -266,16 +266,16 @@ int check_launch(const char* what) {
 }
 
 // Whether 128 query rows of a (request, cached head) shall share each unpacked tile (kv4_prompt.cu) or 16 at a time read the cache for
-// themselves (kv4_decode.cu).  The first takes 2.1 us for 128 tokens in each of 148 CTAs and does not divide the tokens among CTAs; the second
-// divides them evenly and takes 1.1 ns for 16 rows x 16 tokens and 14 us besides.  Measured (rows of a (request, head); the second against the
-// first): 32 pairs of 2048 tokens 64 rows 36 : 40 us, 24 rows 25 : 39; 256 pairs of 1000 tokens 32 rows 46 : 47; 8 pairs of 8192 tokens
-// 128 rows 48 : 134; 32 pairs of 4000 tokens 64 rows 50 : 71, 96 rows 72 : 72, 128 rows 82 : 72.
+// themselves (kv4_decode.cu).  The first takes 2.2 us for 128 tokens in each of 148 CTAs, 6 us besides, and does not divide the tokens among CTAs; the
+// second divides them and takes 0.88 ns for 16 rows x 16 tokens and 12 us besides.  Measured (rows of a (request, head); the second against the
+// first): 32 pairs of 2048 tokens 64 rows 29 : 40 us, 128 rows 39 : 42; 256 pairs of 1000 tokens 32 rows 46 : 47, 64 rows 89 : 48; 8 pairs of
+// 8192 tokens 256 rows 70 : 135; 32 pairs of 4000 tokens 128 rows 65 : 73; 64 pairs of 2000 tokens 64 rows 38 : 41, 96 rows 65 : 41.
 bool prompt_sized(int64_t batch, int64_t heads, int64_t kv_heads, int64_t tokens, int64_t max_q_len) {
     const int64_t rows = max_q_len * (heads / kv_heads);
     if (rows <= 16) return false;
     const double pairs = static_cast<double>(batch) * kv_heads;
     const double turns = ceil(pairs * ((rows + 127) / 128) / 148);
-    return 14 + 0.0011 * pairs * ((rows + 15) / 16) * ((tokens + 15) / 16) > 5 + 2.1 * turns * ((tokens + 127) / 128);
+    return 12 + 0.00088 * pairs * ((rows + 15) / 16) * ((tokens + 15) / 16) > turns * (6 + 2.2 * ((tokens + 127) / 128));
 }
 
 bool aligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }

@@ -831,7 +831,8 @@ __global__ void __launch_bounds__(JT) kv4_join_kernel(const Kv4AttnArgs a, int c
 // ---------------------------------------------------------------------------------------------------- launches
 constexpr int SMS = 148;
 constexpr int LEAST = 2 * W;  // tiles of a CTA's piece, at least: below that the join costs more than it saves
-template <int NT> constexpr int line_ctas() { return SMS * (NT == 1 ? 4 : 2); }
+constexpr int places(int nt) { return SMS * (nt == 1 ? 4 : 2); }  // CTAs that find room on the GPU at once: __launch_bounds__ of the kernels
+template <int NT> constexpr int line_ctas() { return places(NT); }
 
 template <class T, int G, int NT> cudaError_t launch(const Kv4AttnArgs& a, long long max_q_len, cudaStream_t st) {
     constexpr int COLS = 8 * NT;
@@ -861,10 +862,11 @@ template <class T, int G, int NT> cudaError_t launch(const Kv4AttnArgs& a, long 
     const long long items = static_cast<long long>(a.batch) * a.kv_heads;
     const long long q_tiles = (max_q_len * (a.heads / a.kv_heads) + COLS - 1) / COLS;
     const long long tiles = (a.table_width * a.page + KV4_TILE - 1) / KV4_TILE;
-    // As many CTAs to a (request, head) as find room on the GPU at once (4 to an SM; a CTA costs 4 us besides its tiles, a tile 0.5 us of a
-    // warp: 256 pairs of up to 2048 tokens 19.4 us with 2, 23.8 with 4), but at least two tiles to a warp
+    // As many CTAs to a (request, head) as find room on the GPU at once (a CTA costs 4 us besides its tiles, a tile 0.5 us of a
+    // warp: 256 pairs of up to 2048 tokens 19.4 us with 2, 23.8 with 4; of 9 to 16 rows, where half as many find room, 37.9 with 1, 51.6 with
+    // 2, and 64 pairs 17.9 with 4, 26.1 with 8), but at least two tiles to a warp
     int cluster = 1;
-    while (cluster < MAX_CLUSTER && items * q_tiles * cluster * 2 <= 4 * SMS && tiles >= 4 * W * cluster) cluster *= 2;
+    while (cluster < MAX_CLUSTER && items * q_tiles * cluster * 2 <= places(NT) && tiles >= 4 * W * cluster) cluster *= 2;
     static std::atomic<unsigned long long> allowed{0};
     const cudaError_t e = allow_shared_once(reinterpret_cast<const void*>(kv4_few_kernel<T, G, NT>), smem, allowed);
     if (e != cudaSuccess) return e;
@@ -901,11 +903,16 @@ long long kv4_few_workspace(long long heads, long long kv_heads, int D, long lon
 // head_dim 128; below, its second launch and its look at all lengths cost what the even spread gives.  Requests of mixed lengths, the line
 // against clusters: 512 (request, head) pairs of up to 8192 tokens 85 : 115 us, 256 pairs 49 : 59, 128 pairs 33 : 34, 160 pairs of up to 1000
 // tokens 16 : 12), and where there are too few pairs for clusters of 8 CTAs to reach half the GPU and each is long (8 heads x 32768
-// tokens 21 : 34, x 16384 16 : 19, x 8192 13 : 12).
+// tokens 21 : 34, x 16384 16 : 19, x 8192 13 : 12).  With 9 to 16 rows a pair takes twice as long and half as many CTAs find room: there more
+// pairs than places keep the GPU even by themselves (1024 pairs of up to 8192 tokens 359 : 288, 512 pairs 187 : 152), and the line pays for
+// fewer and long ones only (256 pairs of up to 16384 163 : 213, of up to 8192 122 : 112; 128 pairs of up to 16384 88 : 113; 16 pairs x 16384
+// 31 : 37, 32 pairs 44 : 39).
 bool kv4_few_uses_workspace(long long batch, long long heads, long long kv_heads, long long tokens, long long max_q_len) {
     const long long rows = max_q_len * (heads / kv_heads), cols = rows <= 8 ? 8 : 16;
     const long long items = batch * kv_heads * ((rows + cols - 1) / cols), tiles = (tokens + KV4_TILE - 1) / KV4_TILE;
-    return items * tiles >= 100000 || (items * MAX_CLUSTER < 2 * SMS && tiles >= 640);
+    const bool few = items * MAX_CLUSTER < places(cols / 8) / 2;
+    if (cols == 8) return items * tiles >= 100000 || (few && tiles >= 640);
+    return tiles >= 640 && (few || (items <= places(2) && items * tiles >= 100000));
 }
 
 cudaError_t kv4_attention_few(const Kv4AttnArgs& a, bool bf16, long long max_q_len, cudaStream_t st) {
