@@ -90,11 +90,13 @@ struct Call {
             complain("block_table: expected [", batch, ", pages] rows of consecutive entries, got shape ", Shape{t});
         return t;
     }
+    // elements from one entry of axis d to the next; where there is but one, its stride says nothing
+    static int64_t apart(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
     // rows of 16-bit numbers whose last axis is contiguous and whose other strides are multiples of `step` elements
     const at::Tensor& rows(PyObject* o, const char* name, int64_t step) {
         const at::Tensor& t = on_device(o, name, 3);
         half(t.scalar_type(), name);
-        if (t.stride(2) != 1 || t.stride(0) % step || t.stride(1) % step)
+        if (t.stride(2) != 1 || apart(t, 0) % step || apart(t, 1) % step)
             complain(name, ": expected a contiguous last axis and strides in multiples of ", step, " elements, got shape ", Shape{t});
         return t;
     }
@@ -222,7 +224,7 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor& slots = c.ints(a[2], "slot_map", tokens);
         {
             Aside aside;
-            check(cf.append(key.data_ptr(), value.data_ptr(), Call::half(key.scalar_type(), "key"), tokens, heads, dim, key.stride(0), key.stride(1), value.stride(0), value.stride(1),
+            check(cf.append(key.data_ptr(), value.data_ptr(), Call::half(key.scalar_type(), "key"), tokens, heads, dim, Call::apart(key, 0), Call::apart(key, 1), Call::apart(value, 0), Call::apart(value, 1),
                             slots.data_ptr<int>(), cache.data_ptr(), cache.size(0), cache.size(2), c.stream()));
         }
         Py_RETURN_NONE;
@@ -279,7 +281,7 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
             const int64_t need = asked < 0 ? cf.workspace(batch, heads, kv_heads, dim, width * page, max_q) : asked;
             at::Tensor work;  // of this call alone: graphs and streams share nothing
             if (need > 0) work = empty({need}, query, at::kByte);
-            check(cf.attention(query.data_ptr(), Call::half(query.scalar_type(), "query"), rows, heads, dim, query.stride(0), query.stride(1), cache.data_ptr(), cache.size(0), page, kv_heads,
+            check(cf.attention(query.data_ptr(), Call::half(query.scalar_type(), "query"), rows, heads, dim, Call::apart(query, 0), Call::apart(query, 1), cache.data_ptr(), cache.size(0), page, kv_heads,
                                table.data_ptr<int>(), width, apart, lens.data_ptr<int>(), indptr, batch, max_q, static_cast<float>(scale), need > 0 ? work.data_ptr() : nullptr, need,
                                out.data_ptr(), c.stream()));
         }

@@ -365,3 +365,24 @@ def test_attention_marks_them_where_a_cta_takes_several_tiles_of_rows(cuda_devic
     assert torch.equal(got.isnan().cpu(), ref.isnan())
     fine = ~ref.isnan()
     near(got[fine.to(DEV)], ref[fine])
+
+
+# ---------------------------------------------------------------------------------------------------------------------- strides
+def test_strides_of_axes_with_one_entry_do_not_matter(cuda_device):
+    """One token, or one head, cut out of rows that lie an odd number of elements apart."""
+    import clusterfusionplus_b200 as cf
+    room = torch.randn(9, 515, device=DEV).half()
+    x = room[:, :512].unflatten(1, (8, 64))[:1]
+    assert x.stride(0) == 515
+    one_head = torch.as_strided(room, (3, 1, 64), (128, 7, 1))
+    cache, same = cf.kv4_cache(1, 4, 16, 64), cf.kv4_cache(1, 4, 16, 64)
+    cf.kv4_append(x[:, :4], x[:, 4:], ints([3]), cache)
+    cf.kv4_append(x[:, :4].contiguous(), x[:, 4:].contiguous(), ints([3]), same)
+    assert torch.equal(cache, same) and cache.any()
+    table, n = ints([[0]]), ints([16])
+    assert torch.equal(cf.kv4_attention(x, cache, table, n), cf.kv4_attention(x.contiguous(), cache, table, n))
+    single = cf.kv4_cache(1, 1, 16, 64)
+    cf.kv4_append(one_head, one_head, ints([0, 1, 2]), single)
+    assert torch.equal(cf.kv4_attention(one_head, single, ints([[0]] * 3), ints([3] * 3)), cf.kv4_attention(one_head.contiguous(), single, ints([[0]] * 3), ints([3] * 3)))
+    with pytest.raises(RuntimeError, match="strides"):
+        cf.kv4_attention(room[:2, :512].as_strided((2, 8, 64), (515, 64, 1)), cache, ints([[0]] * 2), ints([16] * 2))
