@@ -386,3 +386,28 @@ def test_strides_of_axes_with_one_entry_do_not_matter(cuda_device):
     assert torch.equal(cf.kv4_attention(one_head, single, ints([[0]] * 3), ints([3] * 3)), cf.kv4_attention(one_head.contiguous(), single, ints([[0]] * 3), ints([3] * 3)))
     with pytest.raises(RuntimeError, match="strides"):
         cf.kv4_attention(room[:2, :512].as_strided((2, 8, 64), (515, 64, 1)), cache, ints([[0]] * 2), ints([16] * 2))
+
+
+# ------------------------------------------------------------------------------------------ log probabilities, each to its own bound
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab,spread", [(40, 200, 3.0), (200, 4097, 1.0), (3, 50304, 3.0), (300, 50304, 2.5), (5, 151936, 6.0)])
+def test_log_probabilities_to_fp32_s_precision(cuda_device, dtype, rows, vocab, spread):
+    """log p = (x - m) - log z, with u = 2^-24: x - m and the result round once each, logf is good to 2 u |log z|.  z is a sum of positive terms: runs
+    of at most vocab / 512 and 12 levels of joins, which round twice and scale by ex2 (4 u) each; a term's exponent d = x - m <= 4 + log-distance
+    rounds with 2.5 u |d| (difference, product, constant), whose mean under p is at most E|d| = log z - H + 4, and ex2 is good to 4 u."""
+    import clusterfusionplus_b200 as cf
+    g = torch.Generator(device=DEV).manual_seed(rows + vocab)
+    x = (torch.randn(rows, vocab, device=DEV, generator=g) * spread).to(dtype)
+    tokens = torch.randint(0, vocab, (rows,), device=DEV, generator=g)
+    got = cf.token_logprobs(x, tokens, 8)
+    lp, h, tl, ti = (t.to(DEV) for t in S.logprobs(x, tokens.tolist(), 8))
+    log_z = -tl[:, 0]                                                                 # of the terms relative to the greatest
+    u, z_err = 2.0 ** -24, vocab / 512 + 12 * 6 + 4 + 2.5 * (log_z.abs() + 4)
+    assert got.top_tokens.equal(ti)
+    bound = u * (z_err + 2 * (log_z.abs() + 4) + 8)                                   # the reference m may lie up to 4 below the greatest
+    for a, b in ((got.logprobs[:, None], lp[:, None]), (got.top_logprobs, tl)):
+        err = (a.double() - b).abs()
+        assert (err <= bound[:, None] + u * 2 * b.abs()).all(), (err / bound[:, None]).max().item()
+    # w / z: the same relative errors on a sum whose terms are |d| p
+    err = (got.entropy.double() - h).abs()
+    assert (err <= bound + u * (2 * z_err + 8) * (log_z.abs() + 4)).all(), (err / bound).max().item()
