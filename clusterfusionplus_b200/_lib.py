@@ -48,7 +48,7 @@ class CfDecoderConfig(C.Structure):
 CF_DECODER_GELU_ERF = 1
 CF_DTYPE_FP16, CF_DTYPE_BF16, CF_DTYPE_FP32 = 0, 1, 2
 CF_PLAN_NO_PAGES, CF_PLAN_TABLE_WIDTH, CF_PLAN_MAX_TOKENS, CF_PLAN_MAX_ROWS, CF_PLAN_BAD_LENGTH, CF_PLAN_BAD_PAGE = 1, 2, 4, 8, 16, 32
-CF_ACT_NONE, CF_ACT_GELU_TANH, CF_ACT_GELU_ERF = 0, 1, 2
+CF_ACT_NONE, CF_ACT_GELU_TANH, CF_ACT_GELU_ERF, CF_OUT_FP32 = 0, 1, 2, 3
 
 
 class CfHeadWeights(C.Structure):

@@ -1771,7 +1771,7 @@ int cf_prefill_linear(const void* x, const void* weight, const void* bias, const
     if (m <= 0 || n <= 0 || k <= 0 || m > 0x7fffffff || n > 0x7fffffff || k > 0x7fffffff)
         return fail(CF_ERR_INVALID, "bad GEMM extent %lld x %lld x %lld", (long long)m, (long long)n, (long long)k);
     if ((n % 8) || (k % 8)) return fail(CF_ERR_UNSUPPORTED, "n (%lld) and k (%lld) must be multiples of 8", (long long)n, (long long)k);
-    if (act != CF_ACT_NONE && act != CF_ACT_GELU_TANH && act != CF_ACT_GELU_ERF) return fail(CF_ERR_INVALID, "activation %d", act);
+    if (act != CF_ACT_NONE && act != CF_ACT_GELU_TANH && act != CF_ACT_GELU_ERF && act != CF_OUT_FP32) return fail(CF_ERR_INVALID, "activation %d", act);
     if (residual && act != CF_ACT_NONE) return fail(CF_ERR_INVALID, "a residual goes with CF_ACT_NONE only");
     DeviceState* ds;
     int rc = get_device(&ds);

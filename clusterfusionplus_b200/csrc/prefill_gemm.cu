@@ -1,7 +1,7 @@
 // Prompt ingestion (prefill) linear layers on the 5th-generation tensor cores.
 //
 // out[m, n] = act(x[m, k] . W[n, k]^T + bias[n] + residual[m, n]), fp16 in and out, fp32
-// accumulation in tensor memory.  The kernel is assembled from CUTLASS's sm_100 building
+// accumulation in tensor memory; without activation and residual the output may be fp32 (logits).  The kernel is assembled from CUTLASS's sm_100 building
 // blocks (TMA loads of both operands into shared memory, tcgen05.mma issued by one thread,
 // accumulators in TMEM, epilogue reading them back with tcgen05.ld), with bias, GELU and the
 // residual add fused into the epilogue so that no intermediate goes through HBM twice.
@@ -35,19 +35,20 @@ namespace {
 
 using namespace cute;
 
-template <template <class> class Act>
+template <template <class> class Act, class Out = cutlass::half_t>
 struct LinearGemm {
     using Element = cutlass::half_t;
     using LayoutA = cutlass::layout::RowMajor;     // activations [m, k]
     using LayoutB = cutlass::layout::ColumnMajor;  // weight [n, k] row-major == [k, n] column-major
     using LayoutC = cutlass::layout::RowMajor;     // residual / output [m, n]
     static constexpr int Align = 8;                // 16-byte rows: what TMA needs
+    static constexpr int AlignOut = 16 / sizeof(Out);
     using TileShape = Shape<_128, _128, _64>;
     using ClusterShape = Shape<_1, _1, _1>;
-    using Fusion = cutlass::epilogue::fusion::LinCombPerColBiasEltAct<Act, Element, float, Element, Element, float>;
+    using Fusion = cutlass::epilogue::fusion::LinCombPerColBiasEltAct<Act, Out, float, Element, Element, float>;
     using Epilogue = typename cutlass::epilogue::collective::CollectiveBuilder<
         cutlass::arch::Sm100, cutlass::arch::OpClassTensorOp, TileShape, ClusterShape,
-        cutlass::epilogue::collective::EpilogueTileAuto, float, float, Element, LayoutC, Align, Element, LayoutC, Align,
+        cutlass::epilogue::collective::EpilogueTileAuto, float, float, Element, LayoutC, Align, Out, LayoutC, AlignOut,
         cutlass::epilogue::collective::EpilogueScheduleAuto, Fusion>::CollectiveOp;
     using Mainloop = typename cutlass::gemm::collective::CollectiveBuilder<
         cutlass::arch::Sm100, cutlass::arch::OpClassTensorOp, Element, LayoutA, Align, Element, LayoutB, Align, float,
@@ -71,7 +72,7 @@ struct LinearGemm {
             cutlass::gemm::GemmUniversalMode::kGemm,
             {m, n, k, 1},
             {static_cast<const Element*>(x), sa, static_cast<const Element*>(w), sb},
-            {{}, static_cast<const Element*>(residual), sc, static_cast<Element*>(out), sd}};
+            {{}, static_cast<const Element*>(residual), sc, static_cast<Out*>(out), sd}};
         args.epilogue.thread.alpha = 1.0f;
         args.epilogue.thread.beta = residual ? 1.0f : 0.0f;
         args.epilogue.thread.bias_ptr = static_cast<const Element*>(bias);
@@ -95,6 +96,8 @@ const char* prefill_linear(const void* x, const void* w, const void* bias, const
             return LinearGemm<cutlass::epilogue::thread::GELU_taylor>::run(x, w, bias, residual, out, m, n, k, st);
         case PREFILL_ACT_GELU_ERF:
             return LinearGemm<cutlass::epilogue::thread::GELU>::run(x, w, bias, residual, out, m, n, k, st);
+        case PREFILL_OUT_FP32:
+            return LinearGemm<cutlass::epilogue::thread::Identity, float>::run(x, w, bias, residual, out, m, n, k, st);
         default:
             return "unknown activation";
     }

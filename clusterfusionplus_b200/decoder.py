@@ -13,7 +13,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from ._lib import CF_ACT_GELU_ERF, CF_ACT_GELU_TANH, CF_ACT_NONE, CF_DECODER_GELU_ERF, CfDecoderConfig, CfDims, CfHeadWeights, CfLayerWeights, check, lib
+from ._lib import CF_ACT_GELU_ERF, CF_ACT_GELU_TANH, CF_ACT_NONE, CF_DECODER_GELU_ERF, CF_OUT_FP32, CfDecoderConfig, CfDims, CfHeadWeights, CfLayerWeights, check, lib
 from .api import _req, _wrap
 from .serving import TokenLogprobs, token_logprobs
 
@@ -49,10 +49,11 @@ def layer_weights_struct(d: CfDims, w: Dict[str, torch.Tensor]) -> CfLayerWeight
 def prefill_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                    residual: Optional[torch.Tensor] = None, act: int = CF_ACT_NONE) -> torch.Tensor:
     """act(x @ weight.T + bias + residual) for fp16 x [m, k], weight [n, k] on the tensor cores
-    (cf_prefill_linear: TMA-fed tcgen05 GEMM with the bias, GELU and residual fused in)."""
+    (cf_prefill_linear: TMA-fed tcgen05 GEMM with the bias, GELU and residual fused in).  act CF_OUT_FP32: no
+    activation, the result in fp32."""
     m, k = x.shape
     n = weight.shape[0]
-    out = torch.empty(m, n, device=x.device, dtype=torch.float16)
+    out = torch.empty(m, n, device=x.device, dtype=torch.float32 if act == CF_OUT_FP32 else torch.float16)
     check(lib.cf_prefill_linear(_req(x, "x", m * k), _req(weight, "weight", n * k),
                                 None if bias is None else _req(bias, "bias", n),
                                 None if residual is None else _req(residual, "residual", m * n),
@@ -210,9 +211,8 @@ class PythiaDecoder:
     @torch.no_grad()
     def score(self, tokens: Sequence[int], top_k: int = 0) -> TokenLogprobs:
         """prefill(tokens), and the log probabilities of tokens[1:] given what precedes each, the entropy of every prediction
-        and its top_k alternatives (token_logprobs; len(tokens) - 1 rows).  The logits of the prompt are fp16, as the LM head's
-        tensor-core product leaves them: a log probability is off by up to half an fp16 step of the logits (4e-3 at
-        logits of 8 to 16); those of step() are fp32.  The vocabulary has to be a multiple of 8."""
+        and its top_k alternatives (token_logprobs; len(tokens) - 1 rows).  The logits are fp32, as those of step().  The
+        vocabulary has to be a multiple of 8."""
         ids, x = self._ingest(tokens)
         d = self.dims
         if x is None:
@@ -223,8 +223,8 @@ class PythiaDecoder:
         check(lib.cf_prefill_layernorm2(x.data_ptr(), _req(h["final_ln_weight"], "final_ln_weight", d.hidden),
                                         _req(h["final_ln_bias"], "final_ln_bias", d.hidden), None, None, y.data_ptr(), None, x.shape[0],
                                         d.hidden, 1e-5, torch.cuda.current_stream().cuda_stream))
-        # 2048 rows of logits at a time (206 MB for a vocabulary of 50304)
-        parts = [token_logprobs(prefill_linear(y[i:i + 2048], h["embed_out"]), ids[1 + i:1 + i + 2048], top_k)
+        # 2048 rows of logits at a time (412 MB for a vocabulary of 50304)
+        parts = [token_logprobs(prefill_linear(y[i:i + 2048], h["embed_out"], act=CF_OUT_FP32), ids[1 + i:1 + i + 2048], top_k)
                  for i in range(0, y.shape[0], 2048)]
         return TokenLogprobs(*(torch.cat(p) for p in zip(*parts)))
 

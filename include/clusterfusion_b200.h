@@ -374,11 +374,13 @@ int cf_decoder_destroy(int64_t handle);
  * This is the linear layer of that pass as a tensor-core GEMM:
  *   out[m, n] = act(x[m, k] . weight[n, k]^T + bias[n] + residual[m, n])
  * all fp16, fp32 accumulation; bias and residual may be NULL; residual only
- * with CF_ACT_NONE.  n and k must be multiples of 8.  Asynchronous on `stream`.
+ * with CF_ACT_NONE.  CF_OUT_FP32 in the place of an activation: none, and out
+ * is fp32 (logits, of which an fp16 rounding would be 4e-3 at 8 to 16).  n and k must be multiples of 8.  Asynchronous on `stream`.
  * ------------------------------------------------------------------------- */
 #define CF_ACT_NONE 0
 #define CF_ACT_GELU_TANH 1
 #define CF_ACT_GELU_ERF 2
+#define CF_OUT_FP32 3
 int cf_prefill_linear(const void* x, const void* weight, const void* bias, const void* residual, void* out,
                       int64_t m, int64_t n, int64_t k, int act, void* stream);
 

@@ -411,3 +411,48 @@ def test_log_probabilities_to_fp32_s_precision(cuda_device, dtype, rows, vocab, 
     # w / z: the same relative errors on a sum whose terms are |d| p
     err = (got.entropy.double() - h).abs()
     assert (err <= bound + u * (2 * z_err + 8) * (log_z.abs() + 4)).all(), (err / bound).max().item()
+
+
+# -------------------------------------------------------------------------------------------------------------- a prompt's logits
+@pytest.mark.parametrize("m,n,k", [(1, 1024, 1024), (23, 1024, 512), (130, 2056, 2560), (257, 50304, 1024)])
+def test_linear_with_an_fp32_result(cuda_device, m, n, k):
+    """Products of fp16 numbers are exact in fp32; a sum of k of them is off by at most k 2^-24 of the sum of their sizes."""
+    from clusterfusionplus_b200._lib import CF_OUT_FP32
+    from clusterfusionplus_b200.decoder import prefill_linear
+    g = torch.Generator(device=DEV).manual_seed(m + n)
+    x, w, b = torch.randn(m, k, device=DEV, generator=g).half(), (torch.randn(n, k, device=DEV, generator=g) * 0.3).half(), torch.randn(n, device=DEV, generator=g).half()
+    for bias in (None, b):
+        got = prefill_linear(x, w, bias, act=CF_OUT_FP32)
+        assert got.dtype == torch.float32 and got.shape == (m, n)
+        ref, size = x.double() @ w.double().t(), x.abs().double() @ w.abs().double().t()
+        if bias is not None:
+            ref, size = ref + bias.double(), size + bias.abs().double()
+        assert ((got.double() - ref).abs() <= (k + 1) * 2.0 ** -24 * size).all()
+    with pytest.raises(RuntimeError, match="residual"):
+        prefill_linear(x, w, residual=torch.zeros(m, n, device=DEV, dtype=torch.float16), act=CF_OUT_FP32)
+
+
+def test_score_does_not_round_its_logits(cuda_device):
+    """Logits of tens, where an fp16 rounding alone is 8e-3 to 3e-2: the log probabilities of the hidden states' own logits in 64 bits."""
+    import clusterfusionplus_b200 as cf
+    from clusterfusionplus_b200._lib import check, lib
+    mini = O.Shape("mini", hidden=512, heads=4, head_dim=128, rotary=32, ffn=2048, vocab=1024, layers=1)
+    layers, head = [O.make_layer_weights(mini, 0, seed=5, device=DEV, std=0.05)], O.make_head_weights(mini, seed=5, device=DEV, std=0.05)
+    head["embed_out"] = head["embed_out"] * 20
+    d = cf.CfDims()
+    d.hidden, d.heads, d.head_dim, d.rotary, d.ffn, d.vocab = 512, 4, 128, 32, 2048, 1024
+    dec = cf.PythiaDecoder(d, layers, head, [(torch.zeros(64, 512, dtype=torch.float16, device=DEV), torch.zeros(64, 512, dtype=torch.float16, device=DEV))], 64, use_graph=False)
+    rng = random.Random(3)
+    tokens = [rng.randrange(1024) for _ in range(40)]
+    got = dec.score(tokens, 3)
+    x, y, w = dec._ingest(tokens)[1], torch.empty(39, 512, dtype=torch.float16, device=DEV), head
+    check(lib.cf_prefill_layernorm2(x.data_ptr(), w["final_ln_weight"].data_ptr(), w["final_ln_bias"].data_ptr(), None, None, y.data_ptr(), None, 39, 512, 1e-5,
+                                    torch.cuda.current_stream().cuda_stream))
+    lg = y.double() @ w["embed_out"].double().t()
+    assert 32 < lg.abs().amax() < 128
+    lp, h, tl, _ = S.logprobs(lg, tokens[1:], 3)
+    # a logit is a sum in fp32, in 32 steps of 16 products: each cuts off less than 2^-23 of a partial sum below 128, 5e-4 in all; a log probability takes
+    # two of them, the entropy one for each |log p| <= 1 that p spreads over
+    for a, b in ((got.logprobs, lp), (got.top_logprobs, tl), (got.entropy, h)):
+        assert (a.double().cpu() - b).abs().max() <= 1e-3
+    dec.close()
