@@ -456,3 +456,26 @@ def test_score_does_not_round_its_logits(cuda_device):
     for a, b in ((got.logprobs, lp), (got.top_logprobs, tl), (got.entropy, h)):
         assert (a.double().cpu() - b).abs().max() <= 1e-3
     dec.close()
+
+
+# ------------------------------------------------------------------------------------------------------- few rows: 32-bit precision
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("way", [None, 64 << 20])
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("T,count", [(24, 1), (500, 1), (500, 3), (3000, 8)])
+def test_attention_of_few_rows_rounds_only_its_result(cuda_device, monkeypatch, dtype, way, D, T, count):
+    """Codes, keys and values are exact operands, probabilities keep 22 bits: what is left are fp32 sums (2^-16 of the largest value, as for all schedules)
+    and the result's rounding."""
+    import clusterfusionplus_b200 as cf
+    from clusterfusionplus_b200 import serving
+    monkeypatch.setattr(serving, "_workspace", way)
+    g = torch.Generator(device=DEV).manual_seed(T + D)
+    q, key, value = (torch.randn(n, h, D, device=DEV, generator=g).to(dtype) for n, h in ((count, 4), (T, 2), (T, 2)))
+    cache = cf.kv4_cache(-(-T // 16), 2, 16, D)
+    cf.kv4_append(key, value, ints(list(range(T))), cache)
+    K, V = S.unpack(cache, D)
+    table = [list(range(-(-T // 16)))]
+    got = cf.kv4_attention(q, cache, ints(table), ints([T]), ints([0, count]), max_q_len=count)
+    ref = S.attention(q, K, V, table, [T], [0, count], D ** -0.5)
+    off = (got.double().cpu() - ref).abs() - torch.finfo(dtype).eps / 2 * ref.abs() - 2.0 ** -25
+    assert (off <= 2.0 ** -16 * V.abs().amax()).all(), (off / V.abs().amax()).max().item()
