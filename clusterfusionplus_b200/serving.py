@@ -103,8 +103,15 @@ def kv4_attention(query, cache, block_table, kv_lens, qo_indptr=None, max_q_len:
 
     Request b owns the rows qo_indptr[b] : qo_indptr[b + 1] (int32 [batch + 1]; None: row b).  They are its last tokens and in the cache
     already: of n queries the i-th sees the first kv_lens[b] - n + i + 1 tokens of the pages block_table[b].  A query that sees
-    none gives zeros.  Rows that no request owns are left as they were in `out` (undefined without `out`), which must not overlap the queries.  max_q_len: the most rows
-    of a request; a hint for the size of the launch, the result does not depend on it.  scale: 1 / sqrt(head_dim) if None."""
+    none gives zeros.  Rows that no request owns are left as they were in `out` (undefined without `out`), which must not overlap the queries.  scale:
+    1 / sqrt(head_dim) if None.
+
+    How the work is dealt out is chosen by max_q_len, the most rows of a request, and by the columns of block_table, the most pages of one: neither
+    changes what is computed, but both should fit the step.  Of a table as wide as the longest context pass the columns in use,
+    block_table[:, :n] (8 requests of up to 2048 tokens with 6 queries each: 26 us in a table for 131072 tokens, 21 in its first columns).  Requests of
+    a few rows and long chunks of prompts are better two calls, with the same `out` and the parts of each list: with the n decoding requests first,
+    query, block_table[:n], kv_lens[:n], qo_indptr[: n + 1] and the same from n (63 requests of up to 8192 tokens beside a chunk of 512: 566 us in one
+    call, 243 in two)."""
     return _call.attention(query, cache, block_table, kv_lens, qo_indptr, max_q_len, scale, out, _workspace)
 
 

@@ -471,8 +471,9 @@ int cf_kv4_read(const void* cache, int64_t pages, int64_t page_size, int64_t kv_
  * b); they are its last tokens: of n queries and kv_lens[b] cached tokens, query i sees the first kv_lens[b] - n + i + 1
  * tokens, which lie in the pages block_table[b][0 ..].  A query that sees no token gives zeros.  Rows of out that no
  * request owns stay as they are.  A page number outside the cache is skipped as if its tokens were not there, and recorded
- * (cf_get_status 8); tokens beyond table_width pages are not there either.  max_q_len: the most query rows a request
- * has, for the choice and the size of the launch; what the call computes does not depend on it.  scale: of q . k (1 /
+ * (cf_get_status 8); tokens beyond table_width pages are not there either.  max_q_len, the most query rows a request
+ * has, and table_width choose how the work is dealt out; what the call computes does not depend on them beyond that, but a table_width far above
+ * the pages in use, or one call for single tokens and long chunks together, takes up to twice as long as it needs.  scale: of q . k (1 /
  * sqrt(head_dim) as a rule).  workspace: scratch of cf_kv4_attention_workspace(...) bytes, 16-byte aligned, of any content, which no
  * call that may overlap uses; with it requests of different lengths share the GPU evenly (a second launch joins the parts).
  * NULL works too, and is the faster way where that function gives 0 (max_tokens: table_width * page_size). */

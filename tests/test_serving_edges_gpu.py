@@ -479,3 +479,31 @@ def test_attention_of_few_rows_rounds_only_its_result(cuda_device, monkeypatch, 
     ref = S.attention(q, K, V, table, [T], [0, count], D ** -0.5)
     off = (got.double().cpu() - ref).abs() - torch.finfo(dtype).eps / 2 * ref.abs() - 2.0 ** -25
     assert (off <= 2.0 ** -16 * V.abs().amax()).all(), (off / V.abs().amax()).max().item()
+
+
+@pytest.mark.parametrize("n", [0, 1, 3])
+def test_attention_of_a_mixed_step_in_two_calls(cuda_device, n):
+    """Decoding requests and prompt chunks of one step: parts of the same lists, the columns in use of a wide table, and one output."""
+    import clusterfusionplus_b200 as cf
+    lens, counts, D = [300, 17, 64, 200, 90], [1] * n + [150, 80], 64
+    lens = lens[:n] + lens[3:]
+    g = torch.Generator(device=DEV).manual_seed(n)
+    starts = [0]
+    for c in counts:
+        starts.append(starts[-1] + c)
+    q = torch.randn(starts[-1] + 4, 8, D, device=DEV, generator=g).half()
+    T = sum(-(-x // 16) * 16 for x in lens)
+    key, value = (torch.randn(T, 2, D, device=DEV, generator=g).half() for _ in range(2))
+    cache, table, at = cf.kv4_cache(T // 16, 2, 16, D), [], 0
+    cf.kv4_append(key, value, ints(list(range(T))), cache)
+    for x in lens:
+        table.append(list(range(at, at + -(-x // 16))) + [-1] * (1000 - -(-x // 16)))
+        at += -(-x // 16)
+    out, t, kv, ip = torch.full_like(q, 7.0), ints(table), ints(lens), ints(starts)
+    if n:
+        cf.kv4_attention(q, cache, t[:n, :19], kv[:n], ip[:n + 1], out=out)
+        assert (out[n:] == 7).all()
+    cf.kv4_attention(q, cache, t[n:, :19], kv[n:], ip[n:], max_q_len=150, out=out)
+    assert (out[starts[-1]:] == 7).all()
+    K, V = S.unpack(cache, D)
+    near(out[:starts[-1]], S.attention(q[:starts[-1]], K, V, table, lens, starts, D ** -0.5))
