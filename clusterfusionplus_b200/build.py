@@ -38,7 +38,7 @@ UNITS = {
     "kv4_cache.cu": (["f32x2.cuh", "kv4_layout.cuh", "kv4_attention.h", "host_common.h", HEADER], False),
     "kv4_decode.cu": (["kv4_layout.cuh", "kv4_attention.h", "mma.cuh"], False),
     "kv4_prompt.cu": (["f32x2.cuh", "kv4_layout.cuh", "kv4_attention.h", "mma.cuh", "pipeline.cuh"], False),
-    "logprobs.cu": (["f32x2.cuh", "host_common.h", HEADER], False),
+    "logprobs.cu": (["f32x2.cuh", "mma.cuh", "host_common.h", HEADER], False),
 }
 BINDING = os.path.join(CSRC, "serving_binding.cpp")
 BINDING_OUT = os.path.join(HERE, "lib", "_serving.so")

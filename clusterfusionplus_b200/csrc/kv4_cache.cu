@@ -57,7 +57,8 @@ template <> struct Two<__nv_bfloat16> {
 template <class P> __device__ __forceinline__ uint32_t bits_of(P v) { return *reinterpret_cast<const uint32_t*>(&v); }
 template <class P> __device__ __forceinline__ P pair_of(uint32_t w) { return *reinterpret_cast<const P*>(&w); }
 
-// n / d for n < 2^31 by a multiplication: with 2^(l - 1) < d <= 2^l, (n (floor(2^(31 + l) / d) + 1)) >> (31 + l) is exact
+// n / d for n < 2^31 by a multiplication (T. Granlund and P. Montgomery, Division by Invariant Integers using Multiplication, 1994): with
+// 2^(l - 1) < d <= 2^l, (n (floor(2^(31 + l) / d) + 1)) >> (31 + l) is exact
 struct Divisor {
     unsigned times, shift;
     explicit Divisor(unsigned d) {
@@ -91,8 +92,9 @@ template <class T> __device__ __forceinline__ unsigned quantise8(const uint32_t 
     }
     const __half m = __float2half_rn(end.y);
     const float mf = __half2float(m);
-    // x / 15 correctly rounded: the product with the rounded 1 / 15, corrected by its residual, which is exact in a fused multiply-add (where
-    // that would fall below fp32's range the quotient is far below fp16's)
+    // x / 15 correctly rounded (P. Markstein, Computation of Elementary Functions on the IBM RISC System/6000 Processor, 1990): the product with the
+    // rounded 1 / 15, corrected by its residual, which is exact in a fused multiply-add (where that would fall below fp32's range the quotient is far
+    // below fp16's)
     const float x15 = end.x - mf, near = x15 * (1.f / 15.f);
     __half s = __float2half_rn(fmaf(fmaf(-15.f, near, x15), 1.f / 15.f, near));
     if (fmaf(15.f, __half2float(s), mf) > 65504.f) s = __ushort_as_half(static_cast<unsigned short>(__half_as_ushort(s) - 1));

@@ -25,9 +25,11 @@
 #include "../../include/clusterfusion_b200.h"
 #include "f32x2.cuh"
 #include "host_common.h"
+#include "mma.cuh"
 
 namespace {
 
+using cfb::ex2;
 using cfb::fma2;
 using cfb::Pair;
 
@@ -38,11 +40,6 @@ constexpr int MAX_CLUSTER = 8;
 constexpr int KEEP = 1024;     // candidates that are kept; more (adversarial orders only) take the slow way
 constexpr float LOG2E = 1.4426950408889634f;
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
@@ -165,20 +162,6 @@ template <class T> struct Walk {
     __device__ __forceinline__ int vec_at(int v) const { return begin + head + v * E; }
 };
 
-__device__ __forceinline__ unsigned cluster_rank() {
-    unsigned r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t peer(const void* p, unsigned rank) {
-    uint32_t a;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
-    return a;
-}
 __device__ __forceinline__ float peer_float(uint32_t a) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
@@ -308,7 +291,7 @@ __global__ void __launch_bounds__(LT, 8) token_logprobs_kernel(const LogprobArgs
     constexpr int E = Walk<T>::E;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long r = blockIdx.x / cluster;
-    const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int rank = cluster > 1 ? static_cast<int>(cfb::cluster_ctarank()) : 0;
     const T* row = static_cast<const T*>(a.logits) + r * a.row_stride;
     const int share = ((a.vocab + cluster - 1) / cluster + 63) / 64 * 64;
     const int begin = min(rank * share, a.vocab), end = min(begin + share, a.vocab);
@@ -403,12 +386,12 @@ __global__ void __launch_bounds__(LT, 8) token_logprobs_kernel(const LogprobArgs
         join_lanes(LW);
         if (lane == 0) sh.stat[0] = sum.m, sh.stat[1] = sum.z, sh.stat[2] = sum.w;
     }
-    if (cluster > 1) cluster_sync();
+    if (cluster > 1) cfb::cluster_sync_all();
     if (rank == 0) {
         if (cluster > 1 && a.top > 0) {  // the CTAs' lists, ranked by counting (at most 256 entries: one thread each)
             const int n = cluster * a.top;
             unsigned long long x = 0;
-            if (tid < n) sh.all[tid] = x = peer_u64(peer(&sh.top[tid % a.top], tid / a.top));
+            if (tid < n) sh.all[tid] = x = peer_u64(cfb::cluster_map(&sh.top[tid % a.top], tid / a.top));
             __syncthreads();
             int at = 0;
             for (int j = 0; j < n; ++j) at += sh.all[j] > x;
@@ -419,7 +402,7 @@ __global__ void __launch_bounds__(LT, 8) token_logprobs_kernel(const LogprobArgs
         if (warp == 0) {
             if (cluster > 1) {
                 const int c = lane % cluster;
-                sum = Sum(peer_float(peer(&sh.stat[0], c)), peer_float(peer(&sh.stat[1], c)), peer_float(peer(&sh.stat[2], c)));
+                sum = Sum(peer_float(cfb::cluster_map(&sh.stat[0], c)), peer_float(cfb::cluster_map(&sh.stat[1], c)), peer_float(cfb::cluster_map(&sh.stat[2], c)));
                 join_lanes(cluster);
             }
             __syncwarp();
@@ -435,7 +418,7 @@ __global__ void __launch_bounds__(LT, 8) token_logprobs_kernel(const LogprobArgs
             }
         }
     }
-    if (cluster > 1) cluster_sync();  // a peer's shared memory is read until here
+    if (cluster > 1) cfb::cluster_sync_all();  // a peer's shared memory is read until here
 }
 
 template <class T> cudaError_t launch(const LogprobArgs& a, long long rows, int cluster, cudaStream_t st) {

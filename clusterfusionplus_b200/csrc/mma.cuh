@@ -1,4 +1,4 @@
-// Warp-level matrix instructions and asynchronous copies of the 4-bit attention kernels (thin PTX wrappers).
+// Warp-level matrix instructions, asynchronous copies and cluster primitives of the serving kernels (thin PTX wrappers).
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>
