@@ -469,15 +469,20 @@ __device__ __forceinline__ void Acc<G, NT>::step(const int (&tile)[K], int token
             }
             const uint32_t p0 = h[0], p1 = h[1];
             mma_16816(low[nt], ma, 0u, mb, 0u, p0, p1);
-            mma_16816(low[nt], ma, 0u, mb, 0u, l[0], l[1]);
+            uint32_t t0[G], t1[G];
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const uint32_t h0 = v0[g] >> 8, h1 = v1[g] >> 8, q0 = mul_half2(p0, sa[g]), q1 = mul_half2(p1, sb[g]);
-                const uint32_t t0 = rest_half2(p0, l[0], sa[g], q0), t1 = rest_half2(p1, l[1], sb[g], q1);
                 mma_16816(o[nt][2 * g], v0[g] & 0x000f000fu, h0 & 0x000f000fu, v1[g] & 0x000f000fu, h1 & 0x000f000fu, q0, q1);
                 mma_16816(o[nt][2 * g + 1], v0[g] & 0x00f000f0u, h0 & 0x00f000f0u, v1[g] & 0x00f000f0u, h1 & 0x00f000f0u, q0, q1);
-                mma_16816(o[nt][2 * g], v0[g] & 0x000f000fu, h0 & 0x000f000fu, v1[g] & 0x000f000fu, h1 & 0x000f000fu, t0, t1);
-                mma_16816(o[nt][2 * g + 1], v0[g] & 0x00f000f0u, h0 & 0x00f000f0u, v1[g] & 0x00f000f0u, h1 & 0x00f000f0u, t0, t1);
+                t0[g] = rest_half2(p0, l[0], sa[g], q0), t1[g] = rest_half2(p1, l[1], sb[g], q1);
+            }
+            mma_16816(low[nt], ma, 0u, mb, 0u, l[0], l[1]);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const uint32_t h0 = v0[g] >> 8, h1 = v1[g] >> 8;
+                mma_16816(o[nt][2 * g], v0[g] & 0x000f000fu, h0 & 0x000f000fu, v1[g] & 0x000f000fu, h1 & 0x000f000fu, t0[g], t1[g]);
+                mma_16816(o[nt][2 * g + 1], v0[g] & 0x00f000f0u, h0 & 0x00f000f0u, v1[g] & 0x00f000f0u, h1 & 0x00f000f0u, t0[g], t1[g]);
             }
         }
     }
