@@ -51,15 +51,10 @@ constexpr int STAGES = 2;            // pairs of tiles in a warp's ring
 constexpr int MAX_CLUSTER = 8;
 constexpr float LOWEST = -3.0e38f;   // reference of a result without tokens: finite, so that no difference of infinities is formed
 
-template <class T> __device__ __forceinline__ float2 to_float2(uint32_t v);
-template <> __device__ __forceinline__ float2 to_float2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
-template <> __device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
 template <class T> __device__ __forceinline__ T from_float(float v);
 // (a result is a mean of values within fp16's range: what the sums' rounding puts beyond it is not infinity; NaN stays)
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v > 65504.f ? 65504.f : v < -65504.f ? -65504.f : v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // e in -126 .. 127
 
 // Shared memory by the offset in the CTA's dynamic part: a pointer that may be null loses its address space, and generic loads with 64-bit
 // arithmetic cost a tenth of the instructions of a tile.
@@ -207,8 +202,8 @@ __device__ __forceinline__ void Rows<G, NT>::load(const Kv4AttnArgs& a, const Re
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100);  // 2^e <= top < 2^(e + 1)
-        const float up = power_of_two(min(9 - e, 127));
+        const int e = query_exponent(top);
+        const float up = query_scaling(e);
         float sums[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) {

@@ -1,4 +1,4 @@
-// Layout of the paged cache held in 4 bits, shared by the kernels that write it and those that read it.
+// Layout of the paged cache held in 4 bits, shared by the kernels that write it and those that read it, and what the latter share besides.
 //
 // The cache is [pages][kv_heads][page_size][40 G] bytes, G = ceil(head_dim / 32) groups of 32 values, page_size a multiple
 // of 16.  The bytes of one (page, head) are page_size / 16 tiles of 16 tokens (a tile is what one warp feeds to the matrix
@@ -11,6 +11,7 @@
 // it has to hold for mma.m16n8k16, in 16-byte pieces that the warp reads without gaps; and a token's codes are whole
 // 16-bit halves, so that tokens can be written one by one, by different warps, without reading first.
 #pragma once
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
 
@@ -35,6 +36,15 @@ __host__ __device__ constexpr int kv4_value_half(int G, int token, int dim) {
 __host__ __device__ constexpr int kv4_param(int G, int token, int which, int g) {  // which: 0 key scale, 1 key minimum, 2 value scale, 3 value minimum
     return 512 * G + token * 8 * G + (which * G + g) * 2;
 }
+
+// ---- queries, as both attention kernels take them
+template <class T> __device__ __forceinline__ float2 to_float2(uint32_t v);
+template <> __device__ __forceinline__ float2 to_float2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+template <> __device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // e in -126 .. 127
+// A row of queries whose largest is `top` becomes fp16 numbers of at most 2^10 by the power of two query_scaling(e): 2^e <= top < 2^(e + 1)
+__device__ __forceinline__ int query_exponent(float top) { return max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100); }
+__device__ __forceinline__ float query_scaling(int e) { return power_of_two(min(9 - e, 127)); }
 
 // status word of this unit on the current device (CF status 8: a page or slot outside the cache)
 constexpr int ST_BAD_SLOT = 8;

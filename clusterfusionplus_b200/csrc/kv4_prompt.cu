@@ -101,9 +101,6 @@ __device__ __forceinline__ void tmem_store(uint32_t at, const float (&x)[16]) {
 }
 
 // ------------------------------------------------------------------------------------------------ numbers
-template <class T> __device__ __forceinline__ float2 to_float2(uint32_t v);
-template <> __device__ __forceinline__ float2 to_float2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
-template <> __device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
 template <class T> __device__ __forceinline__ uint32_t pack(float a, float b);
 // (a result is a mean of values within fp16's range: what the sums' rounding puts beyond it is not infinity; NaN stays)
 template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
@@ -114,7 +111,6 @@ template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, flo
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // e in -126 .. 127
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 __device__ __forceinline__ uint32_t as_word(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 
@@ -259,8 +255,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const Kv4AttnArg
                     }
                 }
                 // a power of two takes the row to at most 2^10 (exact; bf16 reaches beyond fp16), the scale's sign goes along
-                const int e = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100);
-                const float up = copysignf(power_of_two(min(9 - e, 127)), a.scale_log2);
+                const int e = query_exponent(top);
+                const float up = copysignf(query_scaling(e), a.scale_log2);
 #pragma unroll
                 for (int j = 0; j < DP / 16; ++j) {
                     const int d = 16 * j + 8 * half;
