@@ -34,8 +34,8 @@ __device__ __forceinline__ void report_bad_slot() { atomicCAS(&g_kv4_status, 0, 
 // value, four lanes a group.  A warp then moves 2 KB of keys and values with two loads a lane, and the index arithmetic, the
 // group reductions (two shuffles) and the parameters' divisions are paid once for 64 values.  Both are bound by integer and
 // comparison instructions, not by memory: 8191 tokens of 8 heads of 128 in bf16, 88 MB both ways and 13.6 us at the copy bandwidth,
-// take 26.2 us together on the GPU (append: ALU 61 % of its rate, issue slots 69 %; read: 57 %, 68 %).  740 resident CTAs that go through
-// their items with the next one's loads in flight took 27.7 us.
+// take 28.7 us together on the GPU, 20.4 and 8.7 alone (append: ALU 61 % of its rate, issue slots 70 %; read: 58 %, 69 %).  740 resident CTAs that go through
+// their items with the next one's loads in flight took 5 % more.
 constexpr int CT = 256;          // threads of a CTA
 constexpr int ITEMS = CT / 16;   // (token, head) pairs of a CTA
 

@@ -14,7 +14,7 @@
 //  - 1 thread issues the products: S of the next tile before P V of this one, so that they run under the softmax.
 // Every wait is bounded; one that runs out ends the kernel with a device status.
 // Measured: chunks of 267, 723 and 985 queries over 267, 3514 and 3954 tokens, 32 heads over 8 of 128: 202 us, 465 TFLOP/s of products
-// (28 % of the measured rate of large products).  The softmax warps are the chain: 3500 clocks a tile, 2400 of them arithmetic, 450 for
+// (28 % of the measured rate of large products); in fp16 205 us.  The softmax warps are the chain: 3500 clocks a tile, 2400 of them arithmetic, 450 for
 // the agreement of a row's two threads, the rest waits that find their event already there; the unpacking warps need as many, and what makes
 // one of them faster (a hardware barrier for the agreement, half the commits, no bank conflicts, look-ups moved) slows the others: 202 to 210.  One
 // thread a row took 234 us, 256 rows a CTA (each unpacked tile used twice, at half the warps a row) 246 us.

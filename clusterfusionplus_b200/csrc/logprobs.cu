@@ -7,8 +7,8 @@
 // fp32's relative precision.  The floor is reading the logits once; one exponential an element comes second (2047 rows of
 // 50304: 32 us of reading, 23 us of MUFU).  One CTA takes a row, or a cluster of CTAs a row when there are few rows: the partial
 // results meet in distributed shared memory, so there is no workspace and no second launch.  Measured on the GPU: 2047 rows of 50304 in
-// fp16 with the top 20 56 us (3.65 TB/s, 57 % of the copy bandwidth; issue slots 73 %, exponentials 51 %, memory 48 %: 14 instructions an
-// element; without the top k 43 us); one row of 50304 in fp32 with the top 5 7.1 us.
+// fp16 with the top 20 58 us (3.55 TB/s, 55 % of the copy bandwidth; issue slots 72 %, exponentials 50 %, memory 47 %: 14 instructions an
+// element; without the top k 46 us), in fp32 101 us (72); one row of 50304 in fp32 with the top 5 7.2 us.
 //
 // The top k (at most 32) cost a quarter more: every thread remembers its greatest element.  Of 32 or 64 groups of threads, the k-th
 // greatest group maximum bounds the k-th greatest element from below (k groups hold one each), and only a thread whose own greatest
