@@ -50,6 +50,7 @@ namespace {
 constexpr int W = 4;                 // warps of a CTA
 constexpr int STAGES = 2;            // pairs of tiles in a warp's ring
 constexpr int MAX_CLUSTER = 8;
+constexpr int RUN = 8;               // pairs of tiles that a warp sums up before it puts the sums by (16: half the cost, twice the error)
 constexpr float LOWEST = -3.0e38f;   // reference of a result without tokens: finite, so that no difference of infinities is formed
 
 template <class T> __device__ __forceinline__ T from_float(float v);
@@ -251,16 +252,19 @@ __device__ __forceinline__ void Rows<G, NT>::load(const Kv4AttnArgs& a, const Re
 }
 
 // ---------------------------------------------------------------------------------------------------- accumulators
-template <int G, int NT> struct Acc {
+template <int G, int NT, bool PUT_BY> struct Acc {
     static constexpr int DP = 32 * G, LINE = DP + 4;
     float o[NT][2 * G][4];  // numerators in units of 2^-24 and 2^-20
     float low[NT][4];       // row g: group g's sum of p times the minimum; row G: the sum of p
     float m[NT][2];         // reference of a column: p = 2^(score - m), at most 2^room
+    float den[NT][2];       // what low's row G was before the last put_by
+    uint32_t kept;          // where this lane's numerators are that were put by, in shared memory
+    bool any_kept;
     float room;
     uint32_t wide;          // 2^(15 - room) twice, fp16: no scale of a token that some row sees is larger
     bool first_tile;
 
-    __device__ __forceinline__ void reset() {
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -269,10 +273,68 @@ template <int G, int NT> struct Acc {
                 for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) low[nt][j] = 0.f;
-            m[nt][0] = m[nt][1] = 0.f;
         }
-        first_tile = true;
+    }
+    __device__ __forceinline__ void reset(uint32_t keep_at) {  // of this warp: keep_bytes()
+        clear();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = den[nt][0] = den[nt][1] = 0.f;
+        first_tile = true, any_kept = false;
         room = 13.f, wide = 0x44004400u;
+        kept = keep_at + (threadIdx.x & 31) * 16;
+    }
+    // eight numerators of this lane, of group g: its columns 2 t and 2 t + 1 in turn, four of o[2 g] and four of o[2 g + 1]
+    __device__ __forceinline__ void numerators(int nt, int g, float (&x)[8]) const {
+        const int t = threadIdx.x & 3;
+        const float least[2] = {__shfl_sync(0xffffffffu, low[nt][0], g * 4 + t), __shfl_sync(0xffffffffu, low[nt][1], g * 4 + t)};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[j] = fmaf(o[nt][2 * g][j], 16777216.f, least[j & 1]);
+            x[4 + j] = fmaf(o[nt][2 * g + 1][j], 1048576.f, least[j & 1]);
+        }
+    }
+    // Numerators that are put by: of each (nt, g) two times four, a lane's next to the other lanes'
+    static __host__ __device__ constexpr int keep_bytes() { return PUT_BY ? NT * G * 2 * 32 * 16 : 0; }
+    __device__ __forceinline__ float4& place(int nt, int g, int half) const { return *reinterpret_cast<float4*>(smem + kept + ((nt * G + g) * 2 + half) * 512); }
+    __device__ __forceinline__ void add_kept(int nt, int g, float (&x)[8]) const {
+        const float4 a = place(nt, g, 0), b = place(nt, g, 1);
+        x[0] += a.x, x[1] += a.y, x[2] += a.z, x[3] += a.w, x[4] += b.x, x[5] += b.y, x[6] += b.z, x[7] += b.w;
+    }
+    __device__ __forceinline__ void keep(int nt, int g, const float (&x)[8]) const {
+        place(nt, g, 0) = make_float4(x[0], x[1], x[2], x[3]);
+        place(nt, g, 1) = make_float4(x[4], x[5], x[6], x[7]);
+    }
+    // The matrix instructions cut their sums off, by up to 2^-23 at each step, and the codes' and the minima's sums, which nearly cancel in the
+    // result, each grow to some hundred times of it: 64 requests of 8192 tokens were off by 1.4e-3, of 131072 by 4e-2 (even probabilities).  So after every
+    // RUN pairs of tiles their sum is added, rounded to nearest, to numbers in shared memory: 0.3e-3 and 0.7e-3, for 2 % of the time.
+    __device__ __forceinline__ void put_by() {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                float x[8];
+                numerators(nt, g, x);
+                if (any_kept) add_kept(nt, g, x);
+                keep(nt, g, x);
+            }
+            den[nt][0] += low[nt][0], den[nt][1] += low[nt][1];
+        }
+        any_kept = true;
+        clear();
+    }
+    __device__ __forceinline__ void scale_kept(const float (&by)[NT][2]) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                add_kept(nt, g, x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] *= by[nt][j & 1];
+                keep(nt, g, x);
+            }
+            den[nt][0] *= by[nt][0], den[nt][1] *= by[nt][1];
+        }
     }
     template <int K> __device__ __forceinline__ void make_room(const uint32_t (&scales)[K]);
     template <int K> __device__ __forceinline__ void step(const int (&tile)[K], int token, const Rows<G, NT>& r, int lane);
@@ -280,9 +342,9 @@ template <int G, int NT> struct Acc {
 };
 
 // scales beyond `wide` among the warp's: room for the greatest of them (one that is not finite makes its group NaN anyway)
-template <int G, int NT>
+template <int G, int NT, bool PUT_BY>
 template <int K>
-__device__ __forceinline__ void Acc<G, NT>::make_room(const uint32_t (&scales)[K]) {
+__device__ __forceinline__ void Acc<G, NT, PUT_BY>::make_room(const uint32_t (&scales)[K]) {
     uint32_t most = 0;
 #pragma unroll
     for (int u = 0; u < K; ++u) {
@@ -297,9 +359,9 @@ __device__ __forceinline__ void Acc<G, NT>::make_room(const uint32_t (&scales)[K
 }
 
 // K tiles of 16 tokens in a row, the first token of all `token`, the tiles at these offsets of shared memory
-template <int G, int NT>
+template <int G, int NT, bool PUT_BY>
 template <int K>
-__device__ __forceinline__ void Acc<G, NT>::step(const int (&tile)[K], int token, const Rows<G, NT>& r, int lane) {
+__device__ __forceinline__ void Acc<G, NT, PUT_BY>::step(const int (&tile)[K], int token, const Rows<G, NT>& r, int lane) {
     constexpr int PAIRS = (G + 1) / 2;
     const int g8 = lane >> 2, t = lane & 3;
 
@@ -389,6 +451,7 @@ __device__ __forceinline__ void Acc<G, NT>::step(const int (&tile)[K], int token
     }
     if (__any_sync(0xffffffffu, rise)) {
         make_room(scales);
+        float kept_by[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -403,11 +466,13 @@ __device__ __forceinline__ void Acc<G, NT>::step(const int (&tile)[K], int token
 #pragma unroll
                 for (int u = 0; u < K; ++u) x[u][nt][c] -= up, x[u][nt][c + 2] -= up;
                 const float keep = first_tile ? 1.f : ex2(-up);
+                kept_by[nt][c] = keep;
                 low[nt][c] *= keep;
 #pragma unroll
                 for (int q = 0; q < 2 * G; ++q) o[nt][q][c] *= keep, o[nt][q][c + 2] *= keep;
             }
         first_tile = false;
+        if (PUT_BY && any_kept) scale_kept(kept_by);
     }
     // ---- values: scales of tokens 2 t, 2 t + 1 (sa) and 2 t + 8, 2 t + 9 (sb), group by group; minima likewise, of group g8
 #pragma unroll
@@ -485,25 +550,26 @@ __device__ __forceinline__ void Acc<G, NT>::step(const int (&tile)[K], int token
 }
 
 // this warp's result: COLS lines of DP numerators, reference and denominator
-template <int G, int NT> __device__ __forceinline__ void Acc<G, NT>::store(float* lines) const {
+template <int G, int NT, bool PUT_BY> __device__ __forceinline__ void Acc<G, NT, PUT_BY>::store(float* lines) const {
     const int lane = threadIdx.x & 31, g8 = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             float* line = lines + (nt * 8 + 2 * t + c) * LINE;
-            const float sum = __shfl_sync(0xffffffffu, low[nt][c], G * 4 + t);
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const float least = __shfl_sync(0xffffffffu, low[nt][c], g * 4 + t);
-                float4 y;
-                y.x = fmaf(o[nt][2 * g][c], 16777216.f, least);
-                y.y = fmaf(o[nt][2 * g + 1][c], 1048576.f, least);
-                y.z = fmaf(o[nt][2 * g][c + 2], 16777216.f, least);
-                y.w = fmaf(o[nt][2 * g + 1][c + 2], 1048576.f, least);
-                *reinterpret_cast<float4*>(line + 32 * g + 4 * g8) = y;
-            }
+            const float sum = __shfl_sync(0xffffffffu, low[nt][c] + den[nt][c], G * 4 + t);
             if (g8 == 0) line[DP] = sum == 0.f ? LOWEST : m[nt][c], line[DP + 1] = sum;  // nothing seen: no reference either
+        }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            float x[8];
+            numerators(nt, g, x);
+            if (PUT_BY && any_kept) add_kept(nt, g, x);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                *reinterpret_cast<float4*>(lines + (nt * 8 + 2 * t + c) * LINE + 32 * g + 4 * g8) = make_float4(x[c], x[4 + c], x[2 + c], x[6 + c]);
         }
 }
 
@@ -568,7 +634,7 @@ template <int G> struct Feed {
         cp_async_commit();
     }
     // waits for the next pair and gives it to `acc`; `token`: its first
-    template <int NT> __device__ __forceinline__ void take(Acc<G, NT>& acc, int token, const Rows<G, NT>& rows) {
+    template <int NT, bool PUT_BY> __device__ __forceinline__ void take(Acc<G, NT, PUT_BY>& acc, int token, const Rows<G, NT>& rows) {
         cp_async_wait<STAGES - 2>();
         __syncwarp();
         const int tile = static_cast<int>(ring + out * 2 * TB);
@@ -580,6 +646,12 @@ template <int G> struct Feed {
         else if (both == 2u) acc.template step<1>({tile + TB}, token + KV4_TILE, rows, lane);
     }
 };
+
+// shared memory of the rings, and in their place later the warps' results; what is put by lies behind
+template <int G, int NT> __host__ __device__ constexpr int shared_bytes() {
+    constexpr int ring = W * STAGES * 2 * kv4_tile_bytes(G), merge = W * 8 * NT * (32 * G + 4) * 4;
+    return ring > merge ? ring : merge;
+}
 
 // The results of the CTA's warps for element e = (column, dim), joined: numerator, denominator, reference
 template <int G, int NT> __device__ __forceinline__ void join_warps(const float* lines, int c, int d, float& num, float& den, float& top) {
@@ -597,16 +669,17 @@ template <int G, int NT> __device__ __forceinline__ void join_warps(const float*
 }
 
 // ---------------------------------------------------------------------------------------------------- little work
-template <class T, int G, int NT>
-__global__ void __launch_bounds__(32 * W, NT == 1 ? 4 : 2) kv4_few_kernel(const Kv4AttnArgs a, int cluster) {
+// LONG: no cluster, and sums are put by, in the shared memory that clusters need for what they exchange
+template <class T, int G, int NT, bool LONG>
+__global__ void __launch_bounds__(32 * W, NT == 1 ? 4 : 2) kv4_few_kernel(const Kv4AttnArgs a, int clusters) {
     constexpr int DP = 32 * G, COLS = 8 * NT, LINE = DP + 4;
     // what the CTAs of the cluster send one another: pieces of 128 numerators go to CTA (piece % cluster), every column's reference
     // and denominator to all
     constexpr int PIECES = (COLS * DP + 32 * W - 1) / (32 * W);
-    __shared__ float received[(PIECES + MAX_CLUSTER) * 32 * W];
-    __shared__ float terms[MAX_CLUSTER][COLS][2];
+    __shared__ float received[LONG ? 1 : (PIECES + MAX_CLUSTER) * 32 * W];
+    __shared__ float terms[LONG ? 1 : MAX_CLUSTER][COLS][2];
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = threadIdx.x >> 5, cluster = LONG ? 1 : clusters;
     const int rank = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
     const int item = static_cast<int>(blockIdx.x / cluster), b = item / a.kv_heads, kvh = item - b * a.kv_heads;
     const Request own(a, b);
@@ -621,9 +694,12 @@ __global__ void __launch_bounds__(32 * W, NT == 1 ? 4 : 2) kv4_few_kernel(const 
         const int pairs = feed.begin(own.table, kvh, 0, tiles, unit, units);
         Rows<G, NT> rows;
         rows.template load<T>(a, own, kvh, r0);
-        Acc<G, NT> acc;
-        acc.reset();
-        for (int i = 0; i < pairs; ++i) feed.take(acc, 2 * (unit + i * units) * KV4_TILE, rows);
+        Acc<G, NT, LONG> acc;
+        acc.reset(shared_bytes<G, NT>() + warp * acc.keep_bytes());
+        for (int i = 0; i < pairs; ++i) {
+            feed.take(acc, 2 * (unit + i * units) * KV4_TILE, rows);
+            if (LONG && i % RUN == RUN - 1) acc.put_by();
+        }
         cp_async_wait<0>();
         __syncthreads();  // the rings are free
         float* lines = reinterpret_cast<float*>(smem);
@@ -705,7 +781,8 @@ __device__ __forceinline__ long long block_sum_before(long long v, long long* to
 template <class T, int G, int NT>
 __global__ void __launch_bounds__(32 * W, NT == 1 ? 4 : 2) kv4_line_kernel(const Kv4AttnArgs a, int least) {
     constexpr int DP = 32 * G, COLS = 8 * NT, LINE = DP + 4;
-    __shared__ long long sums[W], found[2];
+    // all shared memory is dynamic: four CTAs with what they put by take an SM's to the last byte.  Where the rings will be:
+    long long *sums = reinterpret_cast<long long*>(smem), *found = sums + W;
     const int tid = threadIdx.x, warp = tid >> 5;
     asm volatile("griddepcontrol.launch_dependents;");  // the join may be set up; it waits for this grid's end by itself
 
@@ -737,6 +814,7 @@ __global__ void __launch_bounds__(32 * W, NT == 1 ? 4 : 2) kv4_line_kernel(const
     __syncthreads();
     int b = static_cast<int>(found[0]);
     long long base = found[1];  // of request b in the line
+    __syncthreads();
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + cuts_bytes(gridDim.x)) + static_cast<long long>(blockIdx.x) * 2 * COLS * LINE;
     float* lines = reinterpret_cast<float*>(smem);  // the warps' results, where the rings are
 
@@ -763,9 +841,12 @@ __global__ void __launch_bounds__(32 * W, NT == 1 ? 4 : 2) kv4_line_kernel(const
         const int pairs = feed.begin(own.table, kvh, from, own.before + own.rows / own.per <= 0 ? from : to, warp, W);
         Rows<G, NT> rows;
         rows.template load<T>(a, own, kvh, r0);
-        Acc<G, NT> acc;
-        acc.reset();
-        for (int i = 0; i < pairs; ++i) feed.take(acc, (from + 2 * (warp + i * W)) * KV4_TILE, rows);
+        Acc<G, NT, true> acc;
+        acc.reset(shared_bytes<G, NT>() + warp * acc.keep_bytes());
+        for (int i = 0; i < pairs; ++i) {
+            feed.take(acc, (from + 2 * (warp + i * W)) * KV4_TILE, rows);
+            if (i % RUN == RUN - 1) acc.put_by();
+        }
         cp_async_wait<0>();
         __syncthreads();  // the rings are free
         acc.store(lines + warp * COLS * LINE);
@@ -842,12 +923,25 @@ __global__ void __launch_bounds__(JT) kv4_join_kernel(const Kv4AttnArgs a, int c
 // ---------------------------------------------------------------------------------------------------- launches
 constexpr int SMS = 148;
 constexpr int LEAST = 2 * W;  // tiles of a CTA's piece, at least: below that the join costs more than it saves
+constexpr int DEEP = 4 * RUN;  // tiles that a warp of a cluster sums up at most
 constexpr int places(int nt) { return SMS * (nt == 1 ? 4 : 2); }  // CTAs that find room on the GPU at once: __launch_bounds__ of the kernels
 template <int NT> constexpr int line_ctas() { return places(NT); }
 
+// CTAs to each of `items` (request, head, rows) of up to `tiles` tiles: as many as find room on the GPU at once (a CTA costs 4 us besides its tiles, a
+// tile 0.5 us of a warp: 256 pairs of up to 2048 tokens 19.4 us with 2, 23.8 with 4; of 9 to 16 rows, where half as many find room, 37.9 with 1,
+// 51.6 with 2, and 64 pairs 17.9 with 4, 26.1 with 8), but at least two tiles to a warp.
+int cluster_size(long long items, long long tiles, int nt) {
+    int cluster = 1;
+    while (cluster < MAX_CLUSTER && items * cluster * 2 <= places(nt) && tiles >= 4 * W * cluster) cluster *= 2;
+    return cluster;
+}
+// Sums of more tiles a warp are to be put by, for which a cluster, with what its CTAs exchange, has no shared memory
+bool too_deep(int cluster, long long tiles) { return cluster > 1 && tiles > static_cast<long long>(DEEP) * W * cluster; }
+
 template <class T, int G, int NT> cudaError_t launch(const Kv4AttnArgs& a, long long max_q_len, cudaStream_t st) {
     constexpr int COLS = 8 * NT;
-    constexpr int ring = W * STAGES * 2 * kv4_tile_bytes(G), merge = W * COLS * (32 * G + 4) * 4, smem = ring > merge ? ring : merge;
+    constexpr int smem = shared_bytes<G, NT>(), keep = W * Acc<G, NT, true>::keep_bytes();
+    static_assert((smem + keep + 1024) * (NT == 1 ? 4 : 2) <= 228 * 1024, "the CTAs of an SM");
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[1];
     cfg.blockDim = dim3(32 * W);
@@ -856,10 +950,10 @@ template <class T, int G, int NT> cudaError_t launch(const Kv4AttnArgs& a, long 
     if (a.workspace) {
         constexpr int ctas = line_ctas<NT>();
         static std::atomic<unsigned long long> allowed{0};
-        cudaError_t e = allow_shared_once(reinterpret_cast<const void*>(kv4_line_kernel<T, G, NT>), smem, allowed);
+        cudaError_t e = allow_shared_once(reinterpret_cast<const void*>(kv4_line_kernel<T, G, NT>), smem + keep, allowed);
         if (e != cudaSuccess) return e;
         cfg.gridDim = dim3(ctas);
-        cfg.dynamicSmemBytes = smem;
+        cfg.dynamicSmemBytes = smem + keep;
         e = cudaLaunchKernelEx(&cfg, kv4_line_kernel<T, G, NT>, a, LEAST);
         if (e != cudaSuccess) return e;
         cfg.gridDim = dim3(ctas - 1);
@@ -873,21 +967,20 @@ template <class T, int G, int NT> cudaError_t launch(const Kv4AttnArgs& a, long 
     const long long items = static_cast<long long>(a.batch) * a.kv_heads;
     const long long q_tiles = (max_q_len * (a.heads / a.kv_heads) + COLS - 1) / COLS;
     const long long tiles = (a.table_width * a.page + KV4_TILE - 1) / KV4_TILE;
-    // As many CTAs to a (request, head) as find room on the GPU at once (a CTA costs 4 us besides its tiles, a tile 0.5 us of a
-    // warp: 256 pairs of up to 2048 tokens 19.4 us with 2, 23.8 with 4; of 9 to 16 rows, where half as many find room, 37.9 with 1, 51.6 with
-    // 2, and 64 pairs 17.9 with 4, 26.1 with 8), but at least two tiles to a warp
-    int cluster = 1;
-    while (cluster < MAX_CLUSTER && items * q_tiles * cluster * 2 <= places(NT) && tiles >= 4 * W * cluster) cluster *= 2;
-    static std::atomic<unsigned long long> allowed{0};
-    const cudaError_t e = allow_shared_once(reinterpret_cast<const void*>(kv4_few_kernel<T, G, NT>), smem, allowed);
+    int cluster = cluster_size(items * q_tiles, tiles, NT);
+    if (too_deep(cluster, tiles)) cluster = 1;  // only without a workspace
+    const bool put_by = cluster == 1 && tiles > 2 * RUN * W;
+    static std::atomic<unsigned long long> allowed[2] = {{0}, {0}};
+    const auto kernel = put_by ? kv4_few_kernel<T, G, NT, true> : kv4_few_kernel<T, G, NT, false>;
+    const cudaError_t e = allow_shared_once(reinterpret_cast<const void*>(kernel), smem + (put_by ? keep : 0), allowed[put_by]);
     if (e != cudaSuccess) return e;
     cfg.gridDim = dim3(static_cast<unsigned>(items * cluster), static_cast<unsigned>(q_tiles < 65535 ? q_tiles : 65535));
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = smem + (put_by ? keep : 0);
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = cluster;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kv4_few_kernel<T, G, NT>, a, cluster);
+    return cudaLaunchKernelEx(&cfg, kernel, a, cluster);
 }
 
 template <class T, int G> cudaError_t by_rows(const Kv4AttnArgs& a, long long max_q_len, cudaStream_t st) {
@@ -917,11 +1010,12 @@ long long kv4_few_workspace(long long heads, long long kv_heads, int D, long lon
 // tokens 21 : 34, x 16384 16 : 19, x 8192 13 : 12).  With 9 to 16 rows a pair takes twice as long and half as many CTAs find room: there more
 // pairs than places keep the GPU even by themselves (1024 pairs of up to 8192 tokens 359 : 288, 512 pairs 187 : 152), and the line pays for
 // fewer and long ones only (256 pairs of up to 16384 163 : 213, of up to 8192 122 : 112; 128 pairs of up to 16384 88 : 113; 16 pairs x 16384
-// 31 : 37, 32 pairs 44 : 39).
+// 31 : 37, 32 pairs 44 : 39).  And it takes what clusters must not sum up (too_deep).
 bool kv4_few_uses_workspace(long long batch, long long heads, long long kv_heads, long long tokens, long long max_q_len) {
     const long long rows = max_q_len * (heads / kv_heads), cols = rows <= 8 ? 8 : 16;
     const long long items = batch * kv_heads * ((rows + cols - 1) / cols), tiles = (tokens + KV4_TILE - 1) / KV4_TILE;
     const bool few = items * MAX_CLUSTER < places(cols / 8) / 2;
+    if (too_deep(cluster_size(items, tiles, static_cast<int>(cols / 8)), tiles)) return true;
     if (cols == 8) return items * tiles >= 100000 || (few && tiles >= 640);
     return tiles >= 640 && (few || (items <= places(2) && items * tiles >= 100000));
 }

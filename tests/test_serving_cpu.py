@@ -269,7 +269,7 @@ def test_a_build_for_another_torch_is_out_of_date(monkeypatch):
 
 
 @pytest.mark.parametrize("batch,tokens,q,line", [
-    (64, 8192, 1, True), (1, 16384, 1, True), (4, 16384, 1, True), (32, 4096, 1, False), (16, 1000, 8, False),          # up to 8 rows: 592 CTAs at once
+    (64, 8192, 1, True), (1, 16384, 1, True), (4, 16384, 1, True), (32, 4096, 1, False), (16, 1000, 8, False), (20, 4096, 1, False), (20, 4112, 1, True),   # up to 8 rows: 592 CTAs at once
     (1, 16384, 12, True), (2, 16384, 12, True), (4, 16384, 12, False), (32, 8192, 12, False), (32, 16384, 12, True), (16, 16384, 12, True), (64, 16384, 12, False)])   # 9 to 16: 296
 def test_the_line_is_taken_where_it_was_measured_faster(batch, tokens, q, line):
     """8 cached heads of 128, one query head each: room for half as many CTAs with 9 to 16 query rows moves the bounds."""

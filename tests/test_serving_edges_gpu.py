@@ -507,3 +507,26 @@ def test_attention_of_a_mixed_step_in_two_calls(cuda_device, n):
     assert (out[starts[-1]:] == 7).all()
     K, V = S.unpack(cache, D)
     near(out[:starts[-1]], S.attention(q[:starts[-1]], K, V, table, lens, starts, D ** -0.5))
+
+
+@pytest.mark.parametrize("D,heads,kv_heads,B,T,rows", [(64, 2, 2, 256, 16384, 1), (128, 4, 1, 600, 8192, 3), (128, 2, 2, 150, 4096, 1), (64, 1, 1, 1, 200000, 1)])
+@pytest.mark.parametrize("way", ["rule", "no workspace"])
+@pytest.mark.parametrize("size", [0.05, 1.0])
+def test_attention_of_long_requests_in_a_full_batch(cuda_device, monkeypatch, D, heads, kv_heads, B, T, rows, way, size):
+    """Hundreds of tiles for each warp, next to even probabilities: the sums are a few hundred times the result, and cutting off each of their steps must
+    not show in it.  All requests name the same pages."""
+    import clusterfusionplus_b200 as cf
+    from clusterfusionplus_b200 import serving
+    if way == "no workspace":
+        monkeypatch.setattr(serving, "_workspace", 0)
+    g = torch.Generator(device=DEV).manual_seed(T + B)
+    key, value = (torch.randn(T, kv_heads, D, device=DEV, generator=g).half() for _ in range(2))
+    q = (torch.randn(B * rows, heads, D, device=DEV, generator=g) * size).half()
+    cache = cf.kv4_cache(-(-T // 64), kv_heads, 64, D)
+    cf.kv4_append(key, value, torch.arange(T, device=DEV, dtype=torch.int32), cache)
+    table = torch.arange(-(-T // 64), device=DEV, dtype=torch.int32)[None].repeat(B, 1)
+    got = cf.kv4_attention(q, cache, table, ints([T] * B), ints([rows * b for b in range(B + 1)]), max_q_len=rows)
+    K, V = S.unpack(cache, D)
+    for b in {0, B // 3, B - 1}:
+        at = slice(b * rows, (b + 1) * rows)
+        near(got[at], S.attention(q[at], K, V, [list(range(-(-T // 64)))], [T], [0, rows], D ** -0.5))
