@@ -29,10 +29,10 @@
 //    lengths keep every SM busy to the end; what a cut divides goes to a workspace and a second launch joins it.
 // Each warp streams its tiles through its own ring of shared memory by cp.async.
 //
-// Measured on the GPU: one request of 4096 tokens, 32 heads of 128 (21 MB, 3.3 us of reading), 11.3 us: a CTA's queries, first loads
+// Measured on the GPU: one request of 4096 tokens, 32 heads of 128 (21 MB, 3.3 us of reading), 11.2 us: a CTA's queries, first loads
 // and the joining take 4 us.  64 requests of up to 8192 tokens, 8 cached heads under 32 (350 MB, 54 us): line and
-// join 96 us (3.7 TB/s; the join alone takes 9 us, most of them under the line's end).  No unit is full: ~380 instructions a tile fill 57 % of the
-// issue slots (ALU 45 %, memory 46 %, matrix pipe 32 % of their rates), because the chain of a tile, load to last product, is waited for with 4
+// join 97 us (3.6 TB/s; the join alone takes 8 us, most of them under the line's end).  No unit is full: ~390 instructions a tile fill 57 % of the
+// issue slots (ALU 45 %, memory 45 %, matrix pipe 32 % of their rates), because the chain of a tile, load to last product, is waited for with 4
 // warps a scheduler, which is what 128 registers leave.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
