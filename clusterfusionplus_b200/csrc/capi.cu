@@ -289,7 +289,7 @@ int pick_cfg(DeviceState& ds, int D) {
     if (cap > 0 && cap < best_cov) best_cov = (cap / best_cs) * best_cs;
     c.cs = best_cs;
     c.grid = best_cov;
-    c.coop = env_int("CFB200_COOPERATIVE", 1) != 0;
+    c.coop = cf_host_cooperative();
     c.ready = true;
     return CF_OK;
 }
@@ -796,6 +796,7 @@ int noalloc_setup(NoAllocDevice** out) {
 
 // ---- helpers shared with the other translation units (host_common.h)
 CfEncodeTiledFn cf_host_encode_fn() { return get_encode(); }
+bool cf_host_cooperative() { return env_int("CFB200_COOPERATIVE", getenv("NV_NSIGHT_INJECTION_TRANSPORT_TYPE") ? 0 : 1) != 0; }
 int cf_host_fail(int code, const char* fmt, ...) {
     char buf[512];
     va_list ap;
