@@ -7,7 +7,10 @@ ClusterFusion++, behind the reference's `clusterfusion` operator API.
 Everything computes in libclusterfusion_b200.so (hand-written CUDA); importing
 this package fails if that library has not been built.
 """
-from ._lib import CF_PYTHIA_2B8, CF_PYTHIA_6B9, CfDims, LIB_PATH  # noqa: F401
+from ._lib import (  # noqa: F401
+    CF_OUT_FP32, CF_PLAN_BAD_LENGTH, CF_PLAN_BAD_PAGE, CF_PLAN_MAX_ROWS, CF_PLAN_MAX_TOKENS, CF_PLAN_NO_PAGES, CF_PLAN_TABLE_WIDTH,
+    CF_PYTHIA_2B8, CF_PYTHIA_6B9, CfDims, LIB_PATH,
+)
 from .api import (  # noqa: F401
     device_status, launch_info, llama_decoder_layer, llama_decoder_layer_batch_decode_sglang, llama_decoder_layer_sglang,
     llama_mlp_batch_sglang, llama_mlp_sglang, model_dims,

@@ -275,3 +275,14 @@ def test_the_line_is_taken_where_it_was_measured_faster(batch, tokens, q, line):
     """8 cached heads of 128, one query head each: room for half as many CTAs with 9 to 16 query rows moves the bounds."""
     from clusterfusionplus_b200._lib import lib
     assert (lib.cf_kv4_attention_workspace(batch, 8, 8, 128, tokens, q) > 0) == line
+
+
+def test_the_plan_s_status_bits_have_names():
+    """Those of the C header, in the package and its drop-in name."""
+    import re
+
+    import clusterfusion
+    import clusterfusionplus_b200 as cf
+    header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "clusterfusion_b200.h")).read()
+    bits = re.findall(r"#define (CF_PLAN_[A-Z_]+) (\d+)", header)
+    assert len(bits) == 6 and all(getattr(cf, n) == int(v) == getattr(clusterfusion, n) for n, v in bits)
