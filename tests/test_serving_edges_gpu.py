@@ -530,3 +530,22 @@ def test_attention_of_long_requests_in_a_full_batch(cuda_device, monkeypatch, D,
     for b in {0, B // 3, B - 1}:
         at = slice(b * rows, (b + 1) * rows)
         near(got[at], S.attention(q[at], K, V, [list(range(-(-T // 64)))], [T], [0, rows], D ** -0.5))
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("rows", [1, 5, 40])
+def test_attention_of_queries_that_are_not_finite(cuda_device, schedule, bad, rows):
+    """They make their own row and head NaN; every other result keeps its bits."""
+    import clusterfusionplus_b200 as cf
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    key, value = (torch.randn(600, 2, 64, device=DEV, generator=g).half() for _ in range(2))
+    cache, table, lens, starts = cf.kv4_cache(38, 2, 16, 64), ints([list(range(38))]), ints([600]), ints([0, rows])
+    cf.kv4_append(key, value, ints(list(range(600))), cache)
+    q = torch.randn(rows, 8, 64, device=DEV, generator=g).half()
+    want = cf.kv4_attention(q, cache, table, lens, starts, max_q_len=rows)
+    q[rows // 2, 3, 7] = bad
+    got = cf.kv4_attention(q, cache, table, lens, starts, max_q_len=rows)
+    assert got[rows // 2, 3].isnan().all()
+    same = got == want
+    same[rows // 2, 3] = True
+    assert same.all()
